@@ -44,6 +44,14 @@ SIGNATURES: dict[str, tuple] = {
     "hs_verify_attention_noalloc_scratch_bytes": (_sz, []),
     "hs_store_kvcache": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i64,
                                 _i64, _f32, _f32, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "hs_store_kvcache_scaled": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64,
+                                       _i64, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i32, _i32,
+                                       _i32, _i32, _i32, _vp]),
+    "hs_verify_attention_scaled_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "hs_verify_attention_scaled": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp,
+                                          _i64, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp,
+                                          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp,
+                                          _i64, _i64, _vp, _sz, _vp]),
 }
 
 

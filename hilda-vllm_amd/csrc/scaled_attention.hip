@@ -1,0 +1,688 @@
+// Attention over an 8-bit (e4m3fn) paged KV cache with one f32 scale per group of
+// tokens and kv head (written by scaled_kv.hip): decode, verify and prompt rows,
+// causal with bottom-right alignment (query token i of a sequence with Lq queries
+// and Lk keys sees keys 0 .. Lk - Lq + i), grouped heads, head size 128:
+//   s_ij = softmax_scale * ks[g(j)] * <q_i, kc_j>
+//   o_i  = sum_j p_ij vs[g(j)] vc_j / sum_j p_ij,  p_ij = exp(s_ij - max_j s_ij)
+// Codes are decoded exactly to bf16 (every e4m3 value is one) and multiplied on
+// the matrix cores with f32 accumulation; a window of 32 keys lies in one group,
+// so its scales are two scalars: ks joins the softmax scale, vs the
+// probabilities, which round to bf16 once, as the product's second operand.
+// Statistics, sums and partial results are f32.
+//
+// A wave works on its own, without LDS in its loop. It takes a window's K rows as
+// the A operand of S^T = K Q^T (lane l: key l % 16, dims 32 (l / 16) .. + 31, two
+// 16-byte loads) and its V rows as 8 keys x 8 dims a lane (8 loads of 8 bytes, 16
+// lanes to a cache line); byte permutes transpose those 8 x 8 codes in registers
+// into the A operand of O^T = V^T P^T, whose key order is chosen so that the lane's
+// own probabilities are its B operand. The next window is loaded while this one is
+// computed.
+//
+//  * k_scaled_split: decode and verify rows, 16 query rows (head of the kv head's
+//    group, token) to a tile. A workgroup of 8 waves takes `split_len` keys of a
+//    (sequence, kv head, tile), its waves interleaved over the windows, and joins
+//    their results in LDS; k_scaled_combine joins the splits' partials. The partials
+//    are written before they are read and nothing is counted between the launches,
+//    so the workspace needs no preparation.
+//  * k_scaled_rows: prompts. A wave takes 16 QT query rows and all of their keys.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/hilda_spec.h"
+#include "hs_model_dev.h"
+
+namespace hs {
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kD = 128;    // head size
+constexpr int kWin = 32;   // keys of a window
+constexpr int kRows = 16;  // query rows of a tile
+constexpr int kSplitWaves = 8;
+constexpr int kRowWaves = 4;
+
+struct ScaledAttnArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  int64_t c_sb, c_st, c_sh;
+  const float* ks;
+  const float* vs;
+  int64_t s_sb, s_sg, s_sh;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_width, num_blocks;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int Hkv, G, block_size;
+  int bs_shift;  // log2(block_size) for powers of two, else -1
+  int g_shift;   // log2(group)
+  float scale_log2;  // softmax_scale * log2(e)
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  int qtiles, nsplit, split_len;
+  float* part_o;   // [sequence, kv head, tile, split][16][128]
+  float* part_ml;  // [sequence, kv head, tile, split][16][2]
+};
+
+// Sequence b's bounds, clamped so that a call's odd lengths never index out of it.
+struct Seq {
+  int qs, Lq, Lk;
+};
+__device__ __forceinline__ Seq seq_of(const ScaledAttnArgs& a, int b) {
+  Seq s;
+  s.qs = a.cu_q[b];
+  s.Lq = a.cu_q[b + 1] - s.qs;
+  s.Lk = a.cu_k[b + 1] - a.cu_k[b];
+  return s;
+}
+
+// keys that row r (of the sequence's Lq * G) sees
+__device__ __forceinline__ int row_keys(const Seq& s, int G, int r) {
+  const int n = s.Lk - s.Lq + r / G + 1;
+  return n < 0 ? 0 : (n > s.Lk ? s.Lk : n);
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, bool high) {
+  const bf16x2_t p = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false);
+  return __builtin_bit_cast(uint32_t, p);
+}
+union Frag {
+  uint32_t u[4];
+  bf16x8_t v;
+};
+__device__ __forceinline__ bf16x8_t decode8(uint32_t lo, uint32_t hi) {
+  Frag f;
+  f.u[0] = bf16_pair(lo, false);
+  f.u[1] = bf16_pair(lo, true);
+  f.u[2] = bf16_pair(hi, false);
+  f.u[3] = bf16_pair(hi, true);
+  return f.v;
+}
+
+// A window as a lane holds it. K: rows l % 16 and 16 + l % 16, 32 bytes each. V: 8
+// bytes (dims 8 (l % 16) ..) of keys 4g + e and 16 + 4g + e, g = l / 16, e < 4.
+struct Win {
+  uint4 k[4];
+  uint2 v[8];
+  float ks, vs;
+};
+
+// Where a window lies: its block's rows and its group's scales; `ok` is false where
+// the table has no such block, and nothing of the window is then used.
+struct Place {
+  int blk;
+  bool ok;
+};
+__device__ __forceinline__ int block_of(const ScaledAttnArgs& a, int key) {
+  return a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
+}
+__device__ __forceinline__ Place place_of(const ScaledAttnArgs& a, const int32_t* bt, int ws) {
+  const int i = block_of(a, ws);
+  Place p;
+  p.ok = i < a.bt_width;
+  p.blk = p.ok ? bt[i] : 0;
+  if (p.blk < 0 || p.blk >= a.num_blocks) p.ok = false, p.blk = 0;
+  return p;
+}
+
+// Loads the window at key ws; keys at and past `hi` re-read the last one below it.
+__device__ __forceinline__ void load_win(const ScaledAttnArgs& a, int head, int lane, int ws,
+                                         int hi, Place p, Win& w) {
+  const int off = ws - block_of(a, ws) * a.block_size;
+  const int64_t base = (int64_t)p.blk * a.c_sb + (int64_t)off * a.c_st + (int64_t)head * a.c_sh;
+  const int64_t sbase =
+      (int64_t)p.blk * a.s_sb + (int64_t)(off >> a.g_shift) * a.s_sg + (int64_t)head * a.s_sh;
+  w.ks = a.ks[sbase];
+  w.vs = a.vs[sbase];
+  const int last = hi - ws - 1;  // >= 0
+  const int c = lane & 15, g = lane >> 4;
+  const int st = (int)a.c_st;  // the host keeps 32 rows within 2 GiB
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int key = min(16 * t + c, last);
+    const uint8_t* p = a.kc + base + (uint32_t)(key * st + 32 * g);
+    w.k[2 * t] = *reinterpret_cast<const uint4*>(p);
+    w.k[2 * t + 1] = *reinterpret_cast<const uint4*>(p + 16);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int key = min((e & 4) * 4 + 4 * g + (e & 3), last);
+    w.v[e] = *reinterpret_cast<const uint2*>(a.vc + base + (uint32_t)(key * st + 8 * c));
+  }
+}
+
+// The V^T operand of dims 8 i + db (i = l % 16), db = 0 .. 7, from the lane's 8 x 8
+// codes; emit(db, operand).
+template <typename F>
+__device__ __forceinline__ void transposed(const uint2 (&v)[8], F emit) {
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // keys (2 p, 2 p + 1) of dims 4 w + 2 h and the next
+      const uint32_t sel = h ? 0x03070206u : 0x01050004u;
+      uint32_t m[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t x = w ? v[2 * p].y : v[2 * p].x, y = w ? v[2 * p + 1].y : v[2 * p + 1].x;
+        m[p] = __builtin_amdgcn_perm(x, y, sel);
+      }
+      Frag f;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) f.u[p] = bf16_pair(m[p], false);
+      emit(4 * w + 2 * h, f.v);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) f.u[p] = bf16_pair(m[p], true);
+      emit(4 * w + 2 * h + 1, f.v);
+    }
+  }
+}
+
+// 0xff in every byte of x that is a NaN code
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
+  const uint32_t t = (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+  return t * 255u;
+}
+
+// The state of 16 QT query rows: per tile the lane's row (l % 16) has its maximum
+// (log2 domain), the lane's part of its sum and O[d = 32 (l / 16) + 8 j + db] in
+// o[db][j].
+template <int QT>
+struct Rows {
+  bf16x8_t q[QT][4];
+  int lim[QT];  // keys that the row sees
+  float m[QT], l[QT];
+  f32x4_t o[QT][8];
+};
+
+template <int QT>
+__device__ __forceinline__ void load_rows(const ScaledAttnArgs& a, const Seq& s, int head, int r0,
+                                          int lane, Rows<QT>& R) {
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = r0 + 16 * t + n;
+    const bool live = r < s.Lq * a.G;
+    R.lim[t] = live ? row_keys(s, a.G, r) : 0;
+    R.m[t] = -INFINITY;
+    R.l[t] = 0.0f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) R.o[t][db] = f32x4_t{0, 0, 0, 0};
+    const uint16_t* p = a.q;
+    if (live)
+      p += (int64_t)(s.qs + r / a.G) * a.q_st + (int64_t)(head * a.G + r % a.G) * a.q_sh + 32 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (live) x = *reinterpret_cast<const uint4*>(p + 8 * i);
+      R.q[t][i] = __builtin_bit_cast(bf16x8_t, x);
+    }
+  }
+}
+
+// One window. kMask: some row may not see some key. A key that a row does not see
+// takes no part in that row, whatever its codes and scales are: its probability is
+// 0, and NaN codes of V, which a zero does not cancel, are taken out of the product
+// and given to the rows that see them by a product of their own.
+template <int QT, bool kMask>
+__device__ __forceinline__ void step(const ScaledAttnArgs& a, const Win& w, int ws, int lane,
+                                     Rows<QT>& R) {
+  const int g = lane >> 4;
+  const float c = a.scale_log2 * w.ks;
+  f32x4_t s[QT][2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 k = w.k[2 * t + (i >> 1)];
+      const bf16x8_t ka = (i & 1) ? decode8(k.z, k.w) : decode8(k.x, k.y);
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        const f32x4_t z = i ? s[u][t] : f32x4_t{0, 0, 0, 0};
+        s[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, R.q[u][i], z, 0, 0, 0);
+      }
+    }
+  }
+  bf16x8_t p[QT];
+  [[maybe_unused]] uint32_t seen[QT];
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    float x[8];
+    if constexpr (kMask) seen[u] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = s[u][e >> 2][e & 3] * c;
+      if constexpr (kMask) {
+        const bool in = ws + (e & 4) * 4 + 4 * g + (e & 3) < R.lim[u];
+        seen[u] |= in ? 1u << e : 0u;
+        x[e] = in ? x[e] : -INFINITY;
+      }
+    }
+    float m = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                    fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    m = fmaxf(R.m[u], quad_max(m));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    if (__any(m > R.m[u])) {
+      const float f = __builtin_amdgcn_exp2f(R.m[u] - ref);
+      R.l[u] *= f;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) R.o[u][db] *= f;
+      R.m[u] = m;
+    }
+    float sum = 0.0f;
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float y[2];
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const float v = __builtin_amdgcn_exp2f(x[e + d] - ref);
+        sum += v;
+        y[d] = v * w.vs;
+        if constexpr (kMask) y[d] = (seen[u] >> (e + d)) & 1u ? y[d] : 0.0f;
+      }
+      f.u[e >> 1] = (uint32_t)to_bf(y[0]) | ((uint32_t)to_bf(y[1]) << 16);
+    }
+    R.l[u] += sum;
+    p[u] = f.v;
+  }
+  if constexpr (!kMask) {
+    transposed(w.v, [&](int db, bf16x8_t va) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u)
+        R.o[u][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[u], R.o[u][db], 0, 0, 0);
+    });
+  } else {
+    uint2 v[8], bad[8];
+    uint32_t any = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bad[e] = make_uint2(nan_bytes(w.v[e].x), nan_bytes(w.v[e].y));
+      v[e] = make_uint2(w.v[e].x & ~bad[e].x, w.v[e].y & ~bad[e].y);
+      bad[e].x &= 0x38383838u;  // 1.0
+      bad[e].y &= 0x38383838u;
+      any |= bad[e].x | bad[e].y;
+    }
+    transposed(v, [&](int db, bf16x8_t va) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u)
+        R.o[u][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[u], R.o[u][db], 0, 0, 0);
+    });
+    if (__any(any != 0)) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        Frag f;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          f.u[e >> 1] = ((seen[u] >> e) & 1u ? 0x3f80u : 0u) |
+                        ((seen[u] >> (e + 1)) & 1u ? 0x3f800000u : 0u);
+        transposed(bad, [&](int db, bf16x8_t va) {
+          const f32x4_t n =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, f.v, f32x4_t{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n[j] > 0.0f) R.o[u][db][j] = NAN;
+        });
+      }
+    }
+  }
+}
+
+// Windows first, first + stride, ... of keys [lo, hi): `full` is the number of keys
+// that every row sees.
+template <int QT>
+__device__ __forceinline__ void walk(const ScaledAttnArgs& a, const int32_t* bt, int head, int lane,
+                                     int ws, int stride, int hi, int full, Rows<QT>& R) {
+  if (ws >= hi) return;
+  Place p = place_of(a, bt, ws);
+  Win w;
+  load_win(a, head, lane, ws, hi, p, w);
+  Place pn = ws + stride < hi ? place_of(a, bt, ws + stride) : Place{0, false};
+  for (;;) {
+    const int next = ws + stride;
+    Win wn;
+    Place pf{0, false};
+    if (next < hi) {
+      load_win(a, head, lane, next, hi, pn, wn);
+      if (next + stride < hi) pf = place_of(a, bt, next + stride);
+    }
+    if (p.ok) {
+      if (ws + kWin <= full)
+        step<QT, false>(a, w, ws, lane, R);
+      else
+        step<QT, true>(a, w, ws, lane, R);
+    }
+    if (next >= hi) break;
+    ws = next;
+    w = wn;
+    p = pn;
+    pn = pf;
+  }
+}
+
+// row r's 8 outputs of dims d .. d + 7
+__device__ __forceinline__ uint16_t* out_row(const ScaledAttnArgs& a, const Seq& s, int head, int r) {
+  return a.out + (int64_t)(s.qs + r / a.G) * a.o_st + (int64_t)(head * a.G + r % a.G) * a.o_sh;
+}
+
+__global__ __launch_bounds__(64 * kSplitWaves) void k_scaled_split(ScaledAttnArgs a) {
+  __shared__ float s_o[kSplitWaves][kRows][kD];
+  __shared__ float s_ml[kSplitWaves][kRows][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x, head = blockIdx.y % a.Hkv, tile = blockIdx.y / a.Hkv;
+  const int b = blockIdx.z;
+  const Seq s = seq_of(a, b);
+  const int r0 = tile * kRows, rows = s.Lq * a.G - r0;  // rows of this tile, and behind it
+  if (rows <= 0) return;
+  const int live = min(rows, kRows);
+  const int keys = row_keys(s, a.G, r0 + live - 1), full = row_keys(s, a.G, r0);
+  const int lo = split * a.split_len;
+  // the last split also takes the keys past the declared longest sequence
+  const int hi = split == a.nsplit - 1 ? keys : min(keys, lo + a.split_len);
+  if (lo >= hi && split) return;
+  Rows<1> R;
+  load_rows<1>(a, s, head, r0, lane, R);
+  walk<1>(a, a.bt + (int64_t)b * a.bt_stride, head, lane, lo + wave * kWin, kSplitWaves * kWin, hi,
+          full, R);
+  const float l = quad_sum(R.l[0]);
+  const int n = lane & 15, g = lane >> 4;
+  if (g == 0) {
+    s_ml[wave][n][0] = R.m[0];
+    s_ml[wave][n][1] = l;
+  }
+  if (n < live) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float4*>(&s_o[wave][n][32 * g + 8 * j + 4 * h]) =
+            make_float4(R.o[0][4 * h][j], R.o[0][4 * h + 1][j], R.o[0][4 * h + 2][j],
+                        R.o[0][4 * h + 3][j]);
+    }
+  }
+  __syncthreads();
+  // 32 threads a row, 4 dims each
+  const int row = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
+  if (row >= live) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kSplitWaves; ++w) m = fmaxf(m, s_ml[w][row][0]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f, o[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kSplitWaves; ++w) {
+    const float f = __builtin_amdgcn_exp2f(s_ml[w][row][0] - ref);
+    const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
+    sum += f * s_ml[w][row][1];
+    o[0] += f * x.x;
+    o[1] += f * x.y;
+    o[2] += f * x.z;
+    o[3] += f * x.w;
+  }
+  if (a.nsplit == 1 || keys <= a.split_len) {  // the tile's only split
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint2 y;
+    y.x = (uint32_t)to_bf(o[0] * inv) | ((uint32_t)to_bf(o[1] * inv) << 16);
+    y.y = (uint32_t)to_bf(o[2] * inv) | ((uint32_t)to_bf(o[3] * inv) << 16);
+    *reinterpret_cast<uint2*>(out_row(a, s, head, r0 + row) + d) = y;
+  } else {
+    const int64_t slot = (((int64_t)b * a.Hkv + head) * a.qtiles + tile) * a.nsplit + split;
+    *reinterpret_cast<float4*>(a.part_o + (slot * kRows + row) * kD + d) =
+        make_float4(o[0], o[1], o[2], o[3]);
+    if (d == 0) {
+      a.part_ml[(slot * kRows + row) * 2] = m;
+      a.part_ml[(slot * kRows + row) * 2 + 1] = sum;
+    }
+  }
+}
+
+// Joins the splits of one query row: 8 x 32 threads, the first index over the splits.
+__global__ __launch_bounds__(256) void k_scaled_combine(ScaledAttnArgs a) {
+  __shared__ float s_o[8][kD];
+  __shared__ float s_ml[8][2];
+  const int row = blockIdx.x, head = blockIdx.y % a.Hkv, tile = blockIdx.y / a.Hkv;
+  const int b = blockIdx.z;
+  const Seq s = seq_of(a, b);
+  const int r0 = tile * kRows, rows = s.Lq * a.G - r0;
+  if (row >= rows) return;
+  const int keys = row_keys(s, a.G, r0 + min(rows, kRows) - 1);
+  if (keys <= a.split_len) return;  // written by its only split
+  const int n = min(a.nsplit, (keys + a.split_len - 1) / a.split_len);
+  const int64_t slot0 = (((int64_t)b * a.Hkv + head) * a.qtiles + tile) * a.nsplit;
+  const int part = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
+  float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
+  for (int i = part; i < n; i += 8) {
+    const int64_t at = (slot0 + i) * kRows + row;
+    const float mi = a.part_ml[2 * at], li = a.part_ml[2 * at + 1];
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * kD + d);
+    const float mn = fmaxf(m, mi), ref = mn == -INFINITY ? 0.0f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ref), fi = __builtin_amdgcn_exp2f(mi - ref);
+    m = mn;
+    l = l * f + li * fi;
+    o[0] = o[0] * f + x.x * fi;
+    o[1] = o[1] * f + x.y * fi;
+    o[2] = o[2] * f + x.z * fi;
+    o[3] = o[3] * f + x.w * fi;
+  }
+  *reinterpret_cast<float4*>(&s_o[part][d]) = make_float4(o[0], o[1], o[2], o[3]);
+  if (d == 0) s_ml[part][0] = m, s_ml[part][1] = l;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, s_ml[i][0]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  l = 0.0f;
+  o[0] = o[1] = o[2] = o[3] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_ml[i][0] - ref);
+    const float4 x = *reinterpret_cast<const float4*>(&s_o[i][d]);
+    l += f * s_ml[i][1];
+    o[0] += f * x.x;
+    o[1] += f * x.y;
+    o[2] += f * x.z;
+    o[3] += f * x.w;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint2 y;
+  y.x = (uint32_t)to_bf(o[0] * inv) | ((uint32_t)to_bf(o[1] * inv) << 16);
+  y.y = (uint32_t)to_bf(o[2] * inv) | ((uint32_t)to_bf(o[3] * inv) << 16);
+  *reinterpret_cast<uint2*>(out_row(a, s, head, r0 + row) + d) = y;
+}
+
+template <int QT>
+__global__ __launch_bounds__(64 * kRowWaves) void k_scaled_rows(ScaledAttnArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.y, b = blockIdx.z;
+  const Seq s = seq_of(a, b);
+  const int total = s.Lq * a.G;
+  const int r0 = (blockIdx.x * kRowWaves + wave) * kRows * QT;
+  if (r0 >= total) return;
+  const int last = min(total, r0 + kRows * QT) - 1;
+  Rows<QT> R;
+  load_rows<QT>(a, s, head, r0, lane, R);
+  walk<QT>(a, a.bt + (int64_t)b * a.bt_stride, head, lane, 0, kWin, row_keys(s, a.G, last),
+           row_keys(s, a.G, r0), R);
+  const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const float l = quad_sum(R.l[t]);
+    const int r = r0 + 16 * t + n;
+    if (r >= total) continue;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* y = out_row(a, s, head, r) + 32 * g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint16_t h[8];
+#pragma unroll
+      for (int db = 0; db < 8; ++db) h[db] = to_bf(R.o[t][db][j] * inv);
+      *reinterpret_cast<uint4*>(y + 8 * j) = pack8(h);
+    }
+  }
+}
+
+constexpr int kRowsQT = 2;  // tiles of a wave in k_scaled_rows
+
+struct ScaledPlan {
+  bool rows;  // k_scaled_rows
+  int qtiles, nsplit, split_len;
+  size_t bytes;
+};
+
+ScaledPlan plan_of(int num_seqs, int Hkv, int G, int max_q, int max_k) {
+  ScaledPlan p;
+  const int64_t rows = (int64_t)max_q * G;
+  const int64_t q = (rows + kRows - 1) / kRows;
+  p.qtiles = (int)q;
+  p.rows = rows > 64;
+  p.nsplit = 1;
+  p.split_len = INT32_MAX;
+  p.bytes = 0;
+  if (p.rows) return p;
+  const int64_t tiles = (int64_t)num_seqs * Hkv * q;
+  // about 1024 workgroups if every sequence is as long as declared, of at least one
+  // window a wave and at most 1024 keys unless that makes more than 8192 of them
+  int64_t len = (max_k * tiles + 1023) / 1024;
+  if (len > 1024) len = 1024;
+  const int64_t floor_len = (max_k * tiles + 8191) / 8192;
+  if (len < floor_len) len = floor_len;
+  const int64_t unit = kSplitWaves * kWin;
+  len = (len + unit - 1) / unit * unit;
+  p.split_len = (int)(len > INT32_MAX / 2 ? INT32_MAX / 2 : len);
+  p.nsplit = (int)((max_k + (int64_t)p.split_len - 1) / p.split_len);
+  if (p.nsplit > 1) p.bytes = (size_t)tiles * p.nsplit * kRows * (kD + 2) * sizeof(float);
+  return p;
+}
+
+}  // namespace
+}  // namespace hs
+
+using namespace hs;
+
+extern "C" {
+
+size_t hs_verify_attention_scaled_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
+                                                 int max_seqlen_q, int max_seqlen_k) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || max_seqlen_q <= 0 ||
+      max_seqlen_k <= 0)
+    return 0;
+  return plan_of(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_seqlen_q, max_seqlen_k)
+      .bytes;
+}
+
+int hs_verify_attention_scaled(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+    const void* v_cache, int64_t cache_stride_block, int64_t cache_stride_tok,
+    int64_t cache_stride_head, const float* k_scales, const float* v_scales,
+    int64_t scale_stride_block, int64_t scale_stride_group, int64_t scale_stride_head, int group,
+    const int32_t* block_tables, int64_t block_table_stride, int block_table_width, int num_blocks,
+    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int num_seqs, int max_seqlen_q,
+    int max_seqlen_k, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+    float softmax_scale, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+    void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k_cache || !v_cache || !k_scales || !v_scales || !block_tables || !cu_seqlens_q ||
+      !cu_seqlens_k || !out)
+    return HS_ERR_INVALID;
+  if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_seqlen_q <= 0 ||
+      max_seqlen_k <= 0 || num_blocks <= 0 || block_size <= 0 || group <= 0 ||
+      block_table_width <= 0 || block_table_stride < block_table_width)
+    return HS_ERR_INVALID;
+  if (num_q_heads % num_kv_heads || block_size % group) return HS_ERR_INVALID;
+  if (head_dim != kD) return HS_ERR_UNSUPPORTED;
+  if (group != 32 && group != 64 && group != 128 && group != 256) return HS_ERR_UNSUPPORTED;
+  const int G = num_q_heads / num_kv_heads;
+  if (G > kRows) return HS_ERR_UNSUPPORTED;
+  if ((q_stride_tok % 8) || (q_stride_head % 8) || (out_stride_tok % 8) || (out_stride_head % 8))
+    return HS_ERR_UNSUPPORTED;
+  if ((cache_stride_block % 16) || (cache_stride_tok % 16) || (cache_stride_head % 16))
+    return HS_ERR_UNSUPPORTED;
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15)
+    return HS_ERR_UNSUPPORTED;
+  if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3) return HS_ERR_UNSUPPORTED;
+  // a window's rows lie within 2 GiB of its first (32-bit offsets of the lanes)
+  if (cache_stride_tok < 0 || cache_stride_tok > INT32_MAX / (2 * kWin)) return HS_ERR_UNSUPPORTED;
+  const ScaledPlan p = plan_of(num_seqs, num_kv_heads, G, max_seqlen_q, max_seqlen_k);
+  const int64_t tiles = (int64_t)num_kv_heads * p.qtiles;
+  if (num_seqs > 65535 || (int64_t)max_seqlen_q * G > INT32_MAX / 2 || num_kv_heads > 65535)
+    return HS_ERR_UNSUPPORTED;
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return HS_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return HS_ERR_UNSUPPORTED;
+  ScaledAttnArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = q_stride_tok;
+  a.q_sh = q_stride_head;
+  a.kc = static_cast<const uint8_t*>(k_cache);
+  a.vc = static_cast<const uint8_t*>(v_cache);
+  a.c_sb = cache_stride_block;
+  a.c_st = cache_stride_tok;
+  a.c_sh = cache_stride_head;
+  a.ks = k_scales;
+  a.vs = v_scales;
+  a.s_sb = scale_stride_block;
+  a.s_sg = scale_stride_group;
+  a.s_sh = scale_stride_head;
+  a.bt = block_tables;
+  a.bt_stride = block_table_stride;
+  a.bt_width = block_table_width;
+  a.num_blocks = num_blocks;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.Hkv = num_kv_heads;
+  a.G = G;
+  a.block_size = block_size;
+  a.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz((unsigned)block_size) : -1;
+  a.g_shift = __builtin_ctz((unsigned)group);
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_st = out_stride_tok;
+  a.o_sh = out_stride_head;
+  a.qtiles = p.qtiles;
+  a.nsplit = p.nsplit;
+  a.split_len = p.split_len;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + (size_t)num_seqs * tiles * p.nsplit * kRows * kD;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (p.rows) {
+    const int64_t per = (int64_t)kRows * kRowsQT * kRowWaves;
+    const dim3 grid((unsigned)(((int64_t)max_seqlen_q * G + per - 1) / per),
+                    (unsigned)num_kv_heads, (unsigned)num_seqs);
+    hipLaunchKernelGGL(k_scaled_rows<kRowsQT>, grid, dim3(64 * kRowWaves), 0, st, a);
+    return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
+  }
+  if (tiles > 65535) return HS_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(k_scaled_split, dim3((unsigned)p.nsplit, (unsigned)tiles, (unsigned)num_seqs),
+                     dim3(64 * kSplitWaves), 0, st, a);
+  if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
+  if (p.nsplit > 1) {
+    hipLaunchKernelGGL(k_scaled_combine,
+                       dim3((unsigned)kRows, (unsigned)tiles, (unsigned)num_seqs), dim3(256), 0,
+                       st, a);
+    if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
+  }
+  return HS_OK;
+}
+
+}  // extern "C"

@@ -401,6 +401,118 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
     L.check(rc, "hs_store_kvcache")
 
 
+def _call(dev: torch.device, what: str, *args) -> None:
+    """Entry point `what` on the current stream of `dev`, which need not be the
+    current device."""
+    fn = getattr(L.lib(), what)
+    if dev.index == torch.cuda.current_device():
+        L.check(fn(*args, _stream(dev)), what)
+    else:
+        with torch.cuda.device(dev):
+            L.check(fn(*args, _stream(dev)), what)
+
+
+def _scaled_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                  v_scales: torch.Tensor) -> int:
+    """Checks an 8-bit cache with group scales; returns the group (tokens per scale)."""
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError("a cache with group scales must be float8_e4m3fn")
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+        raise TypeError("k_scales / v_scales must be float32")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or \
+            k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
+        raise ValueError("k_cache and v_cache must be [blocks, block_size, kv_heads, head_dim] "
+                         "with identical strides and contiguous head_dim")
+    nb, bs, Hkv, _ = k_cache.shape
+    if k_scales.dim() != 3 or k_scales.shape != v_scales.shape or \
+            k_scales.stride() != v_scales.stride() or k_scales.shape[0] != nb or \
+            k_scales.shape[2] != Hkv or k_scales.shape[1] < 1 or bs % k_scales.shape[1]:
+        raise ValueError("k_scales and v_scales must be [blocks, block_size / group, kv_heads] "
+                         "with identical strides")
+    return bs // k_scales.shape[1]
+
+
+def store_kvcache_scaled(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                         slot_mapping: torch.Tensor) -> None:
+    """store_kvcache into a float8_e4m3fn cache with one f32 scale per group of
+    tokens and kv head: scales [num_blocks, block_size / group, Hkv], group 32, 64,
+    128 or 256, value = code * scale. A call that writes a group's first slot starts
+    the group with the power of two its own rows need; a later one raises the scale
+    where its rows need it and rewrites the group's other codes for it
+    (hs_store_kvcache_scaled). Scales may start as zeros."""
+    dev = _need_cuda(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
+    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+        raise TypeError("key/value must be bfloat16")
+    if key.dim() != 3 or key.shape != value.shape or key.stride(2) != 1 or value.stride(2) != 1:
+        raise ValueError("key and value must be [tokens, kv_heads, head_dim] with contiguous "
+                         "head_dim")
+    group = _scaled_cache(k_cache, v_cache, k_scales, v_scales)
+    N, Hkv, D = key.shape
+    nb, bs, Hc, Dc = k_cache.shape
+    if (Hc, Dc) != (Hkv, D):
+        raise ValueError("cache geometry mismatch")
+    if slot_mapping.numel() != N:
+        raise ValueError("slot_mapping must have one entry per token")
+    sm = slot_mapping.to(torch.int32).contiguous()
+    _call(dev, "hs_store_kvcache_scaled", key.data_ptr(), key.stride(0), key.stride(1),
+          value.data_ptr(), value.stride(0), value.stride(1), k_cache.data_ptr(),
+          v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+          k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1),
+          k_scales.stride(2), group, sm.data_ptr(), N, Hkv, D, bs, nb)
+
+
+def verify_attention_scaled(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            k_scales: torch.Tensor, v_scales: torch.Tensor,
+                            block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                            cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+                            softmax_scale: float, *,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """verify_attention over a float8_e4m3fn cache with group scales (see
+    store_kvcache_scaled): decode, verify and prompt rows, causal, grouped heads.
+
+    q [tokens, Hq, 128] bf16; block_tables int32 [B, W]; cu_seqlens_q/k int32
+    [B+1]. A query row that sees no key gets zeros. The partial results of split
+    keys live in a buffer of the call's own, so calls may overlap on streams and in
+    captured graphs."""
+    dev = _need_cuda(q, k_cache, v_cache, k_scales, v_scales, block_tables, cu_seqlens_q,
+                     cu_seqlens_k, out)
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError("q must be [tokens, heads, head_dim] bf16 with contiguous head_dim")
+    group = _scaled_cache(k_cache, v_cache, k_scales, v_scales)
+    N, Hq, D = q.shape
+    nb, bs, Hkv, Dc = k_cache.shape
+    if D != Dc:
+        raise ValueError("head_dim mismatch")
+    B = cu_seqlens_q.numel() - 1
+    if B < 1 or cu_seqlens_k.numel() != B + 1:
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must have one more entry than sequences")
+    cq = cu_seqlens_q.to(torch.int32).contiguous()
+    ck = cu_seqlens_k.to(torch.int32).contiguous()
+    bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
+    if bt.dim() != 2 or bt.shape[0] < B:
+        raise ValueError("block_tables must be [sequences, blocks]")
+    if bt.stride(1) != 1:
+        bt = bt.contiguous()
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1:
+        raise ValueError("out must have q's shape, bf16 with contiguous head_dim")
+    if N == 0:
+        return out
+    mq, mk = int(max_seqlen_q), int(max_seqlen_k)
+    nbytes = L.lib().hs_verify_attention_scaled_workspace_size(B, Hq, Hkv, mq, mk)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, "hs_verify_attention_scaled", q.data_ptr(), q.stride(0), q.stride(1),
+          k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+          k_cache.stride(2), k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0),
+          k_scales.stride(1), k_scales.stride(2), group, bt.data_ptr(), bt.stride(0), bt.shape[1],
+          nb, cq.data_ptr(), ck.data_ptr(), B, mq, mk, Hq, Hkv, D, bs, float(softmax_scale),
+          out.data_ptr(), out.stride(0), out.stride(1), None if ws is None else ws.data_ptr(),
+          nbytes)
+    return out
+
+
 class SpecStateTensors:
     """Device-resident bookkeeping state of a batch (layout of hs_spec_state).
 

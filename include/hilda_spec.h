@@ -250,6 +250,67 @@ int hs_store_kvcache(const void* key, int64_t key_stride_tok, int64_t key_stride
                      void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* 8-bit KV cache with a scale per token group and kv head.                  */
+/* No counterpart in the reference (its FP8 cache, attention.py:17-56, is an  */
+/* absent external package with one scale per tensor): the same paged cache, */
+/* codes e4m3fn, whose value at (block, offset, head) is                      */
+/* code * scales[block, offset / group, head]; group 32, 64, 128 or 256 and a */
+/* divisor of block_size. Scales are f32 with element strides (block, group,  */
+/* head), the same for K and V.                                               */
+/*                                                                          */
+/* hs_store_kvcache_scaled: hs_store_kvcache into such a cache. Of every      */
+/* (group, kv head) the call writes to, with a = the largest finite |x| of    */
+/* the call's rows in it and need = the smallest power of two >= a / 448, at  */
+/* least 2^-96:                                                               */
+/*  - a call that writes the group's first slot starts the group: the scale   */
+/*    becomes need, and codes of slots it does not write are left (a sequence */
+/*    fills its slots in order, so they belong to an earlier owner). The same */
+/*    where the stored scale is not positive and finite;                      */
+/*  - otherwise the scale becomes max(old, need), and where that is above the */
+/*    old one the group's other codes are rewritten for it:                   */
+/*    e4m3(code * old / scale).                                               */
+/* The rows are stored as sat_e4m3fn(x / scale): round to nearest even,       */
+/* infinities saturate, NaN stays NaN. The tokens of a group may stand        */
+/* anywhere in slot_mapping; a slot that occurs twice takes the later token's */
+/* row; slots < 0 and blocks >= num_blocks are skipped. Rows of K/V 16-byte   */
+/* aligned (strides multiples of 8 elements), cache rows 8-byte.              */
+int hs_store_kvcache_scaled(const void* key, int64_t key_stride_tok, int64_t key_stride_head,
+                            const void* value, int64_t value_stride_tok,
+                            int64_t value_stride_head, void* k_cache, void* v_cache,
+                            int64_t cache_stride_block, int64_t cache_stride_tok,
+                            int64_t cache_stride_head, float* k_scales, float* v_scales,
+                            int64_t scale_stride_block, int64_t scale_stride_group,
+                            int64_t scale_stride_head, int group, const int32_t* slot_mapping,
+                            int num_tokens, int num_kv_heads, int head_dim, int block_size,
+                            int num_blocks, void* stream);
+
+/* hs_verify_attention over such a cache (decode, verify and prompt rows; the */
+/* same causal alignment, tables and alignment rules): scores take the key's  */
+/* k scale, probabilities the v scale. Keys whose block-table entry is not in */
+/* [0, num_blocks), or lies past the table, are left out; a query row that    */
+/* sees no key gets zeros; what a row does not see takes no part in it,       */
+/* whatever its codes and scales are. Sequences longer than max_seqlen_k are  */
+/* attended in full; query tokens past max_seqlen_q are not computed.         */
+/* The workspace needs no preparation and holds nothing between calls; calls  */
+/* that overlap in time need one each. block_size: a multiple of group; at    */
+/* most 16 query heads to a kv head.                                          */
+size_t hs_verify_attention_scaled_workspace_size(int num_seqs, int num_q_heads, int num_kv_heads,
+                                                 int max_seqlen_q, int max_seqlen_k);
+int hs_verify_attention_scaled(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                               const void* k_cache, const void* v_cache,
+                               int64_t cache_stride_block, int64_t cache_stride_tok,
+                               int64_t cache_stride_head, const float* k_scales,
+                               const float* v_scales, int64_t scale_stride_block,
+                               int64_t scale_stride_group, int64_t scale_stride_head, int group,
+                               const int32_t* block_tables, int64_t block_table_stride,
+                               int block_table_width, int num_blocks, const int32_t* cu_seqlens_q,
+                               const int32_t* cu_seqlens_k, int num_seqs, int max_seqlen_q,
+                               int max_seqlen_k, int num_q_heads, int num_kv_heads, int head_dim,
+                               int block_size, float softmax_scale, void* out,
+                               int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Device-resident bookkeeping of the speculative step.                      */
 /*                                                                          */
 /* The state mirrors Sequence (mini_vllm/engine/sequence.py:14-132) and      */
