@@ -16,6 +16,7 @@ HS_F32, HS_BF16, HS_FP8_E4M3 = 0, 1, 2
 HS_ACCEPT_REFERENCE, HS_ACCEPT_FILTERED, HS_ACCEPT_GREEDY = 0, 1, 2
 HS_ACCEPT_TOPK_LE64 = 0x100
 HS_ACCEPT_CHAIN = 0x200
+HS_LINEAR_PLAIN, HS_LINEAR_SWIGLU = 0, 1
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
@@ -90,6 +91,9 @@ SIGNATURES.update({
     "hs_spec_commit_next": (_i32, [_sp, _i32, _vp, _vp, _vp, _vp, _sz, _i32, _vp, _i32, _vp, _vp,
                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "hs_zero_kv_slots": (_i32, [_vp, _i64, _i32, _i64, _i64, _i64, _vp, _i32, _vp]),
+    "hs_linear_int4_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
+    "hs_linear_int4": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp,
+                              _sz, _vp]),
     "hs_linear": (_i32, [_vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "hs_rmsnorm": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _f32, _vp]),
     "hs_qk_norm_rope": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp,

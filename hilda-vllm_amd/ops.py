@@ -8,6 +8,8 @@ are ordered by the current stream.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib as L
@@ -929,3 +931,99 @@ def linear_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: float, weigh
         norm_weight.data_ptr(), float(eps), weight.data_ptr(), M, K, N, 1 if swiglu else 0,
         out.data_ptr(), N, _stream(dev)), "hs_linear_rmsnorm")
     return out, (x if residual is None else res_out)
+
+
+@dataclass(frozen=True)
+class Int4Weight:
+    """A projection's weight in 4 bits with group scales, in the layout of
+    hs_linear_int4: packed int32 [tiles, steps, 64, 4] and scales bf16
+    [tiles, groups, 16] over 16-feature tiles and 128-input steps. pack_int4 and
+    quantize_int4 make one."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    out_features: int
+    in_features: int
+    group: int
+
+
+def pack_int4(codes: torch.Tensor, scales: torch.Tensor) -> Int4Weight:
+    """Lays out codes [N, K] (integers 0 .. 15, the weight is (code - 8) * scale) and
+    scales bf16 [N, K / group], group 32, 64 or 128, for linear_int4. Done once a
+    weight, with torch operations on the tensors' device."""
+    if codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0] or \
+            scales.shape[1] < 1 or codes.shape[1] % scales.shape[1]:
+        raise ValueError("codes must be [N, K] and scales [N, K / group]")
+    if scales.dtype != torch.bfloat16 or codes.is_floating_point() or codes.dtype == torch.bool:
+        raise TypeError("codes must be integers and scales bfloat16")
+    N, K = codes.shape
+    group = K // scales.shape[1]
+    if group not in (32, 64, 128):
+        raise ValueError("a group must be 32, 64 or 128 inputs")
+    if N and (int(codes.min()) < 0 or int(codes.max()) > 15):
+        raise ValueError("codes must lie in 0 .. 15")
+    tiles, steps = -(-N // 16), -(-K // 128)
+    c = torch.full((tiles * 16, steps * 128), 8, dtype=torch.uint8, device=codes.device)
+    c[:N, :K] = codes
+    # [tile, feature, step, i, g, e] -> [tile, step, lane (g, feature), i, e]
+    c = c.view(tiles, 16, steps, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)
+    word = torch.zeros(c.shape[:-1], dtype=torch.int32, device=codes.device)
+    for e in range(8):
+        word |= c[..., e].int() << (4 * (e // 2) + 16 * (e % 2))
+    s = torch.zeros((tiles * 16, steps * (128 // group)), dtype=torch.bfloat16,
+                    device=codes.device)
+    s[:N, :scales.shape[1]] = scales
+    s = s.view(tiles, 16, -1).permute(0, 2, 1).contiguous()
+    return Int4Weight(word.view(tiles, steps, 64, 4), s, N, K, group)
+
+
+def quantize_int4(weight: torch.Tensor, group: int = 128) -> Int4Weight:
+    """A float weight [N, K] to the nearest codes: per group the scale is its largest
+    |w| over 7, rounded to bf16 (a group of zeros: scale 0)."""
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError("weight must be a floating [N, K] tensor")
+    if group not in (32, 64, 128) or weight.shape[1] % group:
+        raise ValueError("group must be 32, 64 or 128 and divide the inputs")
+    w = weight.float().view(weight.shape[0], -1, group)
+    scales = (w.abs().amax(-1) / 7).to(torch.bfloat16)
+    s = scales.float().unsqueeze(-1)
+    codes = torch.where(s > 0, torch.round(w / s), 0).clamp(-8, 7) + 8
+    return pack_int4(codes.to(torch.uint8).view(weight.shape), scales)
+
+
+def linear_int4(x: torch.Tensor, weight: Int4Weight, *, swiglu: bool = False,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """linear with a 4-bit weight (hs_linear_int4): x [rows, K] bf16, any number of
+    rows -> [rows, N] bf16, fp32 accumulation. With swiglu=True the weight is
+    [2F, K] (gate | up), F a multiple of 16, and the result silu(gate) * up
+    [rows, F]. An infinity in a row of x gives NaN in that row."""
+    w = weight
+    dev = _need_cuda(x, w.packed, w.scales, out)
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        raise ValueError("linear_int4 expects a 2-D bf16 input")
+    M, K = x.shape
+    if K != w.in_features:
+        raise ValueError("in_features mismatch")
+    if swiglu and w.out_features % 32:
+        raise ValueError("swiglu needs gate and up halves of a multiple of 16 features")
+    tiles, steps = -(-w.out_features // 16), -(-K // 128)
+    if w.group not in (32, 64, 128) or w.packed.dtype != torch.int32 or \
+            w.scales.dtype != torch.bfloat16 or w.packed.shape != (tiles, steps, 64, 4) or \
+            w.scales.shape != (tiles, steps * (128 // w.group), 16) or \
+            not w.packed.is_contiguous() or not w.scales.is_contiguous():
+        raise ValueError("weight is not laid out as pack_int4 does")
+    N = w.out_features // 2 if swiglu else w.out_features
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    elif out.shape != (M, N) or out.stride(1) != 1 or out.dtype != torch.bfloat16:
+        raise ValueError("out must be [rows, out_features] bf16 with contiguous rows")
+    if M == 0:
+        return out
+    epi = L.HS_LINEAR_SWIGLU if swiglu else L.HS_LINEAR_PLAIN
+    nbytes = L.lib().hs_linear_int4_workspace_size(M, K, N, epi) if M > 16 else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, "hs_linear_int4", x.data_ptr(), x.stride(0), w.packed.data_ptr(),
+          w.scales.data_ptr(), M, K, N, w.group, epi, out.data_ptr(), out.stride(0),
+          None if ws is None else ws.data_ptr(), nbytes)
+    return out

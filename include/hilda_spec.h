@@ -272,8 +272,9 @@ int hs_store_kvcache(const void* key, int64_t key_stride_tok, int64_t key_stride
 /* The rows are stored as sat_e4m3fn(x / scale): round to nearest even,       */
 /* infinities saturate, NaN stays NaN. The tokens of a group may stand        */
 /* anywhere in slot_mapping; a slot that occurs twice takes the later token's */
-/* row; slots < 0 and blocks >= num_blocks are skipped. Rows of K/V 16-byte   */
-/* aligned (strides multiples of 8 elements), cache rows 8-byte.              */
+/* row (and counts once for a); slots < 0 and blocks >= num_blocks are        */
+/* skipped. K/V rows 16-byte aligned (strides multiples of 8 elements), cache */
+/* rows 8-byte.                                                               */
 int hs_store_kvcache_scaled(const void* key, int64_t key_stride_tok, int64_t key_stride_head,
                             const void* value, int64_t value_stride_tok,
                             int64_t value_stride_head, void* k_cache, void* v_cache,
@@ -508,6 +509,26 @@ int hs_linear_rmsnorm(const void* x, int64_t x_stride, const void* residual_in,
                       const void* norm_weight, float eps, const void* weight, int rows,
                       int in_features, int out_features, int epilogue, void* out,
                       int64_t out_stride, void* stream);
+
+/* hs_linear with 4-bit weights and group scales, any number of rows (no       */
+/* counterpart in the reference): weight[n, k] = (code[n, k] - 8) *             */
+/* scale[n, k / group], code 0 .. 15, group 32, 64 or 128 (a divisor of        */
+/* in_features), x and out bf16, fp32 accumulation. HS_LINEAR_SWIGLU: weight    */
+/* [2 * out_features, in_features] gate | up, out = silu(gate) * up rounded     */
+/* once; out_features then a multiple of 16. An infinity in a row of x gives    */
+/* NaN there.                                                                  */
+/* packed: [tiles][steps][64][4] 32-bit words, tile = 16 weight rows, step =    */
+/* 128 inputs: word i of lane l holds row 16 tile + l % 16, inputs 128 step +   */
+/* 32 i + 8 (l / 16) + e, e = 0 .. 7, input 2 p at bits 4 p and input 2 p + 1   */
+/* at bits 16 + 4 p. scales: bf16 [tiles][steps * 128 / group][16]. Rows past   */
+/* the last and inputs past in_features are padded with code 8 and scale 0.     */
+/* x_stride: a multiple of 8 elements; x and packed 16-byte, scales 8-byte      */
+/* aligned. The workspace (for more than 16 rows of a narrow weight) needs no   */
+/* preparation and holds nothing between calls.                                */
+size_t hs_linear_int4_workspace_size(int rows, int in_features, int out_features, int epilogue);
+int hs_linear_int4(const void* x, int64_t x_stride, const void* packed, const void* scales,
+                   int rows, int in_features, int out_features, int group, int epilogue, void* out,
+                   int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out = RMSNorm(x (+ residual)) * weight; with residual != NULL the residual  */
 /* row is replaced by bf16(x + residual) (strides in elements).              */
