@@ -307,6 +307,50 @@ def sample_rows(logits: torch.Tensor, temperatures: torch.Tensor | None = None,
     return dict(probs=probs, tokens=toks, row_stats=stats)
 
 
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0,
+                   temperatures: torch.Tensor | None = None):
+    """Log-probabilities of one given token a row, the rows' entropy and their `top` most
+    likely tokens (hs_token_logprobs), of softmax(logits / temperature).
+
+    logits [rows, V] f32/bf16, tokens [rows] integers (outside [0, V): -inf),
+    temperatures [rows] > 0, top 0 .. 32. Returns dict(logprobs=[rows] f32 or None,
+    entropy=[rows] f32, top_ids=[rows, top] int64 and top_logprobs=[rows, top] f32, None
+    with top 0): largest logits first, the lower id first among equal ones. A row with a
+    NaN, a +inf or nothing but -inf gives NaN. Calls may overlap on streams and in
+    captured graphs."""
+    dev = _need_cuda(logits, tokens, temperatures)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, V]")
+    rows, V = logits.shape
+    dtype, top = _logit_dtype(logits), int(top)
+    if not 0 <= top <= min(32, V):
+        raise ValueError("top must lie in 0 .. 32 and not exceed the vocabulary")
+    if tokens is not None:
+        if tokens.numel() != rows or tokens.is_floating_point() or tokens.dtype == torch.bool:
+            raise ValueError("tokens must be one integer a row")
+        tokens = tokens.to(torch.int64).reshape(rows).contiguous()
+    if temperatures is not None:
+        if temperatures.numel() != rows:
+            raise ValueError("temperatures must be one a row")
+        temperatures = temperatures.to(torch.float32).reshape(rows).contiguous()
+    f32 = dict(dtype=torch.float32, device=dev)
+    lp = torch.empty(rows, **f32) if tokens is not None else None
+    ent = torch.empty(rows, **f32)
+    ids = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
+    tlp = torch.empty((rows, top), **f32) if top else None
+    if rows:
+        lg, lstride = _rows2d(logits, rows, V)
+        nbytes = L.lib().hs_token_logprobs_workspace_size(rows, V, top)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+        def p(t):
+            return None if t is None else t.data_ptr()
+
+        _call(dev, "hs_token_logprobs", lg.data_ptr(), dtype, lstride, rows, V, p(tokens),
+              p(temperatures), top, p(lp), ent.data_ptr(), p(ids), p(tlp), ws.data_ptr(), nbytes)
+    return dict(logprobs=lp, entropy=ent, top_ids=ids, top_logprobs=tlp)
+
+
 _KV_DTYPES = {torch.bfloat16: L.HS_BF16, torch.float8_e4m3fn: L.HS_FP8_E4M3}
 
 

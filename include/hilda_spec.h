@@ -157,6 +157,25 @@ int hs_sampler(const void* logits, int logits_dtype, int64_t logits_row_stride,
                void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Log-probabilities of given tokens, entropy and most likely tokens of rows  */
+/* of logits (no counterpart in the reference). With y = logits / T:          */
+/* logprobs[r] = log softmax(y)[tokens[r]] (-inf for a token outside          */
+/* [0, vocab)); entropy[r] = -sum p log p (a token of probability 0 adds 0);  */
+/* top_ids / top_logprobs [rows, top]: the largest logits, largest first, the */
+/* lower index first among equal ones (-0 equals 0, NaN is the largest), with */
+/* their log-probabilities. top: 0 .. 32, at most vocab. A row with a NaN, a   */
+/* +inf or nothing but -inf gives NaN log-probabilities and entropy.          */
+/* logits [rows, vocab] HS_F32 or HS_BF16, temperatures [rows] f32 > 0 or     */
+/* NULL (1); tokens and logprobs both or neither; entropy may be NULL. At most */
+/* 65535 rows and 2^21 tokens. The workspace needs no preparation and holds    */
+/* nothing between calls.                                                      */
+size_t hs_token_logprobs_workspace_size(int rows, int vocab, int top);
+int hs_token_logprobs(const void* logits, int logits_dtype, int64_t logits_row_stride, int rows,
+                      int vocab, const int64_t* tokens, const float* temperatures, int top,
+                      float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* gamma+1-query paged-attention verify.                                     */
 /*                                                                          */
 /* Replaces the verify branch of Attention.forward,                          */
