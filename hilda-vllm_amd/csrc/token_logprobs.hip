@@ -2,15 +2,21 @@
 // Of a row y = logits / T with maximum m, S = sum exp(y - m), U = sum (y - m) exp(y - m):
 //   log p(t) = (y_t - m) - ln S        entropy = ln S - U / S
 // and the `top` largest logits in order, the lower index first among equal ones.
-// One pass over the logits, which bound it: a workgroup takes a chunk of a row into
-// registers, so its maximum, its two sums and its candidates come from one read.
-//
-// Candidates: a wave's n-th largest lane maximum is at most its n-th largest value, so
-// only values from there on can be among the row's n largest; the lane maxima's n-th
-// largest is found bit by bit with ballots. What passes is ranked by counting and the
-// chunk's n best are written in order (one at a time where more pass than the list
-// holds: many equal values). k_logprobs_join adds up a row's chunks (sums rescaled to
-// the row's maximum, f32) and ranks their lists' values the same way.
+// Exponents are powers of two: (x - max x) log2(e) / T, whose difference is rounded but
+// cannot overflow where its terms do not.
+// k_logprobs_chunk reads the logits, which bound it, once: a workgroup takes a chunk of
+// a row into registers and leaves its maximum, its two sums and the maximum of every 32
+// neighbouring logits. k_logprobs_join, a workgroup a row, adds up the chunks (sums
+// rescaled to the row's maximum, f32) and finds the alternatives: the n-th largest of
+// its 256 threads' shares of those maxima is at most the row's n-th largest value, so
+// only values from there on can be among the n largest, and they lie in the groups of 32
+// whose maxima reach it. It finds that bar bit by bit with ballots, reads those groups
+// again (about n of them), and ranks what passes by counting. (256 rows of 151936 bf16
+// logits, top 20: 39 us with the n largest of every chunk picked in the chunk's
+// workgroup and merged, 31 us so: 21 us for the chunks, 3.7 TB/s, and 11 us for the
+// join.) Where more passes than its
+// list holds - many equal values - the row's values are taken one by one, and -inf, what
+// a mask leaves of excluded tokens, only fills up.
 //
 // Order: values as the row holds them (a temperature does not change it), -0 as 0,
 // and NaN above everything. A row with a NaN, with +inf, or with nothing but -inf gets
@@ -27,8 +33,9 @@ namespace {
 
 constexpr int kLpT = 256;      // threads of a workgroup
 constexpr int kMaxTop = 32;
-constexpr int kListed = 512;   // candidates of a chunk that are ranked by counting
-constexpr int kPerLane = 4;    // chunks of a row over the lanes of a wave: at most 256
+constexpr int kListed = 1024;  // groups and values that are ranked by counting
+constexpr int kGroup = 32;     // neighbouring logits with a maximum kept
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LogprobArgs {
@@ -41,10 +48,9 @@ struct LogprobArgs {
   float* entropy;
   int64_t* top_ids;
   float* top_logprobs;
-  // per (row, chunk): m, S, U, unused; then top keys and ids
-  float4* sums;
-  uint32_t* keys;
-  int32_t* ids;
+  float4* sums;    // [row][chunk]: largest logit, S, U (in powers of two), unused
+  uint32_t* most;  // [row][groups]: order of the groups' maxima
+  int groups;      // of a row: its chunks' logits over kGroup
 };
 
 // order of a value: larger is larger, -0 as 0, NaN the largest
@@ -52,19 +58,26 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return x != x ? 0xffffffffu : hs_key(x);
 }
 
+// a value and its place as one number: larger comes first
+__device__ __forceinline__ uint64_t listing(uint32_t key, int id) {
+  return ((uint64_t)key << 32) | (uint32_t)~(uint32_t)id;
+}
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return v;
+}
+// the value of another lane of the four neighbours (a DPP quad permutation)
+template <int kPerm>
+__device__ __forceinline__ float quad_xor(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kPerm, 0xF, 0xF, false));
+}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// maximum that keeps a NaN
-__device__ __forceinline__ float nan_max(float a, float b) { return (a > b || a != a) ? a : b; }
-__device__ __forceinline__ float wave_nan_max(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = nan_max(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
 template <typename T>
 __device__ __forceinline__ float logit(const T* x, int64_t i) {
   if constexpr (sizeof(T) == 2) return bf16_to_f32(x[i]);
@@ -81,246 +94,246 @@ template <typename T, int E, bool kAligned>
 __global__ __launch_bounds__(kLpT) void k_logprobs_chunk(LogprobArgs a) {
   constexpr int kChunkLen = E * kLpT;
   __shared__ float s_f[3][4];
-  __shared__ uint32_t s_key[kListed];
-  __shared__ int s_id[kListed];
-  __shared__ int s_n;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = blockIdx.y, chunk = blockIdx.x;
   const int base = chunk * kChunkLen, len = min(kChunkLen, a.vocab - base);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride + base;
   float v[E];
+  if (kAligned && len == kChunkLen) {  // every load of the chunk before the first wait
+    constexpr int kWords = sizeof(T) == 2 ? 4 : 8;
+    uint32_t w[E / 8][kWords];
+#pragma unroll
+    for (int i = 0; i < E / 8; ++i)
+#pragma unroll
+      for (int h = 0; h < kWords / 4; ++h) {
+        const uint4 u = reinterpret_cast<const uint4*>(x + elem_of(8 * i))[h];
+        w[i][4 * h] = u.x, w[i][4 * h + 1] = u.y, w[i][4 * h + 2] = u.z, w[i][4 * h + 3] = u.w;
+      }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (sizeof(T) == 2)
+        v[e] = u2f((e & 1) ? w[e >> 3][(e & 7) >> 1] & 0xffff0000u : w[e >> 3][(e & 7) >> 1] << 16);
+      else
+        v[e] = u2f(w[e >> 3][e & 7]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = logit<T>(x, min(elem_of(e), len - 1));
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = elem_of(e) < len ? v[e] : -INFINITY;
+  }
+  // the largest values of the thread's groups of 8 (fmaxf leaves NaN out: a NaN makes
+  // the sums NaN)
+  float group[E / 8], most = -INFINITY;
 #pragma unroll
   for (int i = 0; i < E / 8; ++i) {
-    const int at = elem_of(8 * i);
-    if (kAligned && at + 8 <= len) {
-      if constexpr (sizeof(T) == 2) {
-        const uint4 u = *reinterpret_cast<const uint4*>(x + at);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    group[i] = v[8 * i];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[8 * i + 2 * j] = u2f(w[j] << 16);
-          v[8 * i + 2 * j + 1] = u2f(w[j] & 0xffff0000u);
-        }
-      } else {
-        const float4 f = *reinterpret_cast<const float4*>(x + at);
-        const float4 h = *reinterpret_cast<const float4*>(x + at + 4);
-        v[8 * i] = f.x, v[8 * i + 1] = f.y, v[8 * i + 2] = f.z, v[8 * i + 3] = f.w;
-        v[8 * i + 4] = h.x, v[8 * i + 5] = h.y, v[8 * i + 6] = h.z, v[8 * i + 7] = h.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[8 * i + j] = at + j < len ? logit<T>(x, at + j) : -INFINITY;
-      }
-    }
+    for (int j = 1; j < 8; ++j) group[i] = fmaxf(group[i], v[8 * i + j]);
+    most = fmaxf(most, group[i]);
   }
-  if (threadIdx.x == 0) s_n = 0;
-
-  // the largest value, the sums
-  float most = v[0];
-#pragma unroll
-  for (int e = 1; e < E; ++e) most = nan_max(most, v[e]);
-  const float lane_most = most;
-  most = wave_nan_max(most);
+  most = wave_max_f32(most);
   if (lane == 0) s_f[0][wave] = most;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) most = nan_max(most, s_f[0][w]);
-  const float inv_t = a.temps ? 1.0f / a.temps[row] : 1.0f;
-  const float m = most * inv_t;
+  most = fmaxf(fmaxf(s_f[0][0], s_f[0][1]), fmaxf(s_f[0][2], s_f[0][3]));
+  const float c = a.temps ? kLog2e / a.temps[row] : kLog2e;
+  const float ref = most == -INFINITY ? 0.0f : most;
   float S = 0.0f, U = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const float d = v[e] * inv_t - m;
-    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+    const float d = (v[e] - ref) * c;
+    const float p = __builtin_amdgcn_exp2f(d);
     S += p;
-    U += p == 0.0f ? 0.0f : p * d;  // an excluded token's -inf takes no part
+    // far below, where p is 0, d may be -inf: it takes no part
+    U = fmaf(p, fmaxf(d, -512.0f), U);
+  }
+  if (!(S < INFINITY)) {
+    // a NaN among the thread's values, perhaps: its groups, and no others, count as
+    // +inf, for they do hold a value that no other is above
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (v[e] != v[e]) group[e >> 3] = INFINITY;
   }
   S = wave_sum(S);
   U = wave_sum(U);
   if (lane == 0) s_f[1][wave] = S, s_f[2][wave] = U;
-
   if (a.top > 0) {
-    // the top-th largest lane maximum of the wave, by its bits from the highest
-    const uint32_t mine = order_key(lane_most);
-    uint32_t bar = 0;
+    // four neighbouring lanes hold a group, and lane i of them writes the i-th
+    float mine = -INFINITY;
 #pragma unroll
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t trial = bar | (1u << b);
-      if (__popcll(__ballot(mine >= trial)) >= a.top) bar = trial;
+    for (int i = 0; i < E / 8; ++i) {
+      float g = group[i];
+      g = fmaxf(g, quad_xor<0xB1>(g));
+      g = fmaxf(g, quad_xor<0x4E>(g));
+      if ((lane & 3) == i) mine = g;
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t key = order_key(v[e]);
-      const int id = elem_of(e);
-      if (key >= bar && id < len) {
-        const int at = atomicAdd(&s_n, 1);
-        if (at < kListed) {
-          s_key[at] = key;
-          s_id[at] = id;
-        }
-      }
-    }
+    if ((lane & 3) < E / 8)
+      a.most[(int64_t)row * a.groups + (base + 8 * ((lane & 3) * kLpT + ((int)threadIdx.x & ~3))) / kGroup] =
+          order_key(mine);
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const int64_t o = (int64_t)row * a.chunks + chunk;
-    a.sums[o] = make_float4(m, (s_f[1][0] + s_f[1][1]) + (s_f[1][2] + s_f[1][3]),
-                            (s_f[2][0] + s_f[2][1]) + (s_f[2][2] + s_f[2][3]), 0.0f);
-  }
-  if (a.top > 0) {
-    const int n = s_n;
-    const int64_t o = ((int64_t)row * a.chunks + chunk) * a.top;
-    if (n <= kListed) {
-      for (int c = threadIdx.x; c < n; c += kLpT) {
-        const uint32_t key = s_key[c];
-        const int id = s_id[c];
-        int rank = 0;
-        for (int i = 0; i < n && rank < a.top; ++i)
-          rank += s_key[i] > key || (s_key[i] == key && s_id[i] < id);
-        if (rank < a.top) {
-          a.keys[o + rank] = key;
-          a.ids[o + rank] = base + id;
-        }
-      }
-      // a short last chunk has fewer: key 0 stands for none (no value has it)
-      for (int r = n + threadIdx.x; r < a.top; r += kLpT) {
-        a.keys[o + r] = 0;
-        a.ids[o + r] = 0x7fffffff;
-      }
-    } else {
-      uint32_t last_key = 0xffffffffu;
-      int last_id = -1;
-      for (int r = 0; r < a.top; ++r) {
-        uint32_t key = 0;
-        int id = 0x7fffffff;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t k = order_key(v[e]);
-          const int i = elem_of(e);
-          const bool behind = k < last_key || (k == last_key && i > last_id);
-          if (behind && i < len && (k > key || (k == key && i < id))) key = k, id = i;
-        }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-          const uint32_t k = (uint32_t)__shfl_xor((int)key, d, 64);
-          const int i = __shfl_xor(id, d, 64);
-          if (k > key || (k == key && i < id)) key = k, id = i;
-        }
-        __syncthreads();  // the last round's reads
-        if (lane == 0) s_key[wave] = key, s_id[wave] = id;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t k = s_key[w];
-          const int i = s_id[w];
-          if (k > key || (k == key && i < id)) key = k, id = i;
-        }
-        if (threadIdx.x == 0) a.keys[o + r] = key, a.ids[o + r] = base + id;
-        last_key = key;
-        last_id = id;
-      }
+  if (threadIdx.x == 0)
+    a.sums[(int64_t)row * a.chunks + chunk] =
+        make_float4(most, (s_f[1][0] + s_f[1][1]) + (s_f[1][2] + s_f[1][3]),
+                    (s_f[2][0] + s_f[2][1]) + (s_f[2][2] + s_f[2][3]), 0.0f);
+}
+
+// The `top` largest of a row with many equal ones: value by value, the ids of one in
+// order. s_n: a shared counter of four.
+template <typename T>
+__device__ void top_by_value(const LogprobArgs& a, const T* x, int64_t* ids, int* s_n) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t last = 1ull << 32;  // orders from here on are done
+  int filled = 0;
+  while (filled < a.top) {
+    uint32_t best = 0;
+    for (int i = threadIdx.x; i < a.vocab; i += kLpT) {
+      const uint32_t k = order_key(logit<T>(x, i));
+      if (k < last && k > best) best = k;
     }
+    best = wave_max_u32(best);
+    __syncthreads();
+    if (lane == 0) s_n[wave] = (int)best;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) best = max(best, (uint32_t)s_n[w]);
+    for (int i = 0; i < a.vocab && filled < a.top; i += kLpT) {
+      const int id = i + (int)threadIdx.x;
+      const bool take = id < a.vocab && order_key(logit<T>(x, id)) == best;
+      const uint64_t all = __ballot(take);
+      __syncthreads();
+      if (lane == 0) s_n[wave] = __popcll(all);
+      __syncthreads();
+      int to = filled + __popcll(all & ((1ull << lane) - 1));
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) to += s_n[w];
+        filled += s_n[w];
+      }
+      if (take && to < a.top) ids[to] = id;
+    }
+    last = best;
   }
 }
 
-// One wave a row.
 template <typename T>
-__global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a) {
-  const int lane = threadIdx.x, row = blockIdx.x;
-  const float4* sums = a.sums + (int64_t)row * a.chunks;
-  float m = -INFINITY;
-  for (int c = lane; c < a.chunks; c += 64) m = nan_max(m, sums[c].x);
-  m = wave_nan_max(m);
-  float S = 0.0f, U = 0.0f;
-  for (int c = lane; c < a.chunks; c += 64) {
-    const float4 s = sums[c];
-    // sums under the chunk's maximum, moved to the row's
-    const float d = s.x - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
-    S += f == 0.0f ? 0.0f : f * s.y;
-    U += f == 0.0f ? 0.0f : f * (s.z + d * s.y);
-  }
-  S = wave_sum(S);
-  U = wave_sum(U);
-  const float log_s = logf(S);
-  const float inv_t = a.temps ? 1.0f / a.temps[row] : 1.0f;
+__global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
+  __shared__ uint4 s_most[kLpT / 4];
+  __shared__ int s_group[kListed];
+  __shared__ uint64_t s_list[kListed];
+  __shared__ int s_n[4];
+  __shared__ float s_f[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x;
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride;
-  if (lane == 0) {
-    if (a.entropy) a.entropy[row] = log_s - U / S;
-    if (a.logprobs) {
-      const int64_t tok = a.tokens[row];
-      float lp = -INFINITY;  // a token that the vocabulary does not have
-      if (tok >= 0 && tok < a.vocab) lp = (logit<T>(x, tok) * inv_t - m) - log_s;
-      a.logprobs[row] = lp;
+  const float c = a.temps ? kLog2e / a.temps[row] : kLog2e;
+  const uint32_t* most = a.most + (int64_t)row * a.groups;
+  if (a.top > 0) {
+    uint32_t mine = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.groups; i += kLpT) mine = max(mine, most[i]);
+    reinterpret_cast<uint32_t*>(s_most)[threadIdx.x] = mine;
+    if (threadIdx.x < 4) s_n[threadIdx.x] = 0;
+  }
+  if (wave == 3) {
+    const float4* sums = a.sums + (int64_t)row * a.chunks;
+    float m = -INFINITY;
+    for (int i = lane; i < a.chunks; i += 64) m = fmaxf(m, sums[i].x);
+    m = wave_max_f32(m);
+    float S = 0.0f, U = 0.0f;
+    for (int i = lane; i < a.chunks; i += 64) {
+      const float4 s = sums[i];
+      // sums under the chunk's maximum, moved to the row's
+      const float d = (s.x - m) * c, f = __builtin_amdgcn_exp2f(d);
+      S += f == 0.0f ? 0.0f : f * s.y;
+      U += f == 0.0f ? 0.0f : f * (s.z + d * s.y);
+    }
+    S = wave_sum(S);
+    U = wave_sum(U);
+    if (lane == 0) {
+      const float log_s = log2f(S);
+      if (a.entropy) a.entropy[row] = (log_s - U / S) * kLn2;
+      if (a.logprobs) {
+        const int64_t tok = a.tokens[row];
+        float lp = -INFINITY;  // a token that the vocabulary does not have
+        if (tok >= 0 && tok < a.vocab) lp = ((logit<T>(x, tok) - m) * c - log_s) * kLn2;
+        a.logprobs[row] = lp;
+      }
+      s_f[0] = m;
+      s_f[1] = log_s;
     }
   }
   if (a.top == 0) return;
-  // The chunks' lists are in order and a lane's best is the first of one of its lists.
-  // Only lanes whose best is among the `top` best ones can hold one of the row's.
-  __shared__ uint32_t s_key[kMaxTop * kPerLane * kMaxTop];
-  __shared__ int s_id[kMaxTop * kPerLane * kMaxTop];
-  __shared__ int s_n;
-  const uint32_t* keys = a.keys + (int64_t)row * a.chunks * a.top;
-  const int32_t* ids = a.ids + (int64_t)row * a.chunks * a.top;
-  if (lane == 0) s_n = 0;
-  uint32_t key = 0;
-  int id = 0x7fffffff;
+  __syncthreads();
+
+  // the bar, by the upper half of the order's bits (a bf16's all; the lower bound that
+  // is left of an f32's serves as well)
+  const uint4 k = s_most[lane];
+  uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int c = lane + 64 * i;
-    if (c < a.chunks) {
-      const uint32_t k = keys[c * a.top];
-      const int d = ids[c * a.top];
-      if (k > key || (k == key && d < id)) key = k, id = d;
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t trial = bits | (1u << b);
+    if (__popcll(__ballot(k.x >= trial)) + __popcll(__ballot(k.y >= trial)) +
+            __popcll(__ballot(k.z >= trial)) + __popcll(__ballot(k.w >= trial)) >= a.top)
+      bits = trial;
+  }
+  float bar = hs_unkey(bits);
+  // fewer than `top` threads' shares hold anything above -inf: all such values
+  if (bar != bar || bar == -INFINITY) bar = -3.402823466e38f;
+  const uint32_t reach = max(bits, order_key(-3.402823466e38f));
+  for (int i = threadIdx.x; i < a.groups; i += kLpT) {
+    if (most[i] >= reach) {
+      const int at = atomicAdd(&s_n[0], 1);
+      if (at < kListed) s_group[at] = i;
     }
   }
-  uint32_t bar = 0;
-#pragma unroll
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t trial = bar | (1u << b);
-    if (__popcll(__ballot(key >= trial)) >= a.top) bar = trial;
-  }
-  // of the lanes at the bar, as many as are left, those of the lowest ids
-  const int left = a.top - __popcll(__ballot(key > bar));
-  uint32_t first = 0;  // the ids below it are those of fewer than `left` lanes
-#pragma unroll
-  for (int b = 30; b >= 0; --b) {
-    const uint32_t trial = first | (1u << b);
-    if (__popcll(__ballot(key == bar && (uint32_t)id < trial)) < left) first = trial;
-  }
   __syncthreads();
-  if (key > bar || (key == bar && key != 0 && (uint32_t)id <= first)) {
-    for (int i = 0; i < kPerLane; ++i) {
-      const int c = lane + 64 * i;
-      if (c >= a.chunks) break;
-      for (int r = 0; r < a.top; ++r) {
-        const uint32_t k = keys[c * a.top + r];
-        if (k == 0 || k < bar) break;
-        const int at = atomicAdd(&s_n, 1);
-        s_key[at] = k;
-        s_id[at] = ids[c * a.top + r];
+  const int groups = s_n[0];
+  for (int i = threadIdx.x / kGroup; i < min(groups, kListed); i += kLpT / kGroup) {
+    const int id = s_group[i] * kGroup + (threadIdx.x & (kGroup - 1));
+    if (id < a.vocab) {
+      const float f = logit<T>(x, id);
+      if (!(f < bar)) {
+        const int at = atomicAdd(&s_n[1], 1);
+        if (at < kListed) s_list[at] = listing(order_key(f), id);
       }
     }
   }
   __syncthreads();
-  const int n = s_n;
-  for (int c = lane; c < n; c += 64) {
-    const uint32_t k = s_key[c];
-    const int d = s_id[c];
-    int rank = 0;
-    for (int i = 0; i < n && rank < a.top; ++i)
-      rank += s_key[i] > k || (s_key[i] == k && s_id[i] < d);
-    if (rank < a.top) {
-      a.top_ids[(int64_t)row * a.top + rank] = d;
-      a.top_logprobs[(int64_t)row * a.top + rank] = (logit<T>(x, d) * inv_t - m) - log_s;
+  const int n = s_n[1];
+  int64_t* ids = a.top_ids + (int64_t)row * a.top;
+  if (groups > kListed || n > kListed) {
+    top_by_value<T>(a, x, ids, s_n);
+  } else {
+    for (int i = threadIdx.x; i < n; i += kLpT) {
+      const uint64_t own = s_list[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += s_list[j] > own;
+      if (rank < a.top) ids[rank] = (int)~(uint32_t)own;
     }
+    if (n < a.top && wave == 0) {  // then the first of the -inf ones
+      int filled = n;
+      for (int i = 0; i < a.vocab && filled < a.top; i += 64) {
+        const bool out = i + lane < a.vocab && logit<T>(x, min(i + lane, a.vocab - 1)) == -INFINITY;
+        const uint64_t all = __ballot(out);
+        const int to = filled + __popcll(all & ((1ull << lane) - 1));
+        if (out && to < a.top) ids[to] = i + lane;
+        filled += __popcll(all);
+      }
+    }
+  }
+  __syncthreads();  // the ids, written by this workgroup
+  if (threadIdx.x < a.top) {
+    const int64_t id = ids[threadIdx.x];
+    a.top_logprobs[(int64_t)row * a.top + threadIdx.x] =
+        ((logit<T>(x, id) - s_f[0]) * c - s_f[1]) * kLn2;
   }
 }
 
-// values a thread: short chunks while there are few rows to fill the chip with, but
-// at most 256 chunks a row
+// values a thread: short chunks while there are few rows to fill the chip with
 int elems_of(int rows, int vocab) {
-  const int64_t small = (int64_t)rows * ((vocab + 8 * kLpT - 1) / (8 * kLpT));
-  if (small <= 2048 && vocab <= 256 * 8 * kLpT) return 8;
+  for (int e = 8; e < 32; e *= 2) {
+    const int64_t chunks = ((int64_t)vocab + e * kLpT - 1) / (e * kLpT);
+    if (rows * chunks <= 64 * e) return e;
+  }
   return 32;
 }
 int chunks_of(int rows, int vocab) {
@@ -347,7 +360,9 @@ extern "C" {
 
 size_t hs_token_logprobs_workspace_size(int rows, int vocab, int top) {
   if (!sizes_ok(rows, vocab, top)) return 0;
-  return (size_t)rows * chunks_of(rows, vocab) * (sizeof(float4) + (size_t)top * 8);
+  const size_t chunks = chunks_of(rows, vocab);
+  const size_t groups = top ? chunks * elems_of(rows, vocab) * kLpT / kGroup : 0;
+  return rows * (chunks * sizeof(float4) + groups * 4);
 }
 
 int hs_token_logprobs(const void* logits, int logits_dtype, int64_t logits_row_stride, int rows,
@@ -362,8 +377,8 @@ int hs_token_logprobs(const void* logits, int logits_dtype, int64_t logits_row_s
   if (logits_row_stride < vocab) return HS_ERR_INVALID;
   const int esz = logits_dtype == HS_BF16 ? 2 : 4;
   if ((uintptr_t)logits & (esz - 1)) return HS_ERR_UNSUPPORTED;
-  // 256 chunks of 8192 values a row, a grid's second dimension of rows
-  if (rows > 65535 || vocab > 256 * 32 * kLpT) return HS_ERR_UNSUPPORTED;
+  // a grid's second dimension of rows
+  if (rows > 65535 || vocab > (1 << 21)) return HS_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < hs_token_logprobs_workspace_size(rows, vocab, top))
     return HS_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return HS_ERR_UNSUPPORTED;
@@ -380,24 +395,25 @@ int hs_token_logprobs(const void* logits, int logits_dtype, int64_t logits_row_s
   a.entropy = entropy;
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
-  const size_t n = (size_t)rows * a.chunks;
+  a.groups = a.chunks * elems_of(rows, vocab) * kLpT / kGroup;
   a.sums = static_cast<float4*>(workspace);
-  a.keys = reinterpret_cast<uint32_t*>(a.sums + n);
-  a.ids = reinterpret_cast<int32_t*>(a.keys + n * top);
+  a.most = reinterpret_cast<uint32_t*>(a.sums + (size_t)rows * a.chunks);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // 16-byte loads of every row
   const bool aligned = !(((uintptr_t)logits | (uint64_t)(logits_row_stride * esz)) & 15);
-  const bool wide = elems_of(rows, vocab) == 32;
+  const int e = elems_of(rows, vocab);
   if (esz == 2) {
-    if (wide) launch<uint16_t, 32>(a, aligned, s);
+    if (e == 32) launch<uint16_t, 32>(a, aligned, s);
+    else if (e == 16) launch<uint16_t, 16>(a, aligned, s);
     else launch<uint16_t, 8>(a, aligned, s);
   } else {
-    if (wide) launch<float, 32>(a, aligned, s);
+    if (e == 32) launch<float, 32>(a, aligned, s);
+    else if (e == 16) launch<float, 16>(a, aligned, s);
     else launch<float, 8>(a, aligned, s);
   }
   if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
-  if (esz == 2) hipLaunchKernelGGL(k_logprobs_join<uint16_t>, dim3((unsigned)rows), dim3(64), 0, s, a);
-  else hipLaunchKernelGGL(k_logprobs_join<float>, dim3((unsigned)rows), dim3(64), 0, s, a);
+  if (esz == 2) hipLaunchKernelGGL(k_logprobs_join<uint16_t>, dim3((unsigned)rows), dim3(kLpT), 0, s, a);
+  else hipLaunchKernelGGL(k_logprobs_join<float>, dim3((unsigned)rows), dim3(kLpT), 0, s, a);
   return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 

@@ -2,13 +2,14 @@
 
 Each wrapper validates shapes on the host, passes raw device pointers and the
 current HIP stream to libhilda_spec.so and raises RuntimeError on any non-zero
-status. Workspaces (intermediate partial results only, no initialisation
-needed) are allocated once per (device, kind) and reused; calls on one device
-are ordered by the current stream.
+status. Workspaces are allocated once per (device, kind) and reused, and calls on
+one device are ordered by the current stream; the entry points whose workspace
+needs no preparation (store_kvcache_scaled, verify_attention_scaled, linear_int4,
+token_logprobs) take one of the call's own.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -25,7 +26,7 @@ def _dev_index(device) -> int:
     without an index means the current device, as torch resolves it for tensors."""
     if isinstance(device, int):
         return device
-    d = torch.device(device)
+    d = device if isinstance(device, torch.device) else torch.device(device)
     if d.index is not None:
         return d.index
     try:
@@ -48,7 +49,8 @@ def workspace(device: torch.device, nbytes: int, kind: str) -> torch.Tensor:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the current stream's handle without the Stream object around it (0.1 us, not 1.9)
+    return torch._C._cuda_getCurrentRawStream(_dev_index(device))
 
 
 def _logit_dtype(t: torch.Tensor) -> int:
@@ -328,20 +330,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     if tokens is not None:
         if tokens.numel() != rows or tokens.is_floating_point() or tokens.dtype == torch.bool:
             raise ValueError("tokens must be one integer a row")
-        tokens = tokens.to(torch.int64).reshape(rows).contiguous()
+        if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+            tokens = tokens.to(torch.int64).contiguous()
     if temperatures is not None:
         if temperatures.numel() != rows:
             raise ValueError("temperatures must be one a row")
-        temperatures = temperatures.to(torch.float32).reshape(rows).contiguous()
-    f32 = dict(dtype=torch.float32, device=dev)
-    lp = torch.empty(rows, **f32) if tokens is not None else None
-    ent = torch.empty(rows, **f32)
-    ids = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
-    tlp = torch.empty((rows, top), **f32) if top else None
+        if temperatures.dtype != torch.float32 or not temperatures.is_contiguous():
+            temperatures = temperatures.to(torch.float32).contiguous()
+    f32 = torch.float32
+    lp = logits.new_empty(rows, dtype=f32) if tokens is not None else None
+    ent = logits.new_empty(rows, dtype=f32)
+    ids = logits.new_empty((rows, top), dtype=torch.int64) if top else None
+    tlp = logits.new_empty((rows, top), dtype=f32) if top else None
     if rows:
         lg, lstride = _rows2d(logits, rows, V)
         nbytes = L.lib().hs_token_logprobs_workspace_size(rows, V, top)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = logits.new_empty(nbytes, dtype=torch.uint8)
 
         def p(t):
             return None if t is None else t.data_ptr()
@@ -452,30 +456,39 @@ def _call(dev: torch.device, what: str, *args) -> None:
     current device."""
     fn = getattr(L.lib(), what)
     if dev.index == torch.cuda.current_device():
-        L.check(fn(*args, _stream(dev)), what)
+        status = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            L.check(fn(*args, _stream(dev)), what)
+            status = fn(*args, _stream(dev))
+    if status:
+        L.check(status, what)
+
+
+def _as_int32(t: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _scaled_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
-                  v_scales: torch.Tensor) -> int:
-    """Checks an 8-bit cache with group scales; returns the group (tokens per scale)."""
+                  v_scales: torch.Tensor):
+    """Checks an 8-bit cache with group scales; returns the cache's shape and strides,
+    the scales' strides and the group (tokens per scale)."""
     if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
         raise TypeError("a cache with group scales must be float8_e4m3fn")
     if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
         raise TypeError("k_scales / v_scales must be float32")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or \
-            k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or strides != v_cache.stride() or strides[3] != 1:
         raise ValueError("k_cache and v_cache must be [blocks, block_size, kv_heads, head_dim] "
                          "with identical strides and contiguous head_dim")
-    nb, bs, Hkv, _ = k_cache.shape
-    if k_scales.dim() != 3 or k_scales.shape != v_scales.shape or \
-            k_scales.stride() != v_scales.stride() or k_scales.shape[0] != nb or \
-            k_scales.shape[2] != Hkv or k_scales.shape[1] < 1 or bs % k_scales.shape[1]:
+    sshape, sstrides = k_scales.shape, k_scales.stride()
+    if len(sshape) != 3 or sshape != v_scales.shape or sstrides != v_scales.stride() or \
+            sshape[0] != shape[0] or sshape[2] != shape[2] or sshape[1] < 1 or \
+            shape[1] % sshape[1]:
         raise ValueError("k_scales and v_scales must be [blocks, block_size / group, kv_heads] "
                          "with identical strides")
-    return bs // k_scales.shape[1]
+    return shape, strides, sstrides, shape[1] // sshape[1]
 
 
 def store_kvcache_scaled(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -493,19 +506,18 @@ def store_kvcache_scaled(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
     if key.dim() != 3 or key.shape != value.shape or key.stride(2) != 1 or value.stride(2) != 1:
         raise ValueError("key and value must be [tokens, kv_heads, head_dim] with contiguous "
                          "head_dim")
-    group = _scaled_cache(k_cache, v_cache, k_scales, v_scales)
+    (nb, bs, Hc, Dc), cst, sst, group = _scaled_cache(k_cache, v_cache, k_scales, v_scales)
     N, Hkv, D = key.shape
-    nb, bs, Hc, Dc = k_cache.shape
-    if (Hc, Dc) != (Hkv, D):
+    if Hc != Hkv or Dc != D:
         raise ValueError("cache geometry mismatch")
     if slot_mapping.numel() != N:
         raise ValueError("slot_mapping must have one entry per token")
-    sm = slot_mapping.to(torch.int32).contiguous()
-    _call(dev, "hs_store_kvcache_scaled", key.data_ptr(), key.stride(0), key.stride(1),
-          value.data_ptr(), value.stride(0), value.stride(1), k_cache.data_ptr(),
-          v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-          k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1),
-          k_scales.stride(2), group, sm.data_ptr(), N, Hkv, D, bs, nb)
+    sm = _as_int32(slot_mapping)
+    kst, vst = key.stride(), value.stride()
+    _call(dev, "hs_store_kvcache_scaled", key.data_ptr(), kst[0], kst[1], value.data_ptr(), vst[0],
+          vst[1], k_cache.data_ptr(), v_cache.data_ptr(), cst[0], cst[1], cst[2],
+          k_scales.data_ptr(), v_scales.data_ptr(), sst[0], sst[1], sst[2], group, sm.data_ptr(),
+          N, Hkv, D, bs, nb)
 
 
 def verify_attention_scaled(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -523,39 +535,37 @@ def verify_attention_scaled(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     captured graphs."""
     dev = _need_cuda(q, k_cache, v_cache, k_scales, v_scales, block_tables, cu_seqlens_q,
                      cu_seqlens_k, out)
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
+    qst = q.stride()
+    if q.dtype != torch.bfloat16 or len(qst) != 3 or qst[2] != 1:
         raise ValueError("q must be [tokens, heads, head_dim] bf16 with contiguous head_dim")
-    group = _scaled_cache(k_cache, v_cache, k_scales, v_scales)
+    (nb, bs, Hkv, Dc), cst, sst, group = _scaled_cache(k_cache, v_cache, k_scales, v_scales)
     N, Hq, D = q.shape
-    nb, bs, Hkv, Dc = k_cache.shape
     if D != Dc:
         raise ValueError("head_dim mismatch")
     B = cu_seqlens_q.numel() - 1
     if B < 1 or cu_seqlens_k.numel() != B + 1:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have one more entry than sequences")
-    cq = cu_seqlens_q.to(torch.int32).contiguous()
-    ck = cu_seqlens_k.to(torch.int32).contiguous()
+    cq, ck = _as_int32(cu_seqlens_q), _as_int32(cu_seqlens_k)
     bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
     if bt.dim() != 2 or bt.shape[0] < B:
         raise ValueError("block_tables must be [sequences, blocks]")
     if bt.stride(1) != 1:
         bt = bt.contiguous()
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((N, Hq, D))
     elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1:
         raise ValueError("out must have q's shape, bf16 with contiguous head_dim")
     if N == 0:
         return out
     mq, mk = int(max_seqlen_q), int(max_seqlen_k)
     nbytes = L.lib().hs_verify_attention_scaled_workspace_size(B, Hq, Hkv, mq, mk)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, "hs_verify_attention_scaled", q.data_ptr(), q.stride(0), q.stride(1),
-          k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
-          k_cache.stride(2), k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0),
-          k_scales.stride(1), k_scales.stride(2), group, bt.data_ptr(), bt.stride(0), bt.shape[1],
-          nb, cq.data_ptr(), ck.data_ptr(), B, mq, mk, Hq, Hkv, D, bs, float(softmax_scale),
-          out.data_ptr(), out.stride(0), out.stride(1), None if ws is None else ws.data_ptr(),
-          nbytes)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    ost = out.stride()
+    _call(dev, "hs_verify_attention_scaled", q.data_ptr(), qst[0], qst[1], k_cache.data_ptr(),
+          v_cache.data_ptr(), cst[0], cst[1], cst[2], k_scales.data_ptr(), v_scales.data_ptr(),
+          sst[0], sst[1], sst[2], group, bt.data_ptr(), bt.stride(0), bt.shape[1], nb,
+          cq.data_ptr(), ck.data_ptr(), B, mq, mk, Hq, Hkv, D, bs, float(softmax_scale),
+          out.data_ptr(), ost[0], ost[1], ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
@@ -977,8 +987,7 @@ def linear_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: float, weigh
     return out, (x if residual is None else res_out)
 
 
-@dataclass(frozen=True)
-class Int4Weight:
+class Int4Weight(NamedTuple):
     """A projection's weight in 4 bits with group scales, in the layout of
     hs_linear_int4: packed int32 [tiles, steps, 64, 4] and scales bf16
     [tiles, groups, 16] over 16-feature tiles and 128-input steps. pack_int4 and
@@ -1040,8 +1049,8 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, *, swiglu: bool = False,
     rows -> [rows, N] bf16, fp32 accumulation. With swiglu=True the weight is
     [2F, K] (gate | up), F a multiple of 16, and the result silu(gate) * up
     [rows, F]. An infinity in a row of x gives NaN in that row."""
-    w = weight
-    dev = _need_cuda(x, w.packed, w.scales, out)
+    w, packed, scales = weight, weight.packed, weight.scales
+    dev = _need_cuda(x, packed, scales, out)
     if x.dim() != 2 or x.dtype != torch.bfloat16:
         raise ValueError("linear_int4 expects a 2-D bf16 input")
     M, K = x.shape
@@ -1050,24 +1059,24 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, *, swiglu: bool = False,
     if swiglu and w.out_features % 32:
         raise ValueError("swiglu needs gate and up halves of a multiple of 16 features")
     tiles, steps = -(-w.out_features // 16), -(-K // 128)
-    if w.group not in (32, 64, 128) or w.packed.dtype != torch.int32 or \
-            w.scales.dtype != torch.bfloat16 or w.packed.shape != (tiles, steps, 64, 4) or \
-            w.scales.shape != (tiles, steps * (128 // w.group), 16) or \
-            not w.packed.is_contiguous() or not w.scales.is_contiguous():
+    if w.group not in (32, 64, 128) or packed.dtype != torch.int32 or \
+            scales.dtype != torch.bfloat16 or packed.shape != (tiles, steps, 64, 4) or \
+            scales.shape != (tiles, steps * (128 // w.group), 16) or \
+            not packed.is_contiguous() or not scales.is_contiguous():
         raise ValueError("weight is not laid out as pack_int4 does")
     N = w.out_features // 2 if swiglu else w.out_features
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        out = x.new_empty((M, N))
     elif out.shape != (M, N) or out.stride(1) != 1 or out.dtype != torch.bfloat16:
         raise ValueError("out must be [rows, out_features] bf16 with contiguous rows")
     if M == 0:
         return out
     epi = L.HS_LINEAR_SWIGLU if swiglu else L.HS_LINEAR_PLAIN
-    nbytes = L.lib().hs_linear_int4_workspace_size(M, K, N, epi) if M > 16 else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, "hs_linear_int4", x.data_ptr(), x.stride(0), w.packed.data_ptr(),
-          w.scales.data_ptr(), M, K, N, w.group, epi, out.data_ptr(), out.stride(0),
-          None if ws is None else ws.data_ptr(), nbytes)
+    nbytes = L.lib().hs_linear_int4_workspace_size(M, K, N, epi)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call(dev, "hs_linear_int4", x.data_ptr(), x.stride(0), packed.data_ptr(), scales.data_ptr(),
+          M, K, N, w.group, epi, out.data_ptr(), out.stride(0),
+          ws.data_ptr() if nbytes else None, nbytes)
     return out

@@ -111,6 +111,19 @@ def test_rows_at_the_edges(hv, cuda, rows):
         _check(got, y, tokens, top, None)
 
 
+@pytest.mark.parametrize("rows", [3, 300])
+def test_alternatives_do_not_go_by_the_temperature(hv, cuda, rows):
+    """The order is that of the logits, also where a temperature outside its domain leaves
+    no log-probabilities."""
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(rows, 9001, generator=gen)
+    ids = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :20]
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-30):
+        got = hv.ops.token_logprobs(x.to(cuda), top=20,
+                                    temperatures=torch.full((rows,), t, device=cuda))
+        assert torch.equal(got["top_ids"].cpu(), ids)
+
+
 def test_arguments_left_out(hv, cuda):
     x = torch.randn(3, 500, device=cuda)
     r = hv.ops.token_logprobs(x)

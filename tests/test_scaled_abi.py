@@ -60,7 +60,7 @@ def test_wrappers_refuse_what_is_not_such_a_cache(hv):
     ops = hv.ops
     c = torch.zeros(2, 256, 2, 128).to(torch.float8_e4m3fn)
     s = torch.zeros(2, 8, 2)
-    assert ops._scaled_cache(c, c, s, s) == 32
+    assert ops._scaled_cache(c, c, s, s)[3] == 32
     with pytest.raises(TypeError):
         ops._scaled_cache(c.to(torch.bfloat16), c, s, s)
     with pytest.raises(TypeError):
