@@ -6,20 +6,22 @@
 //   o_i  = sum_j p_ij vs[g(j)] vc_j / sum_j p_ij,  p_ij = exp(s_ij - max_j s_ij)
 // Codes are decoded exactly to bf16 (every e4m3 value is one) and multiplied on
 // the matrix cores with f32 accumulation; a window of 32 keys lies in one group,
-// so its scales are two scalars: ks joins the softmax scale, vs the
-// probabilities, which round to bf16 once, as the product's second operand.
-// Statistics, sums and partial results are f32.
+// so its scales are two scalars: ks joins the softmax scale, and the power of two in vs
+// the decoding of V (what a scale of another producer has besides multiplies the
+// probabilities). The probabilities round to bf16 as the product's second operand;
+// statistics, sums and partial results are f32.
 //
 // A wave works on its own, without LDS in its loop. It takes a window's K rows as
 // the A operand of S^T = K Q^T (lane l: key l % 16, dims 32 (l / 16) .. + 31, two
 // 16-byte loads) and its V rows as 8 keys x 8 dims a lane (8 loads of 8 bytes, 16
 // lanes to a cache line); byte permutes transpose those 8 x 8 codes in registers
 // into the A operand of O^T = V^T P^T, whose key order is chosen so that the lane's
-// own probabilities are its B operand. The next window is loaded while this one is
-// computed.
+// own probabilities are its B operand. A window's K registers take the next window's K
+// as soon as its scores are there, its V registers the next V after its product, so a
+// window costs 32 registers and enough waves fit to hide the loads.
 //
 //  * k_scaled_split: decode and verify rows, 16 query rows (head of the kv head's
-//    group, token) to a tile. A workgroup of 8 waves takes `split_len` keys of a
+//    group, token) to a tile. A workgroup of 4 waves takes `split_len` keys of a
 //    (sequence, kv head, tile), its waves interleaved over the windows, and joins
 //    their results in LDS; k_scaled_combine joins the splits' partials. The partials
 //    are written before they are read and nothing is counted between the launches,
@@ -42,7 +44,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kD = 128;    // head size
 constexpr int kWin = 32;   // keys of a window
 constexpr int kRows = 16;  // query rows of a tile
-constexpr int kSplitWaves = 8;
+constexpr int kSplitWaves = 4;
 constexpr int kRowWaves = 4;
 
 struct ScaledAttnArgs {
@@ -59,7 +61,7 @@ struct ScaledAttnArgs {
   int bt_width, num_blocks;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  int Hkv, G, block_size;
+  int num_seqs, Hkv, G, block_size;
   int bs_shift;  // log2(block_size) for powers of two, else -1
   int g_shift;   // log2(group)
   float scale_log2;  // softmax_scale * log2(e)
@@ -94,17 +96,16 @@ __device__ __forceinline__ float quad_max(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 
-__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, bool high) {
-  const bf16x2_t p = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true)
-                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false);
+// two codes (of the lower or upper half) times the power of two in `scale`
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, bool high, float scale) {
+  const bf16x2_t p = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false);
   return __builtin_bit_cast(uint32_t, p);
+}
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), bf16x2_t));
 }
 union Frag {
   uint32_t u[4];
@@ -112,69 +113,70 @@ union Frag {
 };
 __device__ __forceinline__ bf16x8_t decode8(uint32_t lo, uint32_t hi) {
   Frag f;
-  f.u[0] = bf16_pair(lo, false);
-  f.u[1] = bf16_pair(lo, true);
-  f.u[2] = bf16_pair(hi, false);
-  f.u[3] = bf16_pair(hi, true);
+  f.u[0] = bf16_pair(lo, false, 1.0f);
+  f.u[1] = bf16_pair(lo, true, 1.0f);
+  f.u[2] = bf16_pair(hi, false, 1.0f);
+  f.u[3] = bf16_pair(hi, true, 1.0f);
   return f.v;
 }
 
 // A window as a lane holds it. K: rows l % 16 and 16 + l % 16, 32 bytes each. V: 8
 // bytes (dims 8 (l % 16) ..) of keys 4g + e and 16 + 4g + e, g = l / 16, e < 4.
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 struct Win {
-  uint4 k[4];
-  uint2 v[8];
-  float ks, vs;
+  u32x4_t k[4];
+  u32x2_t v[8];
 };
 
-// Where a window lies: its block's rows and its group's scales; `ok` is false where
-// the table has no such block, and nothing of the window is then used.
-struct Place {
-  int blk;
-  bool ok;
-};
 __device__ __forceinline__ int block_of(const ScaledAttnArgs& a, int key) {
   return a.bs_shift >= 0 ? key >> a.bs_shift : key / a.block_size;
 }
-__device__ __forceinline__ Place place_of(const ScaledAttnArgs& a, const int32_t* bt, int ws) {
-  const int i = block_of(a, ws);
-  Place p;
-  p.ok = i < a.bt_width;
-  p.blk = p.ok ? bt[i] : 0;
-  if (p.blk < 0 || p.blk >= a.num_blocks) p.ok = false, p.blk = 0;
-  return p;
-}
 
-// Loads the window at key ws; keys at and past `hi` re-read the last one below it.
-__device__ __forceinline__ void load_win(const ScaledAttnArgs& a, int head, int lane, int ws,
-                                         int hi, Place p, Win& w) {
-  const int off = ws - block_of(a, ws) * a.block_size;
-  const int64_t base = (int64_t)p.blk * a.c_sb + (int64_t)off * a.c_st + (int64_t)head * a.c_sh;
-  const int64_t sbase =
-      (int64_t)p.blk * a.s_sb + (int64_t)(off >> a.g_shift) * a.s_sg + (int64_t)head * a.s_sh;
-  w.ks = a.ks[sbase];
-  w.vs = a.vs[sbase];
-  const int last = hi - ws - 1;  // >= 0
-  const int c = lane & 15, g = lane >> 4;
-  const int st = (int)a.c_st;  // the host keeps 32 rows within 2 GiB
+// The K or V rows of a window: `rows` rows from row `off` of block `blk`. The buffer ends
+// behind its last row, so further ones read as zeros and, with none, the loads touch no
+// memory: every window's loads are issued alike, whatever is left.
+struct Source {
+  int64_t base;
+  int bytes;
+};
+__device__ __forceinline__ Source source_of(const ScaledAttnArgs& a, int head, int blk, int off,
+                                            int rows) {
+  Source s;
+  s.base = (int64_t)blk * a.c_sb + (int64_t)off * a.c_st + (int64_t)head * a.c_sh;
+  s.bytes = rows > 0 ? (min(rows, kWin) - 1) * (int)a.c_st + kD : 0;
+  return s;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t* cache, const Source& s) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(cache + s.base), 0, s.bytes,
+                                           0x00027000);
+}
+// `at`: the lane's first offset, c * stride + 32 g for K and 4 g * stride + 8 c for V
+// (c = l % 16). The others are sums that are cheaper than the registers to keep them in,
+// so the compiler may not take them out of the loop.
+__device__ __forceinline__ void load_k(const ScaledAttnArgs& a, const Source& s, int at, Win& w) {
+  const auto r = buffer_of(a.kc, s);
+  const int st = (int)a.c_st;
+  asm volatile("" : "+v"(at));
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int key = min(16 * t + c, last);
-    const uint8_t* p = a.kc + base + (uint32_t)(key * st + 32 * g);
-    w.k[2 * t] = *reinterpret_cast<const uint4*>(p);
-    w.k[2 * t + 1] = *reinterpret_cast<const uint4*>(p + 16);
+    w.k[2 * t] = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * t * st, 0, 0);
+    w.k[2 * t + 1] = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * t * st + 16, 0, 0);
   }
+}
+__device__ __forceinline__ void load_v(const ScaledAttnArgs& a, const Source& s, int at, Win& w) {
+  const auto r = buffer_of(a.vc, s);
+  const int st = (int)a.c_st;
+  asm volatile("" : "+v"(at));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int key = min((e & 4) * 4 + 4 * g + (e & 3), last);
-    w.v[e] = *reinterpret_cast<const uint2*>(a.vc + base + (uint32_t)(key * st + 8 * c));
-  }
+  for (int e = 0; e < 8; ++e)
+    w.v[e] = __builtin_amdgcn_raw_buffer_load_b64(r, at + ((e & 4) * 4 + (e & 3)) * st, 0, 0);
 }
 
 // The V^T operand of dims 8 i + db (i = l % 16), db = 0 .. 7, from the lane's 8 x 8
-// codes; emit(db, operand).
+// codes times the power of two in `scale`; emit(db, operand).
 template <typename F>
-__device__ __forceinline__ void transposed(const uint2 (&v)[8], F emit) {
+__device__ __forceinline__ void transposed(const u32x2_t (&v)[8], float scale, F emit) {
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
 #pragma unroll
@@ -189,10 +191,10 @@ __device__ __forceinline__ void transposed(const uint2 (&v)[8], F emit) {
       }
       Frag f;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) f.u[p] = bf16_pair(m[p], false);
+      for (int p = 0; p < 4; ++p) f.u[p] = bf16_pair(m[p], false, scale);
       emit(4 * w + 2 * h, f.v);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) f.u[p] = bf16_pair(m[p], true);
+      for (int p = 0; p < 4; ++p) f.u[p] = bf16_pair(m[p], true, scale);
       emit(4 * w + 2 * h + 1, f.v);
     }
   }
@@ -205,14 +207,14 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
 }
 
 // The state of 16 QT query rows: per tile the lane's row (l % 16) has its maximum
-// (log2 domain), the lane's part of its sum and O[d = 32 (l / 16) + 8 j + db] in
+// (log2 domain), its sum (in every element of l) and O[d = 32 (l / 16) + 8 j + db] in
 // o[db][j].
 template <int QT>
 struct Rows {
   bf16x8_t q[QT][4];
   int lim[QT];  // keys that the row sees
-  float m[QT], l[QT];
-  f32x4_t o[QT][8];
+  float m[QT];
+  f32x4_t l[QT], o[QT][8];
 };
 
 template <int QT>
@@ -225,7 +227,7 @@ __device__ __forceinline__ void load_rows(const ScaledAttnArgs& a, const Seq& s,
     const bool live = r < s.Lq * a.G;
     R.lim[t] = live ? row_keys(s, a.G, r) : 0;
     R.m[t] = -INFINITY;
-    R.l[t] = 0.0f;
+    R.l[t] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
     for (int db = 0; db < 8; ++db) R.o[t][db] = f32x4_t{0, 0, 0, 0};
     const uint16_t* p = a.q;
@@ -240,21 +242,14 @@ __device__ __forceinline__ void load_rows(const ScaledAttnArgs& a, const Seq& s,
   }
 }
 
-// One window. kMask: some row may not see some key. A key that a row does not see
-// takes no part in that row, whatever its codes and scales are: its probability is
-// 0, and NaN codes of V, which a zero does not cancel, are taken out of the product
-// and given to the rows that see them by a product of their own.
-template <int QT, bool kMask>
-__device__ __forceinline__ void step(const ScaledAttnArgs& a, const Win& w, int ws, int lane,
-                                     Rows<QT>& R) {
-  const int g = lane >> 4;
-  const float c = a.scale_log2 * w.ks;
-  f32x4_t s[QT][2];
+// S^T of a window: scores of keys 16 t + 4 g + j in s[u][t][j].
+template <int QT>
+__device__ __forceinline__ void scores(const Win& w, const Rows<QT>& R, f32x4_t (&s)[QT][2]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 k = w.k[2 * t + (i >> 1)];
+      const u32x4_t k = w.k[2 * t + (i >> 1)];
       const bf16x8_t ka = (i & 1) ? decode8(k.z, k.w) : decode8(k.x, k.y);
 #pragma unroll
       for (int u = 0; u < QT; ++u) {
@@ -263,24 +258,39 @@ __device__ __forceinline__ void step(const ScaledAttnArgs& a, const Win& w, int 
       }
     }
   }
-  bf16x8_t p[QT];
-  [[maybe_unused]] uint32_t seen[QT];
+}
+
+// The softmax step of the scores (times c), and the probabilities times `rest` as P^T.
+// kMask: some row may not see some key. A key that a row does not see takes no part in
+// that row, whatever its codes and scales are: its probability is 0. Bit e of seen[u]:
+// the row sees the lane's e-th key. The sum adds the probabilities as they are
+// multiplied, rounded to bf16, on the matrix cores (a row of ones), so that the weights
+// of an output add up to one.
+template <int QT, bool kMask>
+__device__ __forceinline__ void weigh(const f32x4_t (&s)[QT][2], float c, float rest, int ws,
+                                      int rows, int g, Rows<QT>& R, bf16x8_t (&p)[QT],
+                                      uint32_t (&seen)[QT]) {
+  Frag ones;
+  ones.u[0] = ones.u[1] = ones.u[2] = ones.u[3] = 0x3f803f80u;
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
-    float x[8];
-    if constexpr (kMask) seen[u] = 0;
+    seen[u] = 0xff;
+    if constexpr (kMask) {
+      // keys 4 g + j and 16 + 4 g + j of the window's first `rows`, below the row's limit
+      const int left = min(R.lim[u] - ws, rows) - 4 * g;
+      const uint32_t lo = left >= 4 ? 15u : (left <= 0 ? 0u : (1u << left) - 1);
+      const uint32_t hi = left >= 20 ? 15u : (left <= 16 ? 0u : (1u << (left - 16)) - 1);
+      seen[u] = lo | (hi << 4);
+    }
+    float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[e] = s[u][e >> 2][e & 3] * c;
-      if constexpr (kMask) {
-        const bool in = ws + (e & 4) * 4 + 4 * g + (e & 3) < R.lim[u];
-        seen[u] |= in ? 1u << e : 0u;
-        x[e] = in ? x[e] : -INFINITY;
-      }
+      y[e] = s[u][e >> 2][e & 3] * c;
+      if constexpr (kMask) y[e] = (seen[u] >> e) & 1u ? y[e] : -INFINITY;
     }
-    float m = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                    fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    m = fmaxf(R.m[u], quad_max(m));
+    const float most = quad_max(fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                                      fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))));
+    const float m = fmaxf(R.m[u], most);
     const float ref = m == -INFINITY ? 0.0f : m;
     if (__any(m > R.m[u])) {
       const float f = __builtin_amdgcn_exp2f(R.m[u] - ref);
@@ -289,94 +299,164 @@ __device__ __forceinline__ void step(const ScaledAttnArgs& a, const Win& w, int 
       for (int db = 0; db < 8; ++db) R.o[u][db] *= f;
       R.m[u] = m;
     }
-    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(y[e] - ref);
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      float y[2];
+    for (int e = 0; e < 8; e += 2) f.u[e >> 1] = pk_bf16(y[e], y[e + 1]);
+    R.l[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, f.v, R.l[u], 0, 0, 0);
+    if (rest != 1.0f) {  // scales of another producer that are no powers of two
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        const float v = __builtin_amdgcn_exp2f(x[e + d] - ref);
-        sum += v;
-        y[d] = v * w.vs;
-        if constexpr (kMask) y[d] = (seen[u] >> (e + d)) & 1u ? y[d] : 0.0f;
+      for (int e = 0; e < 8; e += 2) {
+        float z[2] = {y[e] * rest, y[e + 1] * rest};
+        if constexpr (kMask) {
+          if (!((seen[u] >> e) & 1u)) z[0] = 0.0f;
+          if (!((seen[u] >> (e + 1)) & 1u)) z[1] = 0.0f;
+        }
+        f.u[e >> 1] = pk_bf16(z[0], z[1]);
       }
-      f.u[e >> 1] = (uint32_t)to_bf(y[0]) | ((uint32_t)to_bf(y[1]) << 16);
     }
-    R.l[u] += sum;
     p[u] = f.v;
-  }
-  if constexpr (!kMask) {
-    transposed(w.v, [&](int db, bf16x8_t va) {
-#pragma unroll
-      for (int u = 0; u < QT; ++u)
-        R.o[u][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[u], R.o[u][db], 0, 0, 0);
-    });
-  } else {
-    uint2 v[8], bad[8];
-    uint32_t any = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bad[e] = make_uint2(nan_bytes(w.v[e].x), nan_bytes(w.v[e].y));
-      v[e] = make_uint2(w.v[e].x & ~bad[e].x, w.v[e].y & ~bad[e].y);
-      bad[e].x &= 0x38383838u;  // 1.0
-      bad[e].y &= 0x38383838u;
-      any |= bad[e].x | bad[e].y;
-    }
-    transposed(v, [&](int db, bf16x8_t va) {
-#pragma unroll
-      for (int u = 0; u < QT; ++u)
-        R.o[u][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[u], R.o[u][db], 0, 0, 0);
-    });
-    if (__any(any != 0)) {
-#pragma unroll
-      for (int u = 0; u < QT; ++u) {
-        Frag f;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2)
-          f.u[e >> 1] = ((seen[u] >> e) & 1u ? 0x3f80u : 0u) |
-                        ((seen[u] >> (e + 1)) & 1u ? 0x3f800000u : 0u);
-        transposed(bad, [&](int db, bf16x8_t va) {
-          const f32x4_t n =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, f.v, f32x4_t{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n[j] > 0.0f) R.o[u][db][j] = NAN;
-        });
-      }
-    }
   }
 }
 
-// Windows first, first + stride, ... of keys [lo, hi): `full` is the number of keys
-// that every row sees.
+// O^T += V^T P^T
+template <int QT>
+__device__ __forceinline__ void gather(const Win& w, float scale, const bf16x8_t (&p)[QT],
+                                       Rows<QT>& R) {
+  transposed(w.v, scale, [&](int db, bf16x8_t va) {
+#pragma unroll
+    for (int u = 0; u < QT; ++u)
+      R.o[u][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[u], R.o[u][db], 0, 0, 0);
+  });
+}
+
+// Takes the NaN codes, which a probability of zero does not cancel, out of V; true where
+// there is one.
+__device__ __forceinline__ bool drop_nan(Win& w) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const u32x2_t bad = {nan_bytes(w.v[e].x), nan_bytes(w.v[e].y)};
+    w.v[e] &= ~bad;
+    any |= bad.x | bad.y;
+  }
+  return __any(any != 0);
+}
+
+// Gives the NaN codes of V (as loaded) to the rows that see them, by a product of their
+// own: 1 for a NaN code by 1 for a key that is seen.
+template <int QT>
+__device__ __forceinline__ void spread_nan(Win& w, const uint32_t (&seen)[QT], Rows<QT>& R) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    w.v[e] = u32x2_t{nan_bytes(w.v[e].x) & 0x38383838u, nan_bytes(w.v[e].y) & 0x38383838u};
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      f.u[e >> 1] = ((seen[u] >> e) & 1u ? 0x3f80u : 0u) |
+                    ((seen[u] >> (e + 1)) & 1u ? 0x3f800000u : 0u);
+    transposed(w.v, 1.0f, [&](int db, bf16x8_t va) {
+      const f32x4_t n =
+          __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, f.v, f32x4_t{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n[j] > 0.0f) R.o[u][db][j] = NAN;
+    });
+  }
+}
+
+// The windows of a walk, 64 at a time: lane i has looked up the i-th one's block (-1: the
+// table has none there) and scales, so that no window waits for its own.
+struct Batch {
+  int n, ws0, stride, hi;
+  int blk, off;
+  float ks, vs;
+};
+__device__ __forceinline__ Batch look_up(const ScaledAttnArgs& a, const int32_t* bt, int head,
+                                         int lane, int ws0, int stride, int hi) {
+  Batch t;
+  t.n = min(64, (hi - ws0 + stride - 1) / stride);
+  t.ws0 = ws0;
+  t.stride = stride;
+  t.hi = hi;
+  const int ws = ws0 + min(lane, t.n - 1) * stride, col = block_of(a, ws);
+  t.off = ws - col * a.block_size;
+  t.blk = col < a.bt_width ? bt[col] : -1;
+  if (t.blk >= a.num_blocks || t.blk < 0) t.blk = -1;
+  const int64_t at = (int64_t)max(t.blk, 0) * a.s_sb + (int64_t)(t.off >> a.g_shift) * a.s_sg +
+                     (int64_t)head * a.s_sh;
+  t.ks = a.ks[at];
+  t.vs = a.vs[at];
+  return t;
+}
+// rows of window i: none past the last window, and of a window without a block
+__device__ __forceinline__ Source source(const ScaledAttnArgs& a, const Batch& t, int head, int i) {
+  const int j = min(i, 63), blk = __builtin_amdgcn_readlane(t.blk, j);
+  return source_of(a, head, max(blk, 0), __builtin_amdgcn_readlane(t.off, j),
+                   i < t.n && blk >= 0 ? t.hi - (t.ws0 + i * t.stride) : 0);
+}
+
+// Window i, in registers, and the loads of the next one.
+template <int QT, bool kMask>
+__device__ __forceinline__ void window(const ScaledAttnArgs& a, const Batch& t, int head, int i,
+                                       int at_k, int at_v, int lane, Win& w, Rows<QT>& R) {
+  const int ws = t.ws0 + i * t.stride;
+  const Source next = source(a, t, head, i + 1);
+  const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.ks), i));
+  const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.vs), i));
+  // vs as a power of two, which V's decoding takes for nothing, and what is left of it
+  // (all of it where it is zero, negative, subnormal or not finite)
+  const uint32_t bits = __float_as_uint(vs);
+  const bool plain = bits >= 0x00800000u && bits < 0x7f800000u;
+  const float scale = plain ? vs : 1.0f;
+  const float rest = plain ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : vs;
+  f32x4_t s[QT][2];
+  scores<QT>(w, R, s);
+  load_k(a, next, at_k, w);  // in flight during the rest of this window
+  bf16x8_t p[QT];
+  uint32_t seen[QT];
+  const int rows = __builtin_amdgcn_readlane(t.blk, i) < 0 ? 0 : kWin;
+  weigh<QT, kMask>(s, a.scale_log2 * ks, rest, ws, rows, lane >> 4, R, p, seen);
+  if constexpr (!kMask) {
+    gather<QT>(w, scale, p, R);
+  } else {
+    const bool bad = drop_nan(w);
+    gather<QT>(w, scale, p, R);
+    if (bad) {
+      load_v(a, source(a, t, head, i), at_v, w);
+      spread_nan<QT>(w, seen, R);
+    }
+  }
+  load_v(a, next, at_v, w);  // in flight during the next window's scores
+}
+
+// windows of a batch before the first one that some row does not see all of
+__device__ __forceinline__ int free_windows(const Batch& t, int full) {
+  if (full - t.ws0 < kWin || __any(t.blk < 0)) return 0;
+  return min(t.n, (full - t.ws0 - kWin) / t.stride + 1);
+}
+
+// Windows at keys ws0, ws0 + stride, ... below hi; `full` is the number of keys that
+// every row sees. Windows whose table entry is no block of the cache, or lies past the
+// table, are left out.
 template <int QT>
 __device__ __forceinline__ void walk(const ScaledAttnArgs& a, const int32_t* bt, int head, int lane,
-                                     int ws, int stride, int hi, int full, Rows<QT>& R) {
-  if (ws >= hi) return;
-  Place p = place_of(a, bt, ws);
-  Win w;
-  load_win(a, head, lane, ws, hi, p, w);
-  Place pn = ws + stride < hi ? place_of(a, bt, ws + stride) : Place{0, false};
-  for (;;) {
-    const int next = ws + stride;
-    Win wn;
-    Place pf{0, false};
-    if (next < hi) {
-      load_win(a, head, lane, next, hi, pn, wn);
-      if (next + stride < hi) pf = place_of(a, bt, next + stride);
-    }
-    if (p.ok) {
-      if (ws + kWin <= full)
-        step<QT, false>(a, w, ws, lane, R);
-      else
-        step<QT, true>(a, w, ws, lane, R);
-    }
-    if (next >= hi) break;
-    ws = next;
-    w = wn;
-    p = pn;
-    pn = pf;
+                                     int ws0, int stride, int hi, int full, Rows<QT>& R) {
+  const int c = lane & 15, g = lane >> 4, st = (int)a.c_st;
+  const int at_k = c * st + 32 * g, at_v = 4 * g * st + 8 * c;
+  for (; ws0 < hi; ws0 += 64 * stride) {
+    const Batch t = look_up(a, bt, head, lane, ws0, stride, hi);
+    const int free = free_windows(t, full);
+    Win w;
+    const Source first = source(a, t, head, 0);
+    load_k(a, first, at_k, w);
+    load_v(a, first, at_v, w);
+    int i = 0;
+    for (; i < free; ++i) window<QT, false>(a, t, head, i, at_k, at_v, lane, w, R);
+    for (; i < t.n; ++i) window<QT, true>(a, t, head, i, at_k, at_v, lane, w, R);
   }
 }
 
@@ -385,13 +465,20 @@ __device__ __forceinline__ uint16_t* out_row(const ScaledAttnArgs& a, const Seq&
   return a.out + (int64_t)(s.qs + r / a.G) * a.o_st + (int64_t)(head * a.G + r % a.G) * a.o_sh;
 }
 
-__global__ __launch_bounds__(64 * kSplitWaves) void k_scaled_split(ScaledAttnArgs a) {
+__global__ __launch_bounds__(64 * kSplitWaves, 3) void k_scaled_split(ScaledAttnArgs a) {
   __shared__ float s_o[kSplitWaves][kRows][kD];
   __shared__ float s_ml[kSplitWaves][kRows][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.x, head = blockIdx.y % a.Hkv, tile = blockIdx.y / a.Hkv;
-  const int b = blockIdx.z;
+  // Workgroups go round the 8 XCDs in order. The heads of a (sequence, split) go to one of
+  // them: side by side in memory, they take all of its L2 channels together. The splits
+  // that every sequence has come first, in turn over the XCDs.
+  const int tiles = a.Hkv * a.qtiles;
+  const int pair = (int)(blockIdx.x >> 3) / tiles * 8 + (blockIdx.x & 7);
+  const int at = (int)(blockIdx.x >> 3) % tiles;
+  const int head = at % a.Hkv, tile = at / a.Hkv;
+  const int split = pair / a.num_seqs, b = pair % a.num_seqs;
+  if (split >= a.nsplit) return;
   const Seq s = seq_of(a, b);
   const int r0 = tile * kRows, rows = s.Lq * a.G - r0;  // rows of this tile, and behind it
   if (rows <= 0) return;
@@ -405,11 +492,10 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_scaled_split(ScaledAttnArg
   load_rows<1>(a, s, head, r0, lane, R);
   walk<1>(a, a.bt + (int64_t)b * a.bt_stride, head, lane, lo + wave * kWin, kSplitWaves * kWin, hi,
           full, R);
-  const float l = quad_sum(R.l[0]);
   const int n = lane & 15, g = lane >> 4;
   if (g == 0) {
     s_ml[wave][n][0] = R.m[0];
-    s_ml[wave][n][1] = l;
+    s_ml[wave][n][1] = R.l[0][0];
   }
   if (n < live) {
 #pragma unroll
@@ -423,46 +509,49 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_scaled_split(ScaledAttnArg
   }
   __syncthreads();
   // 32 threads a row, 4 dims each
-  const int row = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
-  if (row >= live) return;
-  float m = -INFINITY;
+  const int d = 4 * (threadIdx.x & 31);
+  for (int row = threadIdx.x >> 5; row < live; row += 2 * kSplitWaves) {
+    float m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kSplitWaves; ++w) m = fmaxf(m, s_ml[w][row][0]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f, o[4] = {0, 0, 0, 0};
+    for (int w = 0; w < kSplitWaves; ++w) m = fmaxf(m, s_ml[w][row][0]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, o[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < kSplitWaves; ++w) {
-    const float f = __builtin_amdgcn_exp2f(s_ml[w][row][0] - ref);
-    const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
-    sum += f * s_ml[w][row][1];
-    o[0] += f * x.x;
-    o[1] += f * x.y;
-    o[2] += f * x.z;
-    o[3] += f * x.w;
-  }
-  if (a.nsplit == 1 || keys <= a.split_len) {  // the tile's only split
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint2 y;
-    y.x = (uint32_t)to_bf(o[0] * inv) | ((uint32_t)to_bf(o[1] * inv) << 16);
-    y.y = (uint32_t)to_bf(o[2] * inv) | ((uint32_t)to_bf(o[3] * inv) << 16);
-    *reinterpret_cast<uint2*>(out_row(a, s, head, r0 + row) + d) = y;
-  } else {
-    const int64_t slot = (((int64_t)b * a.Hkv + head) * a.qtiles + tile) * a.nsplit + split;
-    *reinterpret_cast<float4*>(a.part_o + (slot * kRows + row) * kD + d) =
-        make_float4(o[0], o[1], o[2], o[3]);
-    if (d == 0) {
-      a.part_ml[(slot * kRows + row) * 2] = m;
-      a.part_ml[(slot * kRows + row) * 2 + 1] = sum;
+    for (int w = 0; w < kSplitWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[w][row][0] - ref);
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][d]);
+      sum += f * s_ml[w][row][1];
+      o[0] += f * x.x;
+      o[1] += f * x.y;
+      o[2] += f * x.z;
+      o[3] += f * x.w;
+    }
+    if (a.nsplit == 1 || keys <= a.split_len) {  // the tile's only split
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint2 y;
+      y.x = (uint32_t)to_bf(o[0] * inv) | ((uint32_t)to_bf(o[1] * inv) << 16);
+      y.y = (uint32_t)to_bf(o[2] * inv) | ((uint32_t)to_bf(o[3] * inv) << 16);
+      *reinterpret_cast<uint2*>(out_row(a, s, head, r0 + row) + d) = y;
+    } else {
+      const int64_t slot = (((int64_t)b * a.Hkv + head) * a.qtiles + tile) * a.nsplit + split;
+      *reinterpret_cast<float4*>(a.part_o + (slot * kRows + row) * kD + d) =
+          make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) {
+        a.part_ml[(slot * kRows + row) * 2] = m;
+        a.part_ml[(slot * kRows + row) * 2 + 1] = sum;
+      }
     }
   }
 }
 
-// Joins the splits of one query row: 8 x 32 threads, the first index over the splits.
+// Joins the splits of 8 / P query rows: 32 threads a row and part of the splits (P: parts).
+template <int P>
 __global__ __launch_bounds__(256) void k_scaled_combine(ScaledAttnArgs a) {
   __shared__ float s_o[8][kD];
   __shared__ float s_ml[8][2];
-  const int row = blockIdx.x, head = blockIdx.y % a.Hkv, tile = blockIdx.y / a.Hkv;
-  const int b = blockIdx.z;
+  const int head = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv, b = blockIdx.y;
+  const int part = (threadIdx.x >> 5) % P, d = 4 * (threadIdx.x & 31);
+  const int row = blockIdx.z * (8 / P) + (threadIdx.x >> 5) / P;
   const Seq s = seq_of(a, b);
   const int r0 = tile * kRows, rows = s.Lq * a.G - r0;
   if (row >= rows) return;
@@ -470,9 +559,9 @@ __global__ __launch_bounds__(256) void k_scaled_combine(ScaledAttnArgs a) {
   if (keys <= a.split_len) return;  // written by its only split
   const int n = min(a.nsplit, (keys + a.split_len - 1) / a.split_len);
   const int64_t slot0 = (((int64_t)b * a.Hkv + head) * a.qtiles + tile) * a.nsplit;
-  const int part = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
   float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
-  for (int i = part; i < n; i += 8) {
+#pragma unroll 4
+  for (int i = part; i < n; i += P) {
     const int64_t at = (slot0 + i) * kRows + row;
     const float mi = a.part_ml[2 * at], li = a.part_ml[2 * at + 1];
     const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * kD + d);
@@ -485,25 +574,27 @@ __global__ __launch_bounds__(256) void k_scaled_combine(ScaledAttnArgs a) {
     o[2] = o[2] * f + x.z * fi;
     o[3] = o[3] * f + x.w * fi;
   }
-  *reinterpret_cast<float4*>(&s_o[part][d]) = make_float4(o[0], o[1], o[2], o[3]);
-  if (d == 0) s_ml[part][0] = m, s_ml[part][1] = l;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  m = -INFINITY;
+  if constexpr (P > 1) {
+    *reinterpret_cast<float4*>(&s_o[part][d]) = make_float4(o[0], o[1], o[2], o[3]);
+    if (d == 0) s_ml[part][0] = m, s_ml[part][1] = l;
+    __syncthreads();
+    if (part) return;
+    m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, s_ml[i][0]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  l = 0.0f;
-  o[0] = o[1] = o[2] = o[3] = 0.0f;
+    for (int i = 0; i < P; ++i) m = fmaxf(m, s_ml[i][0]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+    o[0] = o[1] = o[2] = o[3] = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = __builtin_amdgcn_exp2f(s_ml[i][0] - ref);
-    const float4 x = *reinterpret_cast<const float4*>(&s_o[i][d]);
-    l += f * s_ml[i][1];
-    o[0] += f * x.x;
-    o[1] += f * x.y;
-    o[2] += f * x.z;
-    o[3] += f * x.w;
+    for (int i = 0; i < P; ++i) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[i][0] - ref);
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[i][d]);
+      l += f * s_ml[i][1];
+      o[0] += f * x.x;
+      o[1] += f * x.y;
+      o[2] += f * x.z;
+      o[3] += f * x.w;
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint2 y;
@@ -513,23 +604,26 @@ __global__ __launch_bounds__(256) void k_scaled_combine(ScaledAttnArgs a) {
 }
 
 template <int QT>
-__global__ __launch_bounds__(64 * kRowWaves) void k_scaled_rows(ScaledAttnArgs a) {
+__global__ __launch_bounds__(64 * kRowWaves, QT == 1 ? 3 : 2) void k_scaled_rows(ScaledAttnArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.y, b = blockIdx.z;
+  // as k_scaled_split's workgroups, with the rows that see most keys first
+  const int pair = (int)(blockIdx.x >> 3) / a.Hkv * 8 + (blockIdx.x & 7);
+  const int head = (int)(blockIdx.x >> 3) % a.Hkv;
+  const int tile = a.qtiles - 1 - pair / a.num_seqs, b = pair % a.num_seqs;
+  if (tile < 0) return;
   const Seq s = seq_of(a, b);
   const int total = s.Lq * a.G;
-  const int r0 = (blockIdx.x * kRowWaves + wave) * kRows * QT;
+  const int r0 = (tile * kRowWaves + wave) * kRows * QT;
   if (r0 >= total) return;
-  const int last = min(total, r0 + kRows * QT) - 1;
   Rows<QT> R;
   load_rows<QT>(a, s, head, r0, lane, R);
-  walk<QT>(a, a.bt + (int64_t)b * a.bt_stride, head, lane, 0, kWin, row_keys(s, a.G, last),
-           row_keys(s, a.G, r0), R);
+  walk<QT>(a, a.bt + (int64_t)b * a.bt_stride, head, lane, 0, kWin,
+           row_keys(s, a.G, min(total, r0 + kRows * QT) - 1), row_keys(s, a.G, r0), R);
   const int n = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const float l = quad_sum(R.l[t]);
+    const float l = R.l[t][0];
     const int r = r0 + 16 * t + n;
     if (r >= total) continue;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -544,10 +638,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_scaled_rows(ScaledAttnArgs a
   }
 }
 
-constexpr int kRowsQT = 2;  // tiles of a wave in k_scaled_rows
-
 struct ScaledPlan {
-  bool rows;  // k_scaled_rows
+  int qt;  // tiles of a wave of k_scaled_rows, 0: k_scaled_split
   int qtiles, nsplit, split_len;
   size_t bytes;
 };
@@ -557,12 +649,18 @@ ScaledPlan plan_of(int num_seqs, int Hkv, int G, int max_q, int max_k) {
   const int64_t rows = (int64_t)max_q * G;
   const int64_t q = (rows + kRows - 1) / kRows;
   p.qtiles = (int)q;
-  p.rows = rows > 64;
   p.nsplit = 1;
   p.split_len = INT32_MAX;
   p.bytes = 0;
-  if (p.rows) return p;
   const int64_t tiles = (int64_t)num_seqs * Hkv * q;
+  // Prompts take k_scaled_rows once their tiles fill half the chip's SIMDs without
+  // splitting keys (one prompt of 33 tokens, 72 tiles, behind 967 keys: 12.0 us split,
+  // 26 us not). More tiles to a wave share a window's loads and decoding as long as the
+  // waves still fill the chip: 509 tokens, 1024 tiles, take 17.4 / 20.9 / 25.4 us with 1 /
+  // 2 / 3, 2000 tokens of 16 heads, 2000 tiles, 124 / 82 / 103 us, and 3500 of 32 heads,
+  // 7100 tiles, 353 / 198 / 173 us.
+  p.qt = tiles < 512 || rows <= 64 ? 0 : (tiles >= 6144 ? 3 : (tiles >= 1536 ? 2 : 1));
+  if (p.qt) return p;
   // about 1024 workgroups if every sequence is as long as declared, of at least one
   // window a wave and at most 1024 keys unless that makes more than 8192 of them
   int64_t len = (max_k * tiles + 1023) / 1024;
@@ -623,7 +721,7 @@ int hs_verify_attention_scaled(
     return HS_ERR_UNSUPPORTED;
   if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3) return HS_ERR_UNSUPPORTED;
   // a window's rows lie within 2 GiB of its first (32-bit offsets of the lanes)
-  if (cache_stride_tok < 0 || cache_stride_tok > INT32_MAX / (2 * kWin)) return HS_ERR_UNSUPPORTED;
+  if (cache_stride_tok < kD || cache_stride_tok > INT32_MAX / (2 * kWin)) return HS_ERR_UNSUPPORTED;
   const ScaledPlan p = plan_of(num_seqs, num_kv_heads, G, max_seqlen_q, max_seqlen_k);
   const int64_t tiles = (int64_t)num_kv_heads * p.qtiles;
   if (num_seqs > 65535 || (int64_t)max_seqlen_q * G > INT32_MAX / 2 || num_kv_heads > 65535)
@@ -650,6 +748,7 @@ int hs_verify_attention_scaled(
   a.num_blocks = num_blocks;
   a.cu_q = cu_seqlens_q;
   a.cu_k = cu_seqlens_k;
+  a.num_seqs = num_seqs;
   a.Hkv = num_kv_heads;
   a.G = G;
   a.block_size = block_size;
@@ -665,21 +764,29 @@ int hs_verify_attention_scaled(
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + (size_t)num_seqs * tiles * p.nsplit * kRows * kD;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (p.rows) {
-    const int64_t per = (int64_t)kRows * kRowsQT * kRowWaves;
-    const dim3 grid((unsigned)(((int64_t)max_seqlen_q * G + per - 1) / per),
-                    (unsigned)num_kv_heads, (unsigned)num_seqs);
-    hipLaunchKernelGGL(k_scaled_rows<kRowsQT>, grid, dim3(64 * kRowWaves), 0, st, a);
+  if (p.qt) {
+    const int64_t per = (int64_t)kRows * p.qt * kRowWaves;
+    a.qtiles = (int)(((int64_t)max_seqlen_q * G + per - 1) / per);
+    const int64_t groups = ((int64_t)num_seqs * a.qtiles + 7) / 8 * 8 * num_kv_heads;
+    if (groups > INT32_MAX) return HS_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)groups), block(64 * kRowWaves);
+    if (p.qt == 3) hipLaunchKernelGGL(k_scaled_rows<3>, grid, block, 0, st, a);
+    else if (p.qt == 2) hipLaunchKernelGGL(k_scaled_rows<2>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(k_scaled_rows<1>, grid, block, 0, st, a);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
   }
-  if (tiles > 65535) return HS_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(k_scaled_split, dim3((unsigned)p.nsplit, (unsigned)tiles, (unsigned)num_seqs),
-                     dim3(64 * kSplitWaves), 0, st, a);
+  const int64_t groups = ((int64_t)num_seqs * p.nsplit + 7) / 8 * 8 * tiles;
+  if (groups > INT32_MAX) return HS_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(k_scaled_split, dim3((unsigned)groups), dim3(64 * kSplitWaves), 0, st, a);
   if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   if (p.nsplit > 1) {
-    hipLaunchKernelGGL(k_scaled_combine,
-                       dim3((unsigned)kRows, (unsigned)tiles, (unsigned)num_seqs), dim3(256), 0,
-                       st, a);
+    // a workgroup for 8 rows, or for each where there are many splits to share out
+    if (p.nsplit <= 8)
+      hipLaunchKernelGGL(k_scaled_combine<1>, dim3((unsigned)tiles, (unsigned)num_seqs, kRows / 8),
+                         dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL(k_scaled_combine<8>, dim3((unsigned)tiles, (unsigned)num_seqs, kRows),
+                         dim3(256), 0, st, a);
     if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   }
   return HS_OK;

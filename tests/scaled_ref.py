@@ -72,25 +72,33 @@ def attention(q, k, v, Lq, Lk, scale):
     Hq, Hkv = q.shape[1], k.shape[1]
     out, most = np.zeros(q.shape), np.zeros(q.shape)
     size = np.zeros(q.shape[:2])
-    for i in range(Lq):
-        n = min(Lk, Lk - Lq + i + 1)
-        if n <= 0:
-            continue
-        for h in range(Hq):
-            kk, vv = k[:n, h // (Hq // Hkv)], v[:n, h // (Hq // Hkv)]
-            s = kk @ q[i, h] * scale
-            p = np.exp(s - (s.max() if not np.isnan(s).any() else 0.0))
-            out[i, h] = (p[:, None] * vv).sum(0) / p.sum()
-            most[i, h] = (p[:, None] * np.abs(vv)).sum(0) / p.sum()
-            size[i, h] = (np.abs(kk) @ np.abs(q[i, h])).max() * abs(scale)
+    if Lk == 0 or Lq == 0:
+        return out, most, size
+    seen = np.arange(Lk)[None] <= Lk - Lq + np.arange(Lq)[:, None]
+    any_seen = seen.any(1)
+    for h in range(Hq):
+        kk, vv = k[:, h // (Hq // Hkv)], v[:, h // (Hq // Hkv)]
+        s = np.where(seen, q[:, h] @ kk.T * scale, -np.inf)
+        top = np.where(any_seen, s.max(1), 0.0)
+        p = np.where(seen, np.exp(s - np.where(np.isnan(top), 0.0, top)[:, None]), 0.0)
+        p /= np.where(any_seen, p.sum(1), 1.0)[:, None]
+        clean = np.where(np.isnan(vv), 0.0, vv)
+        out[:, h] = p @ clean
+        hit = seen.astype(float) @ np.isnan(vv).astype(float) > 0
+        out[:, h][hit] = np.nan
+        most[:, h] = p @ np.abs(clean)
+        size[:, h] = np.where(seen, np.abs(q[:, h]) @ np.abs(kk).T, 0.0).max(1) * abs(scale)
     return out, most, size
 
 
 def tolerance(out, most, size):
-    """Elementwise: each probability rounds to bf16 once (2^-8 relative, of terms p |v|) and
-    the output once more; scores are sums of 128 exact products in 32 bits, so off by at most
+    """Elementwise: each probability rounds to bf16 once, p_j (1 + d_j) with |d_j| <= 2^-8, in
+    the sum above and in the sum below, which makes sum p v / sum p at most
+    2^-8 (sum p |v| / sum p + |out|) / (1 - 2^-8) off (both sums move, by sum d p v and sum d p);
+    a scale that is no power of two rounds the product's weights once more, and the output
+    rounds once. Scores are sums of 128 exact products in 32 bits, so off by at most
     128 * 2^-24 of sum |q k|, which moves a probability (and the sum under it) by that
     share, with as much again for the products by the scale and the exponential; sums and
     rescalings in 32 bits: 2^-16."""
     return (2.0 ** -8 + 4 * 128 * 2.0 ** -24 * size[..., None] + 2.0 ** -16) * most * 1.01 \
-        + 2.0 ** -8 * np.abs(out) + 1e-30
+        + 2 * 2.0 ** -8 * 1.01 * np.abs(out) + 1e-30

@@ -133,6 +133,11 @@ _ATTEND = [
     ("two-tiles", 32, 8, 256, 256, [9, 16], [300, 16], 512),
     ("prompts", 32, 8, 256, 32, [61, 130, 1], [61, 333, 500], 512),
     ("prompt-group-1", 4, 4, 256, 128, [300, 77], [300, 400], 512),
+    # one, two and three tiles to a wave, and keys past the first 64 windows
+    ("prompts-1", 32, 8, 256, 32, [130, 61], [333, 61], 512),
+    ("prompts-2", 32, 8, 256, 64, [390, 7], [2500, 1000], 4096),
+    ("prompts-3", 64, 64, 96, 32, [400, 391, 17, 250], [400, 1300, 64, 249], 2048),
+    ("prompts-3-group-8", 128, 16, 256, 256, [300, 290, 1], [2300, 290, 31], 4096),
     ("prompt-odd-heads", 14, 2, 96, 32, [97, 30], [97, 30], 512),
 ]
 
@@ -196,8 +201,9 @@ def test_attention(hv, cuda, case):
     _check(case, host, _run(hv, case, x))
 
 
-@pytest.mark.parametrize("case", [c for c in _ATTEND if c[0] in ("verify-ragged", "prompts")],
-                         ids=["verify", "prompts"])
+@pytest.mark.parametrize("case", [c for c in _ATTEND if c[0] in ("verify-ragged", "prompts-1", "prompts-2",
+                                                                 "prompts-3")],
+                         ids=["verify", "prompts-1", "prompts-2", "prompts-3"])
 def test_nan_values_stay_with_the_rows_that_see_them(hv, cuda, case):
     """A NaN code of V or K in a key that only later query rows see leaves the earlier rows'
     results as they are."""
@@ -214,8 +220,8 @@ def test_nan_values_stay_with_the_rows_that_see_them(hv, cuda, case):
     _check(case, host, _run(hv, case, x))
 
 
-@pytest.mark.parametrize("case", [c for c in _ATTEND if c[0] in ("splits", "prompts")],
-                         ids=["splits", "prompts"])
+@pytest.mark.parametrize("case", [c for c in _ATTEND if c[0] in ("splits", "prompts-1", "prompts-3")],
+                         ids=["splits", "prompts-1", "prompts-3"])
 def test_views_and_rows_behind_the_last_sequence(hv, cuda, case):
     """q and out as slices of wider rows, caches as planes of a layered cache; rows of out
     behind the last sequence's stay as they were."""
@@ -229,6 +235,25 @@ def test_views_and_rows_behind_the_last_sequence(hv, cuda, case):
     _run(hv, case, y, out=out[:, 2:])
     _check(case, host, out[:N, 2:])
     assert bool((out[N:] == 7).all()) and bool((out[:, :2] == 7).all())
+
+
+def test_scales_that_are_no_powers_of_two(hv, cuda):
+    """Scales of another producer: of any size, zero among them."""
+    case = ("odd-scales", 16, 8, 64, 32, [4, 2, 150], [200, 130, 150], 512)
+    host, _ = _attend_inputs(cuda, case, seed=5)
+    for k in ("ks", "vs"):
+        live = ~host[k].isnan()
+        host[k][live] = (torch.rand(int(live.sum()), generator=torch.Generator().manual_seed(1))
+                         * 0.03 + 1e-3)
+        host[k][:, 0, 3] = torch.where(live[:, 0, 3], 0.0, host[k][:, 0, 3])
+    host["vs"][:, 1, 2] *= -1
+    x = {k: v.to(cuda) for k, v in host.items()}
+    _check(case, host, _run(hv, case, x))
+    big = ("odd-scales-prompt", 16, 8, 64, 32, [1100, 2], [1200, 130], 2048)
+    host, _ = _attend_inputs(cuda, big, seed=6)
+    host["vs"] *= 0.7
+    x = {k: v.to(cuda) for k, v in host.items()}
+    _check(big, host, _run(hv, big, x))
 
 
 def test_blocks_that_the_table_does_not_have_are_left_out(hv, cuda):
