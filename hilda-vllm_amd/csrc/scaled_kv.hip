@@ -18,14 +18,16 @@
 // at the low end, and raising one by a power of two moves every other code of
 // the group without rounding it, down to e4m3's subnormals.
 //
-// Launch: one workgroup per (chunk of tokens, kv head, K or V). A workgroup
-// takes the tokens of its chunk whose predecessor in the call lies in another
-// group, looks through the call's whole slot list for the group's other tokens
-// (so the tokens of a group may stand anywhere in the call; the list is a few KB
-// and read from L2), leaves the group to the workgroup of its first token, and
-// otherwise does all of the group's work. No two workgroups write one group, and
-// a slot that occurs twice takes the row of the higher token index, so the
-// result does not depend on any order of execution.
+// Launch: a workgroup per (chunk of tokens, kv head, K or V). It takes the tokens of its
+// chunk whose predecessor in the call lies in another group, looks through the
+// call's whole slot list for the group's other tokens (so the tokens of a group may
+// stand anywhere in the call; the list is a few KB and read from L2), leaves the group to
+// the workgroup of its first token, and otherwise does all of the group's work, the rows
+// held in registers from their maximum to their codes. No two workgroups write one group
+// and head, and a slot that occurs twice takes the row of the higher token index, so the
+// result does not depend on any order of execution. The call is bound by latency - the
+// list, the rows, the codes, one after the other - and the rows that follow the first
+// token in the call, which are nearly always the group's, are loaded during the search.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -37,7 +39,6 @@
 namespace hs {
 namespace {
 
-constexpr int kSkT = 256;       // threads of a workgroup
 constexpr int kSkMinExp = -96;  // smallest exponent of a computed scale
 
 struct ScaledStoreArgs {
@@ -51,15 +52,20 @@ struct ScaledStoreArgs {
   int N, chunk, block_size, num_blocks;
 };
 
-// e4m3 codes of 8 values times `inv`, or over `s` where inv is 0
+// e4m3 codes of 8 values times `inv`, or over `s` where inv is 0, that are at most 448 or
+// NaN (v_cvt_pk_fp8_f32: round to nearest even, the same codes as f32_to_e4m3fn_sat's for
+// all of these; 2 instructions a value against about 25)
 __device__ __forceinline__ uint2 encode8(const float (&f)[8], float s, float inv) {
-  uint32_t w[2] = {0, 0};
+  float y[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float y = inv != 0.0f ? f[k] * inv : f[k] / s;
-    w[k >> 2] |= (uint32_t)f32_to_e4m3fn_sat(y) << (8 * (k & 3));
+  for (int k = 0; k < 8; ++k) y[k] = inv != 0.0f ? f[k] * inv : f[k] / s;
+  int w[2] = {0, 0};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], w[h], false);
+    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w[h], true);
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint2((uint32_t)w[0], (uint32_t)w[1]);
 }
 
 // 1 / s where that is exact (s a power of two with a normal inverse), else 0
@@ -68,17 +74,20 @@ __device__ __forceinline__ float exact_inverse(float s) {
   return ((b & 0x7fffffu) == 0 && e >= 1 && e <= 253) ? __uint_as_float((254u - e) << 23) : 0.0f;
 }
 
+// threads of a group's workgroup: 16 lanes x 8 elements to a row, 2 or 4 rows each
+constexpr int threads_of(int G) { return G <= 64 ? 256 : 4 * G; }
+
 template <int G>
-__global__ __launch_bounds__(kSkT) void k_store_scaled(ScaledStoreArgs a) {
-  constexpr int kPasses = G / 16;  // 16 rows of 16 lanes x 8 elements a pass
+__global__ __launch_bounds__(threads_of(G)) void k_store_scaled(ScaledStoreArgs a) {
+  constexpr int kT = threads_of(G), kWaves = kT / 64;
+  constexpr int kRowsAPass = kT / 16, kPasses = G / kRowsAPass;
   __shared__ int s_owner[G];
   __shared__ int s_earlier;
-  __shared__ uint32_t s_max[kSkT / 64];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int head = blockIdx.y, kv = blockIdx.z;
-  const int t0 = blockIdx.x * a.chunk;
-  const uint16_t* x = a.x[kv] + head * a.x_sh[kv];
-  uint8_t* cache = a.c[kv] + head * a.c_sh;
+  __shared__ uint32_t s_max[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, col = 8 * (tid & 15);
+  const int head = blockIdx.y, t0 = blockIdx.x * a.chunk;
+  const int v = blockIdx.z & 1, odd = blockIdx.z >> 1;  // K or V; which of the chunk's starts
+  const uint16_t* x = a.x[v] + head * a.x_sh[v] + col;
 
   // every wave finds the chunk's run starts for itself
   bool start = false;
@@ -91,40 +100,65 @@ __global__ __launch_bounds__(kSkT) void k_store_scaled(ScaledStoreArgs a) {
               a.slots[t0 + lane - 1] / G != slot / G;
     }
   }
-  for (uint64_t runs = __ballot(start); runs; runs &= runs - 1) {
+  // the chunk's starts in turn, or (two workgroups to a chunk) every other one
+  uint64_t runs = __ballot(start);
+  if (odd) runs &= runs - 1;
+  for (; runs; runs &= runs - 1, runs = gridDim.z == 4 ? runs & (runs - 1) : runs) {
     const int first = t0 + __builtin_ctzll(runs);
-    const int slot0 = a.slots[first] / G * G;
+    const int slot1 = a.slots[first], slot0 = slot1 / G * G;
+    const int blk = slot0 / a.block_size, off0 = slot0 % a.block_size;
+    const int64_t at = (int64_t)blk * a.c_sb + (int64_t)off0 * a.c_st + (int64_t)head * a.c_sh + col;
+    const int64_t sat = (int64_t)blk * a.s_sb + (int64_t)(off0 / G) * a.s_sg + (int64_t)head * a.s_sh;
+    float* scale = a.s[v] + sat;
+    const float old = *scale;
+    uint4 raw[kPasses];
+    int own[kPasses];
+    auto load = [&](int p) {
+      raw[p] = make_uint4(0, 0, 0, 0);
+      if (own[p] >= 0)
+        raw[p] = *reinterpret_cast<const uint4*>(x + (int64_t)own[p] * a.x_st[v]);
+    };
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int slot = slot0 + p * kRowsAPass + (tid >> 4), t = first + slot - slot1;
+      own[p] = slot >= slot1 && t < a.N && a.slots[t] == slot ? t : -1;
+      load(p);
+    }
     __syncthreads();  // the last group's reads of the shared arrays
-    for (int o = tid; o < G; o += kSkT) s_owner[o] = -1;
+    for (int o = tid; o < G; o += kT) s_owner[o] = -1;
     if (tid == 0) s_earlier = 0;
     __syncthreads();
     bool earlier = false;
-#pragma unroll 4
-    for (int j = tid; j < a.N; j += kSkT) {
-      const int slot = a.slots[j];
+    auto look = [&](int j, int slot) {
       const uint32_t o = (uint32_t)slot - (uint32_t)slot0;
-      if (slot >= 0 && o < (uint32_t)G) {
+      if (j < a.N && slot >= 0 && o < (uint32_t)G) {
         earlier |= j < first;
         atomicMax(&s_owner[o], j);
+      }
+    };
+    if (a.N <= kT) {
+      look(tid, a.slots[min(tid, a.N - 1)]);
+    } else {
+      for (int j = tid; j < a.N; j += 8 * kT) {
+        int slot[8];  // every load of the round before the first wait
+#pragma unroll
+        for (int i = 0; i < 8; ++i) slot[i] = a.slots[min(j + i * kT, a.N - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) look(j + i * kT, slot[i]);
       }
     }
     if (earlier) s_earlier = 1;
     __syncthreads();
     if (s_earlier) continue;  // the workgroup of an earlier token has the group
 
-    const int blk = slot0 / a.block_size, off0 = slot0 % a.block_size;
-    uint8_t* rows = cache + (int64_t)blk * a.c_sb + (int64_t)off0 * a.c_st + 8 * (tid & 15);
-    float* scale = a.s[kv] + (int64_t)blk * a.s_sb + (int64_t)(off0 / G) * a.s_sg + head * a.s_sh;
-    const float old = *scale;
-    uint4 raw[kPasses];
-    int own[kPasses];
     uint32_t most = 0;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      own[p] = s_owner[p * 16 + (tid >> 4)];
-      raw[p] = make_uint4(0, 0, 0, 0);
-      if (own[p] >= 0)
-        raw[p] = *reinterpret_cast<const uint4*>(x + (int64_t)own[p] * a.x_st[kv] + 8 * (tid & 15));
+      const int owner = s_owner[p * kRowsAPass + (tid >> 4)];
+      if (owner != own[p]) {
+        own[p] = owner;
+        load(p);
+      }
     }
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
@@ -141,7 +175,7 @@ __global__ __launch_bounds__(kSkT) void k_store_scaled(ScaledStoreArgs a) {
     if (lane == 0) s_max[tid >> 6] = most;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSkT / 64; ++w) most = max(most, s_max[w]);
+    for (int w = 0; w < kWaves; ++w) most = max(most, s_max[w]);
     // a = 1.f 2^(E - 127), 448 = 1.75 * 2^8: the exponent of the power of two
     const int E = (int)(most >> 7);
     int e = E - 135 + ((most & 0x7fu) > 0x60u ? 1 : 0);
@@ -153,13 +187,17 @@ __global__ __launch_bounds__(kSkT) void k_store_scaled(ScaledStoreArgs a) {
     const float inv = exact_inverse(now);
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      uint8_t* row = rows + (int64_t)(p * 16 + (tid >> 4)) * a.c_st;
+      uint8_t* row = a.c[v] + at + (int64_t)(p * kRowsAPass + (tid >> 4)) * a.c_st;
       if (own[p] >= 0) {
         uint16_t h[8];
         float f[8];
         unpack8(raw[p], h);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = bf(h[k]);
+        for (int k = 0; k < 8; ++k) {
+          // |x| <= 448 s by the choice of s, but for infinities, which saturate
+          const bool inf = (h[k] & 0x7fffu) == 0x7f80u;
+          f[k] = inf ? copysignf(448.0f * now, bf(h[k])) : bf(h[k]);
+        }
         *reinterpret_cast<uint2*>(row) = encode8(f, now, inv);
       } else if (raise) {
         const uint2 c = *reinterpret_cast<const uint2*>(row);
@@ -225,18 +263,21 @@ extern "C" int hs_store_kvcache_scaled(
   a.N = num_tokens;
   a.block_size = block_size;
   a.num_blocks = num_blocks;
-  // Decode rows start a group each, so a workgroup takes one token of a small call
-  // (64 tokens one by one: 16 workgroups each, all at once); prompts fill groups,
-  // so a chunk of their tokens holds a start or two
+  // Decode rows start a group each, so a workgroup takes one token of a small call;
+  // prompts fill groups, and a chunk of 32 of their tokens holds a start or, with groups
+  // of 32, two for a workgroup each (2003 tokens: 15 us, 17.5 us with one workgroup;
+  // chunks of 16 start twice as many workgroups, half of them for nothing: 4000 tokens
+  // 20.5 us against 13.7 us)
   a.chunk = 1;
   while (a.chunk < 32 && num_tokens > 64 * a.chunk) a.chunk *= 2;
-  const dim3 grid((unsigned)((num_tokens + a.chunk - 1) / a.chunk), (unsigned)num_kv_heads, 2);
+  const dim3 grid((unsigned)((num_tokens + a.chunk - 1) / a.chunk), (unsigned)num_kv_heads,
+                  a.chunk > 1 && group == 32 ? 4 : 2);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (group) {
-    case 32: hipLaunchKernelGGL(k_store_scaled<32>, grid, dim3(kSkT), 0, st, a); break;
-    case 64: hipLaunchKernelGGL(k_store_scaled<64>, grid, dim3(kSkT), 0, st, a); break;
-    case 128: hipLaunchKernelGGL(k_store_scaled<128>, grid, dim3(kSkT), 0, st, a); break;
-    default: hipLaunchKernelGGL(k_store_scaled<256>, grid, dim3(kSkT), 0, st, a); break;
+    case 32: hipLaunchKernelGGL(k_store_scaled<32>, grid, dim3(threads_of(32)), 0, st, a); break;
+    case 64: hipLaunchKernelGGL(k_store_scaled<64>, grid, dim3(threads_of(64)), 0, st, a); break;
+    case 128: hipLaunchKernelGGL(k_store_scaled<128>, grid, dim3(threads_of(128)), 0, st, a); break;
+    default: hipLaunchKernelGGL(k_store_scaled<256>, grid, dim3(threads_of(256)), 0, st, a); break;
   }
   return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
