@@ -15,10 +15,9 @@
 // the sums a factor of about 24 / 4.6, the size of 16 + c over that of c - 8, in
 // f32's last bits; an infinity in x gives NaN.)
 //
-// k_int4_rows (up to 16 rows): bound by the weights' stream. A workgroup's 8 waves
-// take every eighth step each of its one or two tiles (or a gate and an up tile),
-// with the next steps' weights and rows in flight, and join their sums in LDS. The
-// rows come from L2 in every workgroup, as B operands straight into registers.
+// k_int4_rows (up to 16 rows): bound by the weights' stream. A workgroup's waves share
+// out the steps of its one to four tiles and join their sums in LDS. The rows come from
+// L2 in every workgroup, as B operands straight into registers.
 // k_int4_tile (more rows): 128 features by 64 rows a workgroup, the rows' step in
 // LDS as B operands shared by its four waves, each with 32 features of its own;
 // the steps are split over workgroups where there are few of them, and k_int4_join
@@ -126,69 +125,53 @@ __device__ __forceinline__ void multiply(const Step<GP>& st, const bf16x8_t (&x)
   }
 }
 
-constexpr int kRowWaves = 8;
-
-// Up to 16 rows. TN: weight tiles of a workgroup (with SwiGLU a gate and an up tile);
-// kAhead: steps in flight behind the one being multiplied.
-template <int GP, int TN, bool kGate, int kAhead>
-__global__ __launch_bounds__(64 * kRowWaves) void k_int4_rows(Int4Args a) {
-  __shared__ float s_part[kRowWaves][TN][16][16];  // [wave][tile][row][feature]
+// Up to 16 rows. W: waves of a workgroup; TN: its weight tiles (with SwiGLU half of them
+// gate and half up tiles).
+template <int GP, int W, int TN, bool kGate>
+__global__ __launch_bounds__(64 * W) void k_int4_rows(Int4Args a) {
+  constexpr int kOut = kGate ? TN / 2 : TN;
+  __shared__ float s_part[W][TN][16][16];  // [wave][tile][row][feature]
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u0 = blockIdx.x * (kGate ? 1 : TN);
+  const int u0 = blockIdx.x * kOut;
   int tile[TN];
 #pragma unroll
-  for (int t = 0; t < TN; ++t) tile[t] = kGate ? u0 + t * a.up : min(u0 + t, a.units - 1);
-  struct Stage {
-    Step<GP> w[TN];
-    bf16x8_t x[4];
-  } st[kAhead];
-  // past its last step a wave loads its first again (cached, and never multiplied):
-  // conditional loads would make every wait cover all loads in flight
-  auto load = [&](Stage& s, int step) {
-    if (step >= a.steps) step = min(wave, a.steps - 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s.x[i] = load_x(a, m, step, i, g);
-#pragma unroll
-    for (int t = 0; t < TN; ++t) load_step<GP>(a, tile[t], step, lane, s.w[t]);
-  };
-#pragma unroll
-  for (int d = 0; d < kAhead; ++d) load(st[d], wave + d * kRowWaves);
+  for (int t = 0; t < TN; ++t) tile[t] = min(u0 + t % kOut, a.units - 1) + t / kOut * a.up;
   f32x4_t y[TN];
 #pragma unroll
   for (int t = 0; t < TN; ++t) y[t] = f32x4_t{0, 0, 0, 0};
-  for (int step = wave; step < a.steps;) {
+  // One step's loads at a time: many waves hide them better than many loads of few waves
+  // (12288 features, SwiGLU, 4 rows: 20.8 us with 8 waves and two steps ahead, 17.3 us so)
+  for (int step = wave; step < a.steps; step += W) {
+    bf16x8_t x[4];
+    Step<GP> w[TN];
 #pragma unroll
-    for (int d = 0; d < kAhead; ++d) {
-      if (step < a.steps) {
-        float c0[GP];
+    for (int t = 0; t < TN; ++t) load_step<GP>(a, tile[t], step, lane, w[t]);
 #pragma unroll
-        for (int p = 0; p < GP; ++p) {
-          f32x4_t acc = {0, 0, 0, 0};
+    for (int i = 0; i < 4; ++i) x[i] = load_x(a, m, step, i, g);
+    float c0[GP];
 #pragma unroll
-          for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i) acc = mfma(minus24(), st[d].x[i], acc);
-          c0[p] = acc[0];
-        }
+    for (int p = 0; p < GP; ++p) {
+      f32x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < TN; ++t) multiply<GP>(st[d].w[t], st[d].x, c0, y[t]);
-      }
-      load(st[d], step + kAhead * kRowWaves);
-      step += kRowWaves;
+      for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i) acc = mfma(minus24(), x[i], acc);
+      c0[p] = acc[0];
     }
+#pragma unroll
+    for (int t = 0; t < TN; ++t) multiply<GP>(w[t], x, c0, y[t]);
   }
   if (m < a.rows) {
 #pragma unroll
     for (int t = 0; t < TN; ++t) *reinterpret_cast<f32x4_t*>(&s_part[wave][t][m][4 * g]) = y[t];
   }
   __syncthreads();
-  constexpr int kOut = kGate ? 1 : TN;
-  for (int e = threadIdx.x; e < 16 * a.rows * kOut; e += 64 * kRowWaves) {
+  for (int e = threadIdx.x; e < 16 * a.rows * kOut; e += 64 * W) {
     const int n = e & 15, t = (e >> 4) % kOut, row = (e >> 4) / kOut;
     float v = 0.0f, up = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       v += s_part[w][t][row][n];
-      if (kGate) up += s_part[w][TN - 1][row][n];
+      if (kGate) up += s_part[w][kOut + t][row][n];
     }
     const int col = (u0 + t) * 16 + n;
     if (col < a.N) a.y[(int64_t)row * a.ys + col] = to_bf(kGate ? silu(v) * up : v);
@@ -196,10 +179,23 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_int4_rows(Int4Args a) {
 }
 
 constexpr int kTileRows = 64, kTileWaves = 4;
+constexpr int kPast = INT32_MAX - 511;  // a byte offset past any row: reads zeros
 
-// 32 output features a wave (with SwiGLU 16, gate and up) by 64 rows.
+// waits for the wave's LDS traffic only: the next step's loads stay in flight
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ uint4 as_uint4(u32x4_t v) { return make_uint4(v.x, v.y, v.z, v.w); }
+
+// 32 output features a wave (with SwiGLU 16, gate and up) by 64 rows. The next step's loads
+// are in flight during a step, issued alike whatever is left: past the end their buffers
+// are empty and they touch no memory. Two and three steps ahead took the same time or
+// longer; what bounds it is a wave's own chain of operand reads, code shifts and products.
+// 64 rows of 9728 inputs, 2560 features: 25.7 us (250 TFLOP/s, about 6 of them the join);
+// 600 rows of 2560 inputs, 2 x 9728 features: 172 us (704 TFLOP/s).
 template <int GP, bool kGate>
-__global__ __launch_bounds__(64 * kTileWaves) void k_int4_tile(Int4Args a) {
+__global__ __launch_bounds__(64 * kTileWaves, 3) void k_int4_tile(Int4Args a) {
   constexpr int RT = kTileRows / 16;
   __shared__ uint4 s_x[2][4][RT][64];      // [step parity][i][row tile][lane]
   __shared__ float s_c[2][GP][kTileRows];  // -24 sum x
@@ -214,13 +210,35 @@ __global__ __launch_bounds__(64 * kTileWaves) void k_int4_tile(Int4Args a) {
   const int ub = kGate ? ua + a.up : min(u0 + 1, a.units - 1);
 
   static_assert(RT == kTileWaves, "a wave stages one row tile");
-  bf16x8_t xr[4];
-  Step<GP> wa, wb;
+  u32x4_t x[4];
+  Step<GP> w[2];
+  const int row_at = r0 + 16 * wave + m < a.rows ? (16 * wave + m) * (int)a.xs * 2 + 16 * g
+                                                 : kPast;
+  const int64_t wa0 = (int64_t)ua * a.steps, wb0 = (int64_t)ub * a.steps;
   auto load = [&](int step) {
+    const bool live = step < last;
+    const int k = kStep * min(step, a.steps - 1);
+    const int64_t at = live ? step : 0;
+    const auto xb = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(a.x + (int64_t)r0 * a.xs + k), 0, live ? kPast : 0, 0x00027000);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xr[i] = load_x(a, r0 + 16 * wave + m, step, i, g);
-    load_step<GP>(a, ua, step, lane, wa);
-    load_step<GP>(a, ub, step, lane, wb);
+    for (int i = 0; i < 4; ++i)
+      x[i] = __builtin_amdgcn_raw_buffer_load_b128(
+          xb, k + 32 * i + 8 * g < a.K && row_at != kPast ? row_at + 64 * i : kPast, 0, 0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t tile = (t ? wb0 : wa0) + at;
+      const auto wb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint4*>(a.w + tile * 64), 0,
+                                                        live ? 1024 : 0, 0x00027000);
+      const auto sb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.sc + tile * GP * 16), 0,
+                                                        live ? 32 * GP : 0, 0x00027000);
+      w[t].w = as_uint4(__builtin_amdgcn_raw_buffer_load_b128(wb, 16 * lane, 0, 0));
+#pragma unroll
+      for (int p = 0; p < GP; ++p) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(sb, 32 * p + 8 * g, 0, 0);
+        w[t].s[p] = make_uint2(v[0], v[1]);
+      }
+    }
   };
   f32x4_t y[2][RT];
 #pragma unroll
@@ -228,17 +246,18 @@ __global__ __launch_bounds__(64 * kTileWaves) void k_int4_tile(Int4Args a) {
   load(first);
   for (int step = first, par = 0; step < last; ++step, par ^= 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s_x[par][i][wave][lane] = __builtin_bit_cast(uint4, xr[i]);
+    for (int i = 0; i < 4; ++i) s_x[par][i][wave][lane] = as_uint4(x[i]);
 #pragma unroll
     for (int p = 0; p < GP; ++p) {
       f32x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i) acc = mfma(minus24(), xr[i], acc);
+      for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i)
+        acc = mfma(minus24(), __builtin_bit_cast(bf16x8_t, x[i]), acc);
       if (g == 0) s_c[par][p][16 * wave + m] = acc[0];
     }
-    const Step<GP> ca = wa, cb = wb;
-    if (step + 1 < last) load(step + 1);
-    __syncthreads();
+    const Step<GP> ca = w[0], cb = w[1];
+    load(step + 1);
+    lds_barrier();
     const uint32_t qa[4] = {ca.w.x, ca.w.y, ca.w.z, ca.w.w};
     const uint32_t qb[4] = {cb.w.x, cb.w.y, cb.w.z, cb.w.w};
 #pragma unroll
@@ -343,23 +362,32 @@ Int4Plan plan_of(int rows, int K, int N, bool gate) {
   return p;
 }
 
+template <int GP, int W, int TN, bool kGate>
+void launch_rows(const Int4Args& a, hipStream_t s) {
+  constexpr int kOut = kGate ? TN / 2 : TN;
+  hipLaunchKernelGGL((k_int4_rows<GP, W, TN, kGate>),
+                     dim3((unsigned)((a.units + kOut - 1) / kOut)), dim3(64 * W), 0, s, a);
+}
+
+// Many tiles: workgroups of 4 waves, several of which fit a CU and hide each other's
+// beginning and end, and of several tiles, which share the rows' loads (151936 features, 4
+// rows: 93 us with 8 waves and 2 tiles, 75 us with 4 and 2, 66 us with 4 and 4: 4.9 TB/s).
+// Few: 8 waves to one tile, so that each CU has its tile's steps in flight at once (4096 by
+// 4096, 4 rows: 6.4 us, 7.5 us with 4), more where there are many steps (12288 inputs, 8
+// rows: 13.2 us with 12, 15.4 us with 8).
 template <int GP>
-void launch_rows(const Int4Args& a, bool gate, hipStream_t s) {
-  const dim3 block(64 * kRowWaves);
-  if (gate) {
-    hipLaunchKernelGGL((k_int4_rows<GP, 2, true, 2>), dim3((unsigned)a.units), block, 0, s, a);
-  } else if (a.units >= 4 * kCus) {  // two tiles share the rows' loads
-    hipLaunchKernelGGL((k_int4_rows<GP, 2, false, 2>), dim3((unsigned)((a.units + 1) / 2)), block,
-                       0, s, a);
-  } else {
-    hipLaunchKernelGGL((k_int4_rows<GP, 1, false, 2>), dim3((unsigned)a.units), block, 0, s, a);
-  }
+void dispatch_rows(const Int4Args& a, bool gate, hipStream_t s) {
+  if (gate) launch_rows<GP, 4, 2, true>(a, s);
+  else if (a.units >= 12 * kCus) launch_rows<GP, 4, 4, false>(a, s);
+  else if (a.units >= 4 * kCus) launch_rows<GP, 4, 2, false>(a, s);
+  else if (a.steps < 64) launch_rows<GP, 8, 1, false>(a, s);
+  else launch_rows<GP, 12, 1, false>(a, s);
 }
 
 template <int GP>
 int launch(const Int4Args& a, const Int4Plan& p, bool gate, hipStream_t s) {
   if (p.rows) {
-    launch_rows<GP>(a, gate, s);
+    dispatch_rows<GP>(a, gate, s);
     return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
   }
   const int per = gate ? kTileWaves : 2 * kTileWaves;
@@ -405,10 +433,11 @@ int hs_linear_int4(const void* x, int64_t x_stride, const void* packed, const vo
   // gate and up halves start at a tile each
   if (gate && out_features % 16) return HS_ERR_UNSUPPORTED;
   // grids and 32-bit element counts of the kernels
-  if (rows > (1 << 20) || in_features > (1 << 24) || out_features > (1 << 24))
+  if (rows > (1 << 20) || in_features > (1 << 23) || out_features > (1 << 24))
     return HS_ERR_UNSUPPORTED;
   if ((x_stride % 8) || x_stride < in_features || out_stride < out_features)
     return HS_ERR_UNSUPPORTED;
+  if (x_stride > (1 << 23)) return HS_ERR_UNSUPPORTED;  // 64 rows within 1 GiB
   if (((uintptr_t)x | (uintptr_t)packed) & 15) return HS_ERR_UNSUPPORTED;
   if (((uintptr_t)scales & 7) || ((uintptr_t)out & 1)) return HS_ERR_UNSUPPORTED;
   const Int4Plan p = plan_of(rows, in_features, out_features, gate);

@@ -1065,7 +1065,7 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, *, swiglu: bool = False,
             not packed.is_contiguous() or not scales.is_contiguous():
         raise ValueError("weight is not laid out as pack_int4 does")
     N = w.out_features // 2 if swiglu else w.out_features
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16 or not K <= x.stride(0) <= 1 << 23:
         x = x.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = x.new_empty((M, N))

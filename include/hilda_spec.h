@@ -541,7 +541,7 @@ int hs_linear_rmsnorm(const void* x, int64_t x_stride, const void* residual_in,
 /* 32 i + 8 (l / 16) + e, e = 0 .. 7, input 2 p at bits 4 p and input 2 p + 1   */
 /* at bits 16 + 4 p. scales: bf16 [tiles][steps * 128 / group][16]. Rows past   */
 /* the last and inputs past in_features are padded with code 8 and scale 0.     */
-/* x_stride: a multiple of 8 elements; x and packed 16-byte, scales 8-byte      */
+/* x_stride: a multiple of 8 elements, at most 2^23; x and packed 16-byte, scales 8-byte */
 /* aligned. The workspace (for more than 16 rows of a narrow weight) needs no   */
 /* preparation and holds nothing between calls.                                */
 size_t hs_linear_int4_workspace_size(int rows, int in_features, int out_features, int epilogue);
