@@ -7,7 +7,8 @@ layer's RMSNorm (and residual add) computed in their prologue and SwiGLU in the
 gate_up epilogue, q/k-norm + RoPE fused with the KV-cache store, and the paged
 attention; prefill-sized projections are hipBLASLt GEMMs through torch behind
 the standalone RMSNorm kernel. Weights are N(0, 0.02^2) in bf16 (no checkpoint
-is loaded).
+is loaded); Qwen3Host.quantize_int4 turns the projections into 4-bit weights with
+group scales, which run behind the standalone RMSNorm kernel at every size.
 """
 from __future__ import annotations
 
@@ -56,6 +57,19 @@ def add_rms_norm(x, residual, w, eps):
     res = xf.to(x.dtype)
     xf = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     return xf.to(x.dtype) * w, res
+
+
+def _norm_proj(x, norm, eps, w, residual=None, swiglu=False):
+    """ops.linear_rmsnorm, or with a 4-bit weight the RMSNorm kernel and its projection
+    (the residual is then updated in place)."""
+    if isinstance(w, _ops.Int4Weight):
+        xn = _ops.rmsnorm(x, norm, eps, residual=residual)
+        return _ops.linear_int4(xn, w, swiglu=swiglu), (x if residual is None else residual)
+    return _ops.linear_rmsnorm(x, norm, eps, w, residual=residual, swiglu=swiglu)
+
+
+def _proj(x, w):
+    return _ops.linear_int4(x, w) if isinstance(w, _ops.Int4Weight) else _ops.linear(x, w)
 
 
 class Rope(nn.Module):
@@ -111,7 +125,7 @@ class Qwen3Layer(nn.Module):
         decode and verify steps, two for prefill); o projection; post-attention RMSNorm
         inside the gate_up projection with SwiGLU; down projection."""
         g = self.g
-        qkv, residual = _ops.linear_rmsnorm(h, self.ln1, g.rms_eps, self.qkv, residual=residual)
+        qkv, residual = _norm_proj(h, self.ln1, g.rms_eps, self.qkv, residual)
         attn = self.attn
         ctx = get_context()
         attn._check_bound(ctx)
@@ -132,14 +146,22 @@ class Qwen3Layer(nn.Module):
             # q/k-norm + RoPE + KV store + attention: one launch for decode and verify steps
             o = attn.attend_qkv(qkv, self.q_norm, self.k_norm, self.rope.cos_sin, positions,
                                 g.rms_eps)
-        h = _ops.linear(o.reshape(o.shape[0], -1), self.o)
-        x, residual = _ops.linear_rmsnorm(h, self.ln2, g.rms_eps, self.gate_up, residual=residual,
-                                          swiglu=True)
-        h = _ops.linear(x, self.down)
+        h = _proj(o.reshape(o.shape[0], -1), self.o)
+        x, residual = _norm_proj(h, self.ln2, g.rms_eps, self.gate_up, residual, swiglu=True)
+        h = _proj(x, self.down)
         return h, residual
 
+    def quantize_int4(self, group: int = 128):
+        """The four projections to 4-bit weights (ops.quantize_int4)."""
+        for name in ("qkv", "o", "gate_up", "down"):
+            w = getattr(self, name)
+            if not isinstance(w, _ops.Int4Weight):
+                q = _ops.quantize_int4(w, group)
+                delattr(self, name)
+                setattr(self, name, q)
+
     def forward_reference(self, positions, h, residual):
-        """Eager PyTorch restatement of the same layer (used by tests)."""
+        """Eager PyTorch restatement of the same layer (used by tests; bf16 weights)."""
         g = self.g
         if residual is None:
             x, residual = rms_norm(h, self.ln1, g.rms_eps), h
@@ -200,6 +222,18 @@ class Qwen3Host(nn.Module):
                 requires_grad=False)
         torch.cuda.set_rng_state(gen_state, device)
 
+    def quantize_int4(self, group: int = 128, lm_head: bool = False) -> "Qwen3Host":
+        """Every layer's projections (and with lm_head=True the LM head; a tied
+        embedding stays as it is) to 4-bit weights with one scale per `group` inputs.
+        A model that shares this one's weights keeps those it was built with."""
+        for layer in self.layers:
+            layer.quantize_int4(group)
+        if lm_head and not isinstance(self.lm_head, _ops.Int4Weight):
+            q = _ops.quantize_int4(self.lm_head, group)
+            del self.lm_head
+            self.lm_head = q
+        return self
+
     def attention_layers(self):
         return [layer.attn for layer in self.layers]
 
@@ -217,4 +251,4 @@ class Qwen3Host(nn.Module):
         return _ops.rmsnorm(h, self.norm, self.g.rms_eps, residual=residual)
 
     def compute_logits(self, h):
-        return _ops.linear(h, self.lm_head)
+        return _proj(h, self.lm_head)

@@ -15,7 +15,12 @@ around the gfx950 kernels:
     graph and replayed (one pair of graphs per gamma);
   * with adaptive=True gamma follows the acceptance-rate controller of
     llm_engine.py:197-208 (AdaptiveGamma); the step's accepted/proposed
-    totals are read back after every step, as the reference does on the host.
+    totals are read back after every step, as the reference does on the host;
+  * kv_cache_dtype="fp8_block" keeps the target's K/V in e4m3 with one scale per
+    kv_group tokens and kv head, found as the rows are stored (no calibration);
+  * with logprobs=n every verify phase also leaves the target's log-probabilities
+    of the emitted tokens, its rows' entropy and the n most likely tokens of each
+    row (runner.logprobs), and prefill those of the first tokens (first_logprobs).
 Uniforms are drawn on the device from torch's generator (graph-safe).
 """
 from __future__ import annotations
@@ -39,7 +44,16 @@ class SpecRunner:
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                  mode: str = "reference", eos: int = -1, k_scale: float | None = None,
                  v_scale: float | None = None, device="cuda", adaptive: bool = False,
-                 max_gamma: int | None = None, chain_steps: bool | None = None):
+                 max_gamma: int | None = None, chain_steps: bool | None = None,
+                 kv_group: int = 32, logprobs: int | None = None):
+        if kv_cache_dtype == "fp8_block":
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("k_scale / v_scale belong to kv_cache_dtype fp8: fp8_block "
+                                 "keeps a scale per group")
+            if kv_group not in (32, 64, 128, 256) or block_size % kv_group:
+                raise ValueError("kv_group must be 32, 64, 128 or 256 and divide block_size")
+        if logprobs is not None and not 0 <= int(logprobs) <= min(32, target.g.vocab):
+            raise ValueError("logprobs must lie in 0 .. 32")
         filters = 0 < top_k < target.g.vocab or top_p < 1.0
         # reference mode with top-k / top-p draws the draft tokens from the filtered
         # Sampler and keeps the unfiltered softmax as the draft probabilities
@@ -60,12 +74,22 @@ class SpecRunner:
         self.device = torch.device("cuda", ops._dev_index(device))
         self.V = target.g.vocab
         dev = self.device
-        kv_dtype = torch.float8_e4m3fn if kv_cache_dtype == "fp8" else torch.bfloat16
+        kv_dtype = (torch.float8_e4m3fn if kv_cache_dtype in ("fp8", "fp8_block")
+                    else torch.bfloat16)
         tg, dg = target.g, draft.g
         self.kv = torch.zeros((2, len(target.layers), self.num_blocks, block_size,
                                tg.num_kv_heads, tg.head_dim), dtype=kv_dtype, device=dev)
         self.dkv = torch.zeros((2, len(draft.layers), self.num_blocks, block_size,
                                 dg.num_kv_heads, dg.head_dim), dtype=torch.bfloat16, device=dev)
+        self.kv_block_scales = None
+        if kv_cache_dtype == "fp8_block":
+            # zeros: a group starts with the store of its first rows
+            self.kv_block_scales = torch.zeros(
+                (2, len(target.layers), self.num_blocks, block_size // kv_group,
+                 tg.num_kv_heads), dtype=torch.float32, device=dev)
+        # alternatives a row (None: no log-probabilities)
+        self.top_logprobs = None if logprobs is None else int(logprobs)
+        self.logprobs = self.first_logprobs = None
         kmax = max_model_len + self.max_gamma + 2
         # FP8 per-tensor scales: given, or calibrated from the prompt by prefill()
         self.kv_calibrate = kv_cache_dtype == "fp8" and k_scale is None and v_scale is None
@@ -74,6 +98,8 @@ class SpecRunner:
             a.kv_cache_dtype = kv_cache_dtype
             a.k_scale = 1.0 if k_scale is None else float(k_scale)
             a.v_scale = 1.0 if v_scale is None else float(v_scale)
+            if self.kv_block_scales is not None:
+                a.k_scales, a.v_scales = self.kv_block_scales[0, i], self.kv_block_scales[1, i]
             a.max_model_len = kmax
         for i, a in enumerate(draft.attention_layers()):
             a.k_cache, a.v_cache = self.dkv[0, i], self.dkv[1, i]
@@ -133,7 +159,8 @@ class SpecRunner:
                 u_acc=u_all[g * B:2 * g * B].view(B, g),
                 u_res=u_all[2 * g * B:],
                 elig=torch.zeros(B, dtype=torch.int32, device=dev),
-                graphs=None, last=None, graph_last=None, logits=None, graph_logits=None)
+                graphs=None, last=None, graph_last=None, logits=None, graph_logits=None,
+                logprobs=None, graph_logprobs=None)
             self._per_gamma[g] = G
         return G
 
@@ -223,6 +250,8 @@ class SpecRunner:
         last = h[cu[1:].long() - 1]
         logits = self.target.compute_logits(last)
         first = self.sampler(logits, self.temps, self.top_ks, self.top_ps)
+        if self.top_logprobs is not None:
+            self.first_logprobs = ops.token_logprobs(logits, first, top=self.top_logprobs)
         set_context(True, cu, cu, max(lens), max(lens), slots, None, self.state.block_tables)
         self.draft(ids, pos)
         reset_context()
@@ -262,8 +291,9 @@ class SpecRunner:
         """Fraction of the FP8 target cache's codes in use (the blocks of the running
         sequences' tables) that sit at the e4m3fn saturation value +-448 (codes 0x7e,
         0xfe): values the per-tensor scales clipped. 0 for a bf16 cache. Reads the
-        cache back (a diagnostic, synchronises)."""
-        if self.kv.dtype != torch.float8_e4m3fn:
+        cache back (a diagnostic, synchronises). A cache with group scales clips
+        nothing (its largest values sit between 224 and 448 by design): 0."""
+        if self.kv.dtype != torch.float8_e4m3fn or self.kv_block_scales is not None:
             return 0.0
         nb = self.state.num_seq_blocks.cpu().tolist()
         bt = self.state.block_tables.cpu()
@@ -429,6 +459,15 @@ class SpecRunner:
         G.last = (nacc, out, olen)
         G.logits = logits  # the acceptance call's target rows (read by checks)
         self.last = G.last
+        if self.top_logprobs is not None:
+            # softmax(logits) as the target gives it, no temperature or filter; row j of a
+            # sequence is the one its j-th emitted token was accepted or drawn from.
+            # Entries past the sequence's out_len mean nothing.
+            lp = ops.token_logprobs(logits.view(-1, self.V), out.reshape(-1),
+                                    top=self.top_logprobs)
+            G.logprobs = self.logprobs = {
+                k: None if t is None else t.view(self.B, g + 1, *t.shape[1:])
+                for k, t in lp.items()}
 
     def step(self):
         """One eager speculative step (then the gamma update when adaptive)."""
@@ -484,7 +523,7 @@ class SpecRunner:
         # the captured verify phase rebinds G.last to the graph's output tensors, which
         # hold nothing until the first replay: keep the eager step's outputs as the
         # last results and switch to the graph's on replay
-        eager_last, eager_logits = G.last, G.logits
+        eager_last, eager_logits, eager_logprobs = G.last, G.logits, G.logprobs
         gd, gv = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
@@ -497,9 +536,10 @@ class SpecRunner:
         torch.cuda.synchronize()
         self._restore(snap)  # capture executed nothing, but keep the state exact
         G.graphs = (gd, gv)
-        G.graph_last, G.graph_logits = G.last, G.logits
+        G.graph_last, G.graph_logits, G.graph_logprobs = G.last, G.logits, G.logprobs
         G.last = self.last = eager_last
         G.logits = eager_logits
+        G.logprobs = self.logprobs = eager_logprobs
 
     def replay(self):
         G = self._g()
@@ -508,6 +548,7 @@ class SpecRunner:
         gv.replay()
         G.last = self.last = G.graph_last
         G.logits = G.graph_logits
+        G.logprobs = self.logprobs = G.graph_logprobs
 
     def _snapshot(self):
         st = self.state

@@ -21,6 +21,10 @@ kv_cache_dtype "fp8" means float8_e4m3fn caches with per-tensor scales
 k_scale / v_scale, used by every phase (the reference keeps a separate BF16
 prefill cache for verify, attention.py:114-131; one FP8 cache keeps the
 accepted tokens' K/V in the cache decode reads).
+kv_cache_dtype "fp8_block" means float8_e4m3fn caches with one f32 scale per group
+of tokens and kv head, k_scales / v_scales [num_blocks, block_size / group, Hkv]
+(ops.store_kvcache_scaled): the scales follow the rows as they are stored, so
+nothing is calibrated and no row saturates.
 """
 from __future__ import annotations
 
@@ -56,6 +60,8 @@ class Attention(nn.Module):
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = 1.0
         self.v_scale = 1.0
+        # "fp8_block": the scales of token groups, bound with the caches
+        self.k_scales = self.v_scales = torch.tensor([])
         # upper bound of keys per sequence used to size the launch (set by the runner
         # for graph capture; 0 means "use the context's max_seqlen_k")
         self.max_model_len = 0
@@ -69,13 +75,19 @@ class Attention(nn.Module):
         if ctx.block_tables is None:
             raise RuntimeError("Attention over the cache needs context.block_tables")
 
+    def _store(self, k, v, slots):
+        if self.kv_cache_dtype == "fp8_block":
+            _ops.store_kvcache_scaled(k, v, self.k_cache, self.v_cache, self.k_scales,
+                                      self.v_scales, slots)
+        else:
+            store_kvcache(k, v, self.k_cache, self.v_cache, slots, self.k_scale, self.v_scale)
+
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         ctx = get_context()
         k = k.view(-1, self.num_kv_heads, self.head_dim)
         v = v.view(-1, self.num_kv_heads, self.head_dim)
         if self.k_cache.numel() and self.v_cache.numel():
-            store_kvcache(k, v, self.k_cache, self.v_cache, ctx.slot_mapping, self.k_scale,
-                          self.v_scale)
+            self._store(k, v, ctx.slot_mapping)
         if ctx.is_prefill and ctx.block_tables is None:
             # attention.py:147-160 with block_table None: the step's own k / v
             q = q.view(-1, self.num_heads, self.head_dim)
@@ -90,6 +102,10 @@ class Attention(nn.Module):
         self._check_bound(ctx)
         q = q.view(-1, self.num_heads, self.head_dim)
         cu_q, cu_k, max_q, max_k = self._bounds(ctx, q.shape[0], q.device)
+        if self.kv_cache_dtype == "fp8_block":
+            return _ops.verify_attention_scaled(q, self.k_cache, self.v_cache, self.k_scales,
+                                                self.v_scales, ctx.block_tables, cu_q, cu_k,
+                                                max_q, max_k, self.scale)
         return _ops.verify_attention(q, self.k_cache, self.v_cache, ctx.block_tables, cu_q, cu_k,
                                      max_q, max_k, self.scale, k_scale=self.k_scale,
                                      v_scale=self.v_scale)
@@ -98,9 +114,17 @@ class Attention(nn.Module):
                    positions: torch.Tensor, eps: float) -> torch.Tensor:
         """q/k-norm + RoPE of the fused qkv rows, the K/V store of the current tokens
         and the attention, one launch for decode and verify steps
-        (ops.qk_norm_rope_attend; qwen3.py:83-86 then forward)."""
+        (ops.qk_norm_rope_attend; qwen3.py:83-86 then forward). A cache with group
+        scales takes three: the store finds a group's largest value before it writes
+        a code of it."""
         ctx = get_context()
         self._check_bound(ctx)
+        if self.kv_cache_dtype == "fp8_block":
+            q, k = _ops.qk_norm_rope(qkv, self.num_heads, self.num_kv_heads, q_norm, k_norm,
+                                     cos_sin, positions, eps)
+            v = qkv[:, (self.num_heads + self.num_kv_heads) * self.head_dim:]
+            self._store(k, v.unflatten(1, (self.num_kv_heads, self.head_dim)), ctx.slot_mapping)
+            return self.attend(q)
         cu_q, cu_k, max_q, max_k = self._bounds(ctx, qkv.shape[0], qkv.device)
         return _ops.qk_norm_rope_attend(qkv, self.num_heads, self.num_kv_heads, q_norm, k_norm,
                                         cos_sin, positions, eps, self.k_cache, self.v_cache,
