@@ -52,13 +52,17 @@ struct ScaledStoreArgs {
   int N, chunk, block_size, num_blocks;
 };
 
-// e4m3 codes of 8 values times `inv`, or over `s` where inv is 0, that are at most 448 or
+// e4m3 codes of 8 values times `inv`, or over `s` where inv is 0, that are at most 448, or
+// infinities, which saturate (before the conversion: 448 s may be past f32's largest), or
 // NaN (v_cvt_pk_fp8_f32: round to nearest even, the same codes as f32_to_e4m3fn_sat's for
 // all of these; 2 instructions a value against about 25)
 __device__ __forceinline__ uint2 encode8(const float (&f)[8], float s, float inv) {
   float y[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) y[k] = inv != 0.0f ? f[k] * inv : f[k] / s;
+  for (int k = 0; k < 8; ++k) {
+    y[k] = inv != 0.0f ? f[k] * inv : f[k] / s;
+    if (fabsf(f[k]) == INFINITY) y[k] = copysignf(448.0f, f[k]);
+  }
   int w[2] = {0, 0};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -193,21 +197,20 @@ __global__ __launch_bounds__(threads_of(G)) void k_store_scaled(ScaledStoreArgs 
         float f[8];
         unpack8(raw[p], h);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          // |x| <= 448 s by the choice of s, but for infinities, which saturate
-          const bool inf = (h[k] & 0x7fffu) == 0x7f80u;
-          f[k] = inf ? copysignf(448.0f * now, bf(h[k])) : bf(h[k]);
-        }
+        for (int k = 0; k < 8; ++k) f[k] = bf(h[k]);  // |x| <= 448 s by the choice of s
         *reinterpret_cast<uint2*>(row) = encode8(f, now, inv);
       } else if (raise) {
         const uint2 c = *reinterpret_cast<const uint2*>(row);
+        // the new scale is a power of two from 2^-96 to 2^120, so the quotient of the
+        // scales rounds only where no code survives it; 448 old may overflow
+        const float shrink = old * inv;
         float f[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t b = (k < 4 ? c.x : c.y) >> (8 * (k & 3));
-          f[k] = __builtin_amdgcn_cvt_f32_fp8((int)b, 0) * old;
+          f[k] = __builtin_amdgcn_cvt_f32_fp8((int)b, 0) * shrink;
         }
-        *reinterpret_cast<uint2*>(row) = encode8(f, now, inv);
+        *reinterpret_cast<uint2*>(row) = encode8(f, 1.0f, 1.0f);
       }
     }
     if (tid == 0) *scale = now;  // every thread read the old one before the last barrier

@@ -313,3 +313,26 @@ def test_two_streams_and_a_replayed_graph(hv, cuda):
             torch.cuda.synchronize()
             assert torch.equal(out.view(torch.int16), want[i].view(torch.int16))
             assert torch.equal(eager.view(torch.int16), want[1 - i].view(torch.int16))
+
+
+def test_store_at_the_ends_of_the_range(hv, cuda):
+    """Scales whose 448-fold is past the largest f32: an infinity still saturates, and the
+    group's other codes still move to the raised scale."""
+    print("scaled store, largest scales", flush=True)
+    gen = torch.Generator().manual_seed(2)
+    olds = [1.3e36, 0.0, 1e37, 2.0 ** -120, 3e38]  # of five blocks of one group each
+    slots = [5, 32, 64 + 9, 96 + 1, 128 + 30]
+    k = torch.randn(5, 1, D, generator=gen).to(torch.bfloat16)
+    k[:, :, 0], k[:, :, 1], k[:, :, 2] = 3.3e38, float("inf"), float("-inf")
+    v = (torch.randn(5, 1, D, generator=gen) * 1e30).to(torch.bfloat16)
+    v[:, :, 7] = float("-inf")
+    codes = (torch.randn(5, 32, 1, D, generator=gen) * 300).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.tensor(olds).view(5, 1, 1)
+    dk, dv, dks, dvs = (t.clone().to(cuda) for t in (codes, codes, scales, scales))
+    want = [t.double().numpy().copy() for t in (codes, codes, scales, scales)]
+    hv.ops.store_kvcache_scaled(k.to(cuda), v.to(cuda), dk, dv, dks, dvs,
+                                torch.tensor(slots, dtype=torch.int32, device=cuda))
+    ref.store(k.double().numpy(), want[0], want[2], slots)
+    ref.store(v.double().numpy(), want[1], want[3], slots)
+    for got, w in zip((dk, dv, dks, dvs), want):
+        assert np.array_equal(got.double().cpu().numpy(), w, equal_nan=True)
