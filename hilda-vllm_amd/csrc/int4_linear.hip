@@ -19,9 +19,9 @@
 // out the steps of its one to four tiles and join their sums in LDS. The rows come from
 // L2 in every workgroup, as B operands straight into registers.
 // k_int4_tile (more rows): 128 features by 64 rows a workgroup, the rows' step in
-// LDS as B operands shared by its four waves, each with 32 features of its own;
-// the steps are split over workgroups where there are few of them, and k_int4_join
-// adds the parts.
+// LDS as B operands shared by its four waves, each with 32 features of its own; where
+// there are few workgroups the steps are split over two sets of waves and over
+// workgroups, whose parts k_int4_join adds.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -192,15 +192,19 @@ __device__ __forceinline__ uint4 as_uint4(u32x4_t v) { return make_uint4(v.x, v.
 // are in flight during a step, issued alike whatever is left: past the end their buffers
 // are empty and they touch no memory. Two and three steps ahead took the same time or
 // longer; what bounds it is a wave's own chain of operand reads, code shifts and products.
-// 64 rows of 9728 inputs, 2560 features: 25.7 us (250 TFLOP/s, about 6 of them the join);
-// 600 rows of 2560 inputs, 2 x 9728 features: 172 us (704 TFLOP/s).
-template <int GP, bool kGate>
-__global__ __launch_bounds__(64 * kTileWaves, 3) void k_int4_tile(Int4Args a) {
+// H = 2: two sets of waves, each with rows of its own in LDS, take the steps in turn and
+// join their sums in LDS. 64 rows of 12288 inputs, 4096 features: 23.0 us (280 TFLOP/s, 5
+// of them the join's launch); 600 rows of 4096 inputs, 2 x 12288 features: 170 us (711 TFLOP/s).
+template <int GP, bool kGate, int H>
+__global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2) void k_int4_tile(Int4Args a) {
   constexpr int RT = kTileRows / 16;
-  __shared__ uint4 s_x[2][4][RT][64];      // [step parity][i][row tile][lane]
-  __shared__ float s_c[2][GP][kTileRows];  // -24 sum x
+  __shared__ uint4 s_xs[H][2][4][RT][64];      // [half][step parity][i][row tile][lane]
+  __shared__ float s_cs[H][2][GP][kTileRows];  // -24 sum x
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kTileWaves;
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kTileWaves;
+  auto& s_x = s_xs[half];
+  auto& s_c = s_cs[half];
   const int r0 = blockIdx.y * kTileRows;
   const int first = blockIdx.z * a.split_steps;
   const int last = min(a.steps, first + a.split_steps);
@@ -243,8 +247,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void k_int4_tile(Int4Args a) {
   f32x4_t y[2][RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) y[0][t] = y[1][t] = f32x4_t{0, 0, 0, 0};
-  load(first);
-  for (int step = first, par = 0; step < last; ++step, par ^= 1) {
+  load(first + half);
+  // the halves take turns, and as many steps (the last one may be empty)
+  for (int step = first, par = 0; step < last; step += H, par ^= 1) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) s_x[par][i][wave][lane] = as_uint4(x[i]);
 #pragma unroll
@@ -256,7 +261,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void k_int4_tile(Int4Args a) {
       if (g == 0) s_c[par][p][16 * wave + m] = acc[0];
     }
     const Step<GP> ca = w[0], cb = w[1];
-    load(step + 1);
+    load(step + H + half);
     lds_barrier();
     const uint32_t qa[4] = {ca.w.x, ca.w.y, ca.w.z, ca.w.w};
     const uint32_t qb[4] = {cb.w.x, cb.w.y, cb.w.z, cb.w.w};
@@ -284,7 +289,21 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void k_int4_tile(Int4Args a) {
         add_scaled(y[1][t], acc[1][t], cb.s[p]);
       }
     }
-    // one barrier a step: the half written next was read before this step's barrier
+    // one barrier a step: the buffer written next was read before this step's barrier
+  }
+  if constexpr (H == 2) {
+    // the second half's sums, through its own buffers of x
+    static_assert(sizeof(s_xs[0]) == sizeof(y) * 64 * kTileWaves, "");
+    f32x4_t* part = reinterpret_cast<f32x4_t*>(&s_xs[1]) + wave * 2 * RT * 64 + lane;
+    __syncthreads();
+    if (half) {
+#pragma unroll
+      for (int t = 0; t < 2 * RT; ++t) part[64 * t] = y[t / RT][t % RT];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int t = 0; t < 2 * RT; ++t) y[t / RT][t % RT] += part[64 * t];
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -321,6 +340,7 @@ __global__ __launch_bounds__(256) void k_int4_join(Int4Args a) {
   const int64_t row = e / quads, n = 4 * (e % quads);
   const int64_t width = (int64_t)a.units * 16 * (kGate ? 2 : 1);
   f32x4_t v = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+#pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) {
     const float* p = a.part + ((int64_t)s * a.rows + row) * width + n;
     v += *reinterpret_cast<const f32x4_t*>(p);
@@ -337,6 +357,7 @@ constexpr int kCus = 256;
 
 struct Int4Plan {
   bool rows;  // k_int4_rows
+  int halves;
   int split_steps, nsplit;
   size_t bytes;
 };
@@ -348,11 +369,17 @@ Int4Plan plan_of(int rows, int K, int N, bool gate) {
   p.split_steps = steps;
   p.rows = rows <= 16;
   if (p.rows) return p;
-  // split the steps until there are about two workgroups a CU, at least 4 steps each
+  // split the steps until there are about two workgroups a CU, at least 4 steps a wave
   const int64_t groups = (int64_t)((units + (gate ? 4 : 8) - 1) / (gate ? 4 : 8)) *
                          ((rows + kTileRows - 1) / kTileRows);
-  int want = (int)((2 * kCus + groups - 1) / groups);
-  if (want > (steps + 3) / 4) want = (steps + 3) / 4;
+  // With 8 steps for every CU, one workgroup a CU whose halves share its steps: half the
+  // parts (64 rows of 12288 inputs, 4096 features: 23.0 us, 25.1 us with two workgroups),
+  // or none (64 rows of 4096, 2 x 12288: 31.2 us, 34.9 us). Fewer steps go to more
+  // workgroups (17 rows of 4096, 4096 features: 11.3 us, 12.9 us in halves).
+  p.halves = groups < kCus && groups * steps >= 8 * kCus ? 2 : 1;
+  int want = (int)(p.halves == 2 ? kCus / groups : (2 * kCus + groups - 1) / groups);
+  const int least = 4 * p.halves;
+  if (want > (steps + least - 1) / least) want = (steps + least - 1) / least;
   if (want > 1) {
     p.split_steps = (steps + want - 1) / want;
     p.nsplit = (steps + p.split_steps - 1) / p.split_steps;
@@ -393,8 +420,14 @@ int launch(const Int4Args& a, const Int4Plan& p, bool gate, hipStream_t s) {
   const int per = gate ? kTileWaves : 2 * kTileWaves;
   const dim3 grid((unsigned)((a.units + per - 1) / per),
                   (unsigned)((a.rows + kTileRows - 1) / kTileRows), (unsigned)p.nsplit);
-  if (gate) hipLaunchKernelGGL((k_int4_tile<GP, true>), grid, dim3(64 * kTileWaves), 0, s, a);
-  else hipLaunchKernelGGL((k_int4_tile<GP, false>), grid, dim3(64 * kTileWaves), 0, s, a);
+  const dim3 block(64 * kTileWaves * p.halves);
+  if (p.halves == 2) {
+    if (gate) hipLaunchKernelGGL((k_int4_tile<GP, true, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_int4_tile<GP, false, 2>), grid, block, 0, s, a);
+  } else {
+    if (gate) hipLaunchKernelGGL((k_int4_tile<GP, true, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_int4_tile<GP, false, 1>), grid, block, 0, s, a);
+  }
   if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   if (p.nsplit > 1) {
     const int64_t quads = (int64_t)a.units * 4 * a.rows;

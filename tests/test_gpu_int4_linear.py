@@ -127,3 +127,12 @@ def test_captured_calls_share_nothing(hv, cuda):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(graphs[i][1], want[i]) and torch.equal(eager[i], want[i])
+
+
+@pytest.mark.parametrize("case", [(12288, 4100, 64, 40, False), (4000, 5200, 32, 33, True),
+                                  (1056, 30000, 32, 20, False), (4096, 8208, 128, 64, True)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_linear_int4_many_steps(hv, cuda, case):
+    """Enough steps that a workgroup's two sets of waves share them: split and not, odd
+    numbers of steps."""
+    test_linear_int4(hv, cuda, case)
