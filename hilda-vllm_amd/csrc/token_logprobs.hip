@@ -13,8 +13,8 @@
 // whose maxima reach it. It finds that bar bit by bit with ballots, reads those groups
 // again (about n of them), and ranks what passes by counting. (256 rows of 151936 bf16
 // logits, top 20: 39 us with the n largest of every chunk picked in the chunk's
-// workgroup and merged, 31 us so: 21 us for the chunks, 3.7 TB/s, and 11 us for the
-// join.) Where more passes than its
+// workgroup and merged, 29.5 us so, of which the join is about 10; 512 rows of f32
+// logits, top 5: 67 us, 4.6 TB/s.) Where more passes than its
 // list holds - many equal values - the row's values are taken one by one, and -inf, what
 // a mask leaves of excluded tokens, only fills up.
 //
@@ -27,6 +27,7 @@
 
 #include "../../include/hilda_spec.h"
 #include "hs_device.h"
+#include "hs_model_dev.h"
 
 namespace hs {
 namespace {
@@ -34,6 +35,7 @@ namespace {
 constexpr int kLpT = 256;      // threads of a workgroup
 constexpr int kMaxTop = 32;
 constexpr int kListed = 1024;  // groups and values that are ranked by counting
+constexpr int kKept = 20;      // group maxima of a row that a thread of the join keeps
 constexpr int kGroup = 32;     // neighbouring logits with a maximum kept
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -68,15 +70,25 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
   return v;
 }
-// the value of another lane of the four neighbours (a DPP quad permutation)
-template <int kPerm>
-__device__ __forceinline__ float quad_xor(float v) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kPerm, 0xF, 0xF, false));
+// Over a wave, by lane swaps in the vector pipe (through LDS the three of a chunk took
+// 1.2 us of the 256-row call): with f commutative and associative but for rounding, every
+// lane gets the same result.
+template <typename F>
+__device__ __forceinline__ float over_wave(float v, F f) {
+  v = f(v, row_xor1(v));
+  v = f(v, row_xor2(v));
+  v = f(v, row_mirror8(v));
+  v = f(v, row_xor8(v));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return over_wave(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return over_wave(v, [](float a, float b) { return a + b; });
 }
 template <typename T>
 __device__ __forceinline__ float logit(const T* x, int64_t i) {
@@ -132,7 +144,7 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_chunk(LogprobArgs a) {
     for (int j = 1; j < 8; ++j) group[i] = fmaxf(group[i], v[8 * i + j]);
     most = fmaxf(most, group[i]);
   }
-  most = wave_max_f32(most);
+  most = wave_max(most);
   if (lane == 0) s_f[0][wave] = most;
   __syncthreads();
   most = fmaxf(fmaxf(s_f[0][0], s_f[0][1]), fmaxf(s_f[0][2], s_f[0][3]));
@@ -163,8 +175,8 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_chunk(LogprobArgs a) {
 #pragma unroll
     for (int i = 0; i < E / 8; ++i) {
       float g = group[i];
-      g = fmaxf(g, quad_xor<0xB1>(g));
-      g = fmaxf(g, quad_xor<0x4E>(g));
+      g = fmaxf(g, row_xor1(g));
+      g = fmaxf(g, row_xor2(g));
       if ((lane & 3) == i) mine = g;
     }
     if ((lane & 3) < E / 8)
@@ -225,10 +237,22 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.stride;
   const float c = a.temps ? kLog2e / a.temps[row] : kLog2e;
   const uint32_t* most = a.most + (int64_t)row * a.groups;
+  // the thread's share, kept for the second look at it
+  uint32_t share[kKept];
   if (a.top > 0) {
     uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < kKept; ++j) {
+      const int i = j * kLpT + (int)threadIdx.x;
+      share[j] = most[min(i, a.groups - 1)];
+    }
+#pragma unroll
+    for (int j = 0; j < kKept; ++j) {
+      if (j * kLpT + (int)threadIdx.x >= a.groups) share[j] = 0;
+      mine = max(mine, share[j]);
+    }
 #pragma unroll 8
-    for (int i = threadIdx.x; i < a.groups; i += kLpT) mine = max(mine, most[i]);
+    for (int i = kKept * kLpT + (int)threadIdx.x; i < a.groups; i += kLpT) mine = max(mine, most[i]);
     reinterpret_cast<uint32_t*>(s_most)[threadIdx.x] = mine;
     if (threadIdx.x < 4) s_n[threadIdx.x] = 0;
   }
@@ -236,7 +260,7 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
     const float4* sums = a.sums + (int64_t)row * a.chunks;
     float m = -INFINITY;
     for (int i = lane; i < a.chunks; i += 64) m = fmaxf(m, sums[i].x);
-    m = wave_max_f32(m);
+    m = wave_max(m);
     float S = 0.0f, U = 0.0f;
     for (int i = lane; i < a.chunks; i += 64) {
       const float4 s = sums[i];
@@ -278,12 +302,15 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
   // fewer than `top` threads' shares hold anything above -inf: all such values
   if (bar != bar || bar == -INFINITY) bar = -3.402823466e38f;
   const uint32_t reach = max(bits, order_key(-3.402823466e38f));
-  for (int i = threadIdx.x; i < a.groups; i += kLpT) {
-    if (most[i] >= reach) {
+  auto reached = [&](uint32_t key, int i) {
+    if (key >= reach) {
       const int at = atomicAdd(&s_n[0], 1);
       if (at < kListed) s_group[at] = i;
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kKept; ++j) reached(share[j], j * kLpT + (int)threadIdx.x);
+  for (int i = kKept * kLpT + (int)threadIdx.x; i < a.groups; i += kLpT) reached(most[i], i);
   __syncthreads();
   const int groups = s_n[0];
   for (int i = threadIdx.x / kGroup; i < min(groups, kListed); i += kLpT / kGroup) {
@@ -328,13 +355,11 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
   }
 }
 
-// values a thread: short chunks while there are few rows to fill the chip with
+// values a thread: short chunks while there are few rows to fill the chip with (16 rows of
+// 151936: 11.8 us either way; 64: 12.0 us, 13.0 us with 8; 32 values took as long as 16)
 int elems_of(int rows, int vocab) {
-  for (int e = 8; e < 32; e *= 2) {
-    const int64_t chunks = ((int64_t)vocab + e * kLpT - 1) / (e * kLpT);
-    if (rows * chunks <= 64 * e) return e;
-  }
-  return 32;
+  const int64_t chunks = ((int64_t)vocab + 8 * kLpT - 1) / (8 * kLpT);
+  return rows * chunks <= 512 ? 8 : 16;
 }
 int chunks_of(int rows, int vocab) {
   const int len = elems_of(rows, vocab) * kLpT;
@@ -403,12 +428,10 @@ int hs_token_logprobs(const void* logits, int logits_dtype, int64_t logits_row_s
   const bool aligned = !(((uintptr_t)logits | (uint64_t)(logits_row_stride * esz)) & 15);
   const int e = elems_of(rows, vocab);
   if (esz == 2) {
-    if (e == 32) launch<uint16_t, 32>(a, aligned, s);
-    else if (e == 16) launch<uint16_t, 16>(a, aligned, s);
+    if (e == 16) launch<uint16_t, 16>(a, aligned, s);
     else launch<uint16_t, 8>(a, aligned, s);
   } else {
-    if (e == 32) launch<float, 32>(a, aligned, s);
-    else if (e == 16) launch<float, 16>(a, aligned, s);
+    if (e == 16) launch<float, 16>(a, aligned, s);
     else launch<float, 8>(a, aligned, s);
   }
   if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
