@@ -26,7 +26,12 @@
 //    their results in LDS; k_scaled_combine joins the splits' partials. The partials
 //    are written before they are read and nothing is counted between the launches,
 //    so the workspace needs no preparation.
-//  * k_scaled_rows: prompts. A wave takes 16 QT query rows and all of their keys.
+//    It is bound by the cache's stream, which it reads once: 256 decodes of 64 to 2048
+//    keys of 8 heads 123 us (4.6 TB/s), 32 of 2048 to 8192 84 us (4.1), 64 verify steps of
+//    64 to 2048 keys 41.8 us (3.4, of which the join's launch is about 5).
+//  * k_scaled_rows: prompts. A wave takes 16 QT query rows and all of their keys; bound by
+//    decoding and the softmax beside the products (prompts of up to 2043 tokens behind up
+//    to 1000 keys: 175 us, 636 TFLOP/s).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -654,18 +659,21 @@ ScaledPlan plan_of(int num_seqs, int Hkv, int G, int max_q, int max_k) {
   p.bytes = 0;
   const int64_t tiles = (int64_t)num_seqs * Hkv * q;
   // Prompts take k_scaled_rows once their tiles fill half the chip's SIMDs without
-  // splitting keys (one prompt of 33 tokens, 72 tiles, behind 967 keys: 12.0 us split,
-  // 26 us not). More tiles to a wave share a window's loads and decoding as long as the
+  // splitting keys (one prompt of 33 tokens, 72 tiles, behind 967 keys: 18.9 us split,
+  // 26.7 us not). More tiles to a wave share a window's loads and decoding as long as the
   // waves still fill the chip: 509 tokens, 1024 tiles, take 17.4 / 20.9 / 25.4 us with 1 /
   // 2 / 3, 2000 tokens of 16 heads, 2000 tiles, 124 / 82 / 103 us, and 3500 of 32 heads,
   // 7100 tiles, 353 / 198 / 173 us.
   p.qt = tiles < 512 || rows <= 64 ? 0 : (tiles >= 6144 ? 3 : (tiles >= 1536 ? 2 : 1));
   if (p.qt) return p;
-  // about 1024 workgroups if every sequence is as long as declared, of at least one
-  // window a wave and at most 1024 keys unless that makes more than 8192 of them
-  int64_t len = (max_k * tiles + 1023) / 1024;
-  if (len > 1024) len = 1024;
-  const int64_t floor_len = (max_k * tiles + 8191) / 8192;
+  // about 512 workgroups if every sequence is as long as declared, of at least one window
+  // a wave and at most 512 keys unless that makes more than 4096 of them. With 1024,
+  // 1024 keys and 8192: 64 verify steps of 64 to 2048 keys 44.2 us (41.8 so), 8 of 1000 to
+  // 2000 16.4 us (14.8), 64 decodes of 2048 to 8192 153 us (150), 32 of them 85.6 us (86.0),
+  // 16 verify steps of up to 200 keys declared as 8192 9.0 us (9.8).
+  int64_t len = (max_k * tiles + 511) / 512;
+  if (len > 512) len = 512;
+  const int64_t floor_len = (max_k * tiles + 4095) / 4096;
   if (len < floor_len) len = floor_len;
   const int64_t unit = kSplitWaves * kWin;
   len = (len + unit - 1) / unit * unit;
