@@ -667,12 +667,13 @@ ScaledPlan plan_of(int num_seqs, int Hkv, int G, int max_q, int max_k) {
   p.qt = tiles < 512 || rows <= 64 ? 0 : (tiles >= 6144 ? 3 : (tiles >= 1536 ? 2 : 1));
   if (p.qt) return p;
   // about 512 workgroups if every sequence is as long as declared, of at least one window
-  // a wave and at most 512 keys unless that makes more than 4096 of them. With 1024,
-  // 1024 keys and 8192: 64 verify steps of 64 to 2048 keys 44.2 us (41.8 so), 8 of 1000 to
-  // 2000 16.4 us (14.8), 64 decodes of 2048 to 8192 153 us (150), 32 of them 85.6 us (86.0),
-  // 16 verify steps of up to 200 keys declared as 8192 9.0 us (9.8).
+  // a wave and at most 512 keys (an eighth of the longest sequence up to 1024, so that long
+  // ones leave few parts) unless that makes more than 4096 of them. 64 verify steps of 64
+  // to 2048 keys: 41.4 us, 44.2 us with 1024 keys; 32 decodes of 2048 to 8192: 84.2 us,
+  // 86.4 us with 512; one verify step of 40001 keys: 26.9 us, 28.3 us with 1024 workgroups.
   int64_t len = (max_k * tiles + 511) / 512;
-  if (len > 512) len = 512;
+  const int cap = max_k / 8 < 512 ? 512 : (max_k / 8 > 1024 ? 1024 : max_k / 8);
+  if (len > cap) len = cap;
   const int64_t floor_len = (max_k * tiles + 4095) / 4096;
   if (len < floor_len) len = floor_len;
   const int64_t unit = kSplitWaves * kWin;
