@@ -56,13 +56,21 @@ __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 8 codes -> bf16 16 + c
-__device__ __forceinline__ bf16x8_t codes8(uint32_t w) {
+// 8 codes -> bf16 16 + c: a shift and an and-or for two, with the mask in a vector and the
+// base in a scalar register (as two literals they would take an instruction more)
+struct CodeMask {
+  uint32_t mask, base;
+  __device__ __forceinline__ CodeMask() : mask(0x00780078u), base(0x41804180u) {
+    asm("" : "+v"(mask));
+    asm("" : "+s"(base));
+  }
+};
+__device__ __forceinline__ bf16x8_t codes8(uint32_t w, const CodeMask& m) {
   u32x4_t u;
-  u.x = ((w << 3) & 0x00780078u) | 0x41804180u;
-  u.y = ((w >> 1) & 0x00780078u) | 0x41804180u;
-  u.z = ((w >> 5) & 0x00780078u) | 0x41804180u;
-  u.w = ((w >> 9) & 0x00780078u) | 0x41804180u;
+  u.x = ((w << 3) & m.mask) | m.base;
+  u.y = ((w >> 1) & m.mask) | m.base;
+  u.z = ((w >> 5) & m.mask) | m.base;
+  u.w = ((w >> 9) & m.mask) | m.base;
   return __builtin_bit_cast(bf16x8_t, u);
 }
 // -24 in every element: the operand whose product with x is -24 sum x
@@ -114,13 +122,13 @@ __device__ __forceinline__ void add_scaled(f32x4_t& y, const f32x4_t& acc, uint2
 // y += the step's products. c0[p]: -24 sum x of group p (the lane's column).
 template <int GP>
 __device__ __forceinline__ void multiply(const Step<GP>& st, const bf16x8_t (&x)[4],
-                                         const float (&c0)[GP], f32x4_t& y) {
+                                         const float (&c0)[GP], const CodeMask& mask, f32x4_t& y) {
   const uint32_t w[4] = {st.w.x, st.w.y, st.w.z, st.w.w};
 #pragma unroll
   for (int p = 0; p < GP; ++p) {
     f32x4_t acc = {c0[p], c0[p], c0[p], c0[p]};
 #pragma unroll
-    for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i) acc = mfma(codes8(w[i]), x[i], acc);
+    for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i) acc = mfma(codes8(w[i], mask), x[i], acc);
     add_scaled(y, acc, st.s[p]);
   }
 }
@@ -134,6 +142,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_rows(Int4Args a) {
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u0 = blockIdx.x * kOut;
+  const CodeMask mask;
   int tile[TN];
 #pragma unroll
   for (int t = 0; t < TN; ++t) tile[t] = min(u0 + t % kOut, a.units - 1) + t / kOut * a.up;
@@ -158,7 +167,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_rows(Int4Args a) {
       c0[p] = acc[0];
     }
 #pragma unroll
-    for (int t = 0; t < TN; ++t) multiply<GP>(w[t], x, c0, y[t]);
+    for (int t = 0; t < TN; ++t) multiply<GP>(w[t], x, c0, mask, y[t]);
   }
   if (m < a.rows) {
 #pragma unroll
@@ -193,10 +202,11 @@ __device__ __forceinline__ uint4 as_uint4(u32x4_t v) { return make_uint4(v.x, v.
 // are empty and they touch no memory. Two and three steps ahead took the same time or
 // longer; what bounds it is a wave's own chain of operand reads, code shifts and products.
 // H = 2: two sets of waves, each with rows of its own in LDS, take the steps in turn and
-// join their sums in LDS. 64 rows of 12288 inputs, 4096 features: 23.0 us (280 TFLOP/s, 5
-// of them the join's launch); 600 rows of 4096 inputs, 2 x 12288 features: 170 us (711 TFLOP/s).
+// join their sums in LDS. 64 rows of 12288 inputs, 4096 features: 21.0 us (307 TFLOP/s), 4
+// of them the join's launch; 600 rows of 4096 inputs, 2 x 12288 features: 167 us (723 TFLOP/s).
 template <int GP, bool kGate, int H>
-__global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2) void k_int4_tile(Int4Args a) {
+__global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2)
+void k_int4_tile(Int4Args a) {
   constexpr int RT = kTileRows / 16;
   __shared__ uint4 s_xs[H][2][4][RT][64];      // [half][step parity][i][row tile][lane]
   __shared__ float s_cs[H][2][GP][kTileRows];  // -24 sum x
@@ -213,6 +223,7 @@ __global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2) void
   const int ua = min(u0, a.units - 1);
   const int ub = kGate ? ua + a.up : min(u0 + 1, a.units - 1);
 
+  const CodeMask mask;
   static_assert(RT == kTileWaves, "a wave stages one row tile");
   u32x4_t x[4];
   Step<GP> w[2];
@@ -234,8 +245,8 @@ __global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2) void
       const int64_t tile = (t ? wb0 : wa0) + at;
       const auto wb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint4*>(a.w + tile * 64), 0,
                                                         live ? 1024 : 0, 0x00027000);
-      const auto sb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.sc + tile * GP * 16), 0,
-                                                        live ? 32 * GP : 0, 0x00027000);
+      const auto sb = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint16_t*>(a.sc + tile * GP * 16), 0, live ? 32 * GP : 0, 0x00027000);
       w[t].w = as_uint4(__builtin_amdgcn_raw_buffer_load_b128(wb, 16 * lane, 0, 0));
 #pragma unroll
       for (int p = 0; p < GP; ++p) {
@@ -275,7 +286,7 @@ __global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2) void
       }
 #pragma unroll
       for (int i = p * 4 / GP; i < (p + 1) * 4 / GP; ++i) {
-        const bf16x8_t fa = codes8(qa[i]), fb = codes8(qb[i]);
+        const bf16x8_t fa = codes8(qa[i], mask), fb = codes8(qb[i], mask);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           const bf16x8_t b = __builtin_bit_cast(bf16x8_t, s_x[par][i][t][lane]);
@@ -373,9 +384,9 @@ Int4Plan plan_of(int rows, int K, int N, bool gate) {
   const int64_t groups = (int64_t)((units + (gate ? 4 : 8) - 1) / (gate ? 4 : 8)) *
                          ((rows + kTileRows - 1) / kTileRows);
   // With 8 steps for every CU, one workgroup a CU whose halves share its steps: half the
-  // parts (64 rows of 12288 inputs, 4096 features: 23.0 us, 25.1 us with two workgroups),
-  // or none (64 rows of 4096, 2 x 12288: 31.2 us, 34.9 us). Fewer steps go to more
-  // workgroups (17 rows of 4096, 4096 features: 11.3 us, 12.9 us in halves).
+  // parts (64 rows of 12288 inputs, 4096 features: 21.0 us, 23.0 us with two workgroups),
+  // or none (64 rows of 4096, 2 x 12288: 30.5 us, 33.9 us). Fewer steps go to more
+  // workgroups (17 rows of 4096, 4096 features: 11.1 us, 12.9 us in halves).
   p.halves = groups < kCus && groups * steps >= 8 * kCus ? 2 : 1;
   int want = (int)(p.halves == 2 ? kCus / groups : (2 * kCus + groups - 1) / groups);
   const int least = 4 * p.halves;
@@ -398,10 +409,10 @@ void launch_rows(const Int4Args& a, hipStream_t s) {
 
 // Many tiles: workgroups of 4 waves, several of which fit a CU and hide each other's
 // beginning and end, and of several tiles, which share the rows' loads (151936 features, 4
-// rows: 93 us with 8 waves and 2 tiles, 75 us with 4 and 2, 66 us with 4 and 4: 4.9 TB/s).
+// rows: 67 us with 8 waves and 2 tiles, 71 us with 4 and 2, 60 us with 4 and 4: 5.4 TB/s).
 // Few: 8 waves to one tile, so that each CU has its tile's steps in flight at once (4096 by
-// 4096, 4 rows: 6.4 us, 7.5 us with 4), more where there are many steps (12288 inputs, 8
-// rows: 13.2 us with 12, 15.4 us with 8).
+// 4096, 4 rows: 7.4 us, 9.8 us with 4), more where there are many steps (12288 inputs, 8
+// rows: 12.4 us with 12, 14.3 us with 8).
 template <int GP>
 void dispatch_rows(const Int4Args& a, bool gate, hipStream_t s) {
   if (gate) launch_rows<GP, 4, 2, true>(a, s);
