@@ -70,17 +70,18 @@ def _mode(mode) -> int:
 
 
 def _need_cuda(*ts):
-    dev = None
+    first, index = None, -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()  # -1: not on a GPU
+        if i < 0:
             raise ValueError("all tensors must live on the GPU")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if first is None:
+            first, index = t, i
+        elif i != index:
             raise ValueError("all tensors must live on the same GPU")
-    return dev
+    return None if first is None else first.device
 
 
 def _rows2d(t: torch.Tensor, rows: int, V: int) -> tuple[torch.Tensor, int]:
