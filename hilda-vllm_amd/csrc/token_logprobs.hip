@@ -2,8 +2,7 @@
 // Of a row y = logits / T with maximum m, S = sum exp(y - m), U = sum (y - m) exp(y - m):
 //   log p(t) = (y_t - m) - ln S        entropy = ln S - U / S
 // and the `top` largest logits in order, the lower index first among equal ones.
-// Exponents are powers of two: (x - max x) log2(e) / T, whose difference is rounded but
-// cannot overflow where its terms do not.
+// Exponents are powers of two: (x - max x) log2(e) / T.
 // k_logprobs_chunk reads the logits, which bound it, once: a workgroup takes a chunk of
 // a row into registers and leaves its maximum, its two sums and the maximum of every 32
 // neighbouring logits. k_logprobs_join, a workgroup a row, adds up the chunks (sums
@@ -13,8 +12,8 @@
 // whose maxima reach it. It finds that bar bit by bit with ballots, reads those groups
 // again (about n of them), and ranks what passes by counting. (256 rows of 151936 bf16
 // logits, top 20: 39 us with the n largest of every chunk picked in the chunk's
-// workgroup and merged, 29.5 us so, of which the join is about 10; 512 rows of f32
-// logits, top 5: 67 us, 4.6 TB/s.) Where more passes than its
+// workgroup and merged, 28 us so, of which the join is about 9; 512 rows of f32
+// logits, top 5: 67 us, 4.7 TB/s.) Where more passes than its
 // list holds - many equal values - the row's values are taken one by one, and -inf, what
 // a mask leaves of excluded tokens, only fills up.
 //
@@ -101,6 +100,13 @@ __device__ __forceinline__ int elem_of(int e) {
   return 8 * ((e >> 3) * kLpT + (int)threadIdx.x) + (e & 7);
 }
 
+// The largest of three, in one instruction: fmaxf would quiet every operand before it.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // E values a thread: a chunk is E * kLpT elements.
 template <typename T, int E, bool kAligned>
 __global__ __launch_bounds__(kLpT) void k_logprobs_chunk(LogprobArgs a) {
@@ -134,14 +140,13 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_chunk(LogprobArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = elem_of(e) < len ? v[e] : -INFINITY;
   }
-  // the largest values of the thread's groups of 8 (fmaxf leaves NaN out: a NaN makes
-  // the sums NaN)
+  // the largest values of the thread's groups of 8 (of a NaN, a number or NaN: the sums
+  // are NaN then, and the group is marked below)
   float group[E / 8], most = -INFINITY;
 #pragma unroll
   for (int i = 0; i < E / 8; ++i) {
-    group[i] = v[8 * i];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) group[i] = fmaxf(group[i], v[8 * i + j]);
+    const float* e = v + 8 * i;
+    group[i] = max3(max3(e[0], e[1], e[2]), max3(e[3], e[4], e[5]), max3(e[6], e[6], e[7]));
     most = fmaxf(most, group[i]);
   }
   most = wave_max(most);
@@ -151,13 +156,19 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_chunk(LogprobArgs a) {
   const float c = a.temps ? kLog2e / a.temps[row] : kLog2e;
   const float ref = most == -INFINITY ? 0.0f : most;
   float S = 0.0f, U = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float d = (v[e] - ref) * c;
+  auto add = [&](float d) {
     const float p = __builtin_amdgcn_exp2f(d);
     S += p;
     // far below, where p is 0, d may be -inf: it takes no part
     U = fmaf(p, fmaxf(d, -512.0f), U);
+  };
+  const float rc = ref * c;
+  if (fabsf(rc) < 128.0f) {  // v c - ref c in one step: rounding ref c moves it by 2^-18 at most
+#pragma unroll
+    for (int e = 0; e < E; ++e) add(fmaf(v[e], c, -rc));
+  } else {  // the difference first, which is exact where it counts and cannot overflow
+#pragma unroll
+    for (int e = 0; e < E; ++e) add((v[e] - ref) * c);
   }
   if (!(S < INFINITY)) {
     // a NaN among the thread's values, perhaps: its groups, and no others, count as
