@@ -455,9 +455,9 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 def _call(dev: torch.device, what: str, *args) -> None:
     """Entry point `what` on the current stream of `dev`, which need not be the
     current device."""
-    fn = getattr(L.lib(), what)
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, _stream(dev))
+    fn, index = getattr(L.lib(), what), dev.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
             status = fn(*args, _stream(dev))
