@@ -336,3 +336,19 @@ def test_store_at_the_ends_of_the_range(hv, cuda):
     ref.store(v.double().numpy(), want[1], want[3], slots)
     for got, w in zip((dk, dv, dks, dvs), want):
         assert np.array_equal(got.double().cpu().numpy(), w, equal_nan=True)
+
+
+_FEW_SPLITS = [
+    ("few-longer-than-declared", 16, 8, 64, 32, [2, 1], [1500, 90], 600),
+    ("few-group-5", 10, 2, 160, 32, [4, 7], [77, 900], 900),
+    ("few-no-queries", 32, 8, 256, 64, [0, 2, 0, 1], [40, 1024, 0, 33], 1024),
+    ("one-split-at-its-limit", 32, 8, 256, 32, [4, 3], [512, 511], 512),
+    ("one-split-of-1024", 32, 8, 256, 32, [1] * 16, [1024 - 61 * i for i in range(16)], 1024),
+    ("many-of-1025", 32, 8, 256, 32, [1] * 16, [1025 - 61 * i for i in range(16)], 1025),
+]
+
+
+@pytest.mark.parametrize("case", _FEW_SPLITS, ids=[c[0] for c in _FEW_SPLITS])
+def test_attention_with_few_splits(hv, cuda, case):
+    """Where a call leaves its keys whole, and where two to nine workgroups share them."""
+    test_attention(hv, cuda, case)
