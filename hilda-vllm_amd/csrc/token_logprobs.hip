@@ -277,8 +277,11 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
       const float4 s = sums[i];
       // sums under the chunk's maximum, moved to the row's
       const float d = (s.x - m) * c, f = __builtin_amdgcn_exp2f(d);
-      S += f == 0.0f ? 0.0f : f * s.y;
-      U += f == 0.0f ? 0.0f : f * (s.z + d * s.y);
+      // far below, where f is 0 and d may be -inf, a chunk's numbers take no part; a NaN,
+      // which the chunk's maximum does not show, always does
+      const bool none = f == 0.0f && s.y == s.y;
+      S += none ? 0.0f : f * s.y;
+      U += none ? 0.0f : f * (s.z + d * s.y);
     }
     S = wave_sum(S);
     U = wave_sum(U);
