@@ -361,7 +361,8 @@ __global__ __launch_bounds__(kLpT) void k_logprobs_join(LogprobArgs a) {
   }
   __syncthreads();  // the ids, written by this workgroup
   if (threadIdx.x < a.top) {
-    const int64_t id = ids[threadIdx.x];
+    // every place was written above; an index that comes from memory is bounded all the same
+    const int64_t id = min(max(ids[threadIdx.x], (int64_t)0), (int64_t)a.vocab - 1);
     a.top_logprobs[(int64_t)row * a.top + threadIdx.x] =
         ((logit<T>(x, id) - s_f[0]) * c - s_f[1]) * kLn2;
   }
