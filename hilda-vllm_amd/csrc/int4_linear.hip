@@ -6,14 +6,16 @@
 // lane l holds the codes of feature l % 16, inputs 32 i + 8 (l / 16) .. + 7, so a
 // wave loads a step with one 16-byte load a lane, contiguous over the tile, and
 // each dword is one lane's share of a 16x16x32 MFMA A operand. The codes are not
-// converted: shifted into the top four mantissa bits of a bf16 16.0 they read 16 + c
-// (one shift and one and-or for two of them), and
-//   sum x (c - 8) = sum x (16 + c) - 24 sum x,
+// converted: shifted into the top four mantissa bits of a bf16 2^-8 they read
+// (16 + c) 2^-12 (one shift and one and-or for two of them), and
+//   sum x (c - 8) = 2^12 (sum x (16 + c) 2^-12 - sum x 24 2^-12),
 // whose last sum is the same for every feature and enters as the accumulator's
 // start. A group's products end in an accumulator of their own that its scales
-// then multiply: nothing is rounded below f32 before the output. (The offset costs
-// the sums a factor of about 24 / 4.6, the size of 16 + c over that of c - 8, in
-// f32's last bits; an infinity in x gives NaN.)
+// then multiply; 2^12 multiplies the output's sum: nothing is rounded below f32 before
+// the output. (The offset costs the sums a factor of about 24 / 4.6, the size of 16 + c
+// over that of c - 8, in f32's last bits. 2^-12, because the partial sums of a group then
+// stay finite whatever finite x are: 128 products of at most 31 2^-12 |x|. An infinity in
+// x gives NaN.)
 //
 // k_int4_rows (up to 16 rows): bound by the weights' stream. A workgroup's waves share
 // out the steps of its one to four tiles and join their sums in LDS. The rows come from
@@ -56,11 +58,13 @@ __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 8 codes -> bf16 16 + c: a shift and an and-or for two, with the mask in a vector and the
+constexpr float kUnit = 4096.0f;  // the sums are kept in units of 2^12
+
+// 8 codes -> bf16 (16 + c) 2^-12: a shift and an and-or for two, with the mask in a vector and the
 // base in a scalar register (as two literals they would take an instruction more)
 struct CodeMask {
   uint32_t mask, base;
-  __device__ __forceinline__ CodeMask() : mask(0x00780078u), base(0x41804180u) {
+  __device__ __forceinline__ CodeMask() : mask(0x00780078u), base(0x3b803b80u) {
     asm("" : "+v"(mask));
     asm("" : "+s"(base));
   }
@@ -73,9 +77,9 @@ __device__ __forceinline__ bf16x8_t codes8(uint32_t w, const CodeMask& m) {
   u.w = ((w >> 9) & m.mask) | m.base;
   return __builtin_bit_cast(bf16x8_t, u);
 }
-// -24 in every element: the operand whose product with x is -24 sum x
+// -24 2^-12 in every element: the operand whose product with x is the accumulator's start
 __device__ __forceinline__ bf16x8_t minus24() {
-  const u32x4_t u = {0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};
+  const u32x4_t u = {0xbbc0bbc0u, 0xbbc0bbc0u, 0xbbc0bbc0u, 0xbbc0bbc0u};
   return __builtin_bit_cast(bf16x8_t, u);
 }
 
@@ -94,6 +98,12 @@ __device__ __forceinline__ bf16x8_t load_x(const Int4Args& a, int row, int step,
 }
 
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
+
+// the output of sums in units of 2^12
+template <bool kGate>
+__device__ __forceinline__ uint16_t result(float v, float up) {
+  return to_bf(kGate ? silu(v * kUnit) * (up * kUnit) : v * kUnit);
+}
 
 // a lane's share of one step of one tile: its codes, and the scales of features
 // 4 g .. 4 g + 3 in the step's GP groups
@@ -119,7 +129,7 @@ __device__ __forceinline__ void add_scaled(f32x4_t& y, const f32x4_t& acc, uint2
   y[3] += acc[3] * __uint_as_float(s.y & 0xffff0000u);
 }
 
-// y += the step's products. c0[p]: -24 sum x of group p (the lane's column).
+// y += the step's products. c0[p]: -24 2^-12 sum x of group p (the lane's column).
 template <int GP>
 __device__ __forceinline__ void multiply(const Step<GP>& st, const bf16x8_t (&x)[4],
                                          const float (&c0)[GP], const CodeMask& mask, f32x4_t& y) {
@@ -183,7 +193,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_rows(Int4Args a) {
       if (kGate) up += s_part[w][kOut + t][row][n];
     }
     const int col = (u0 + t) * 16 + n;
-    if (col < a.N) a.y[(int64_t)row * a.ys + col] = to_bf(kGate ? silu(v) * up : v);
+    if (col < a.N) a.y[(int64_t)row * a.ys + col] = result<kGate>(v, up);
   }
 }
 
@@ -209,7 +219,7 @@ __global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2)
 void k_int4_tile(Int4Args a) {
   constexpr int RT = kTileRows / 16;
   __shared__ uint4 s_xs[H][2][4][RT][64];      // [half][step parity][i][row tile][lane]
-  __shared__ float s_cs[H][2][GP][kTileRows];  // -24 sum x
+  __shared__ float s_cs[H][2][GP][kTileRows];  // -24 2^-12 sum x
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kTileWaves;
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kTileWaves;
@@ -335,8 +345,7 @@ void k_int4_tile(Int4Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int n = tile * 16 + 4 * g + j;
-        const float r = kGate ? silu(y[0][t][j]) * y[1][t][j] : y[h][t][j];
-        if (n < a.N) a.y[(int64_t)row * a.ys + n] = to_bf(r);
+        if (n < a.N) a.y[(int64_t)row * a.ys + n] = result<kGate>(y[h][t][j], y[1][t][j]);
       }
     }
   }
@@ -359,8 +368,7 @@ __global__ __launch_bounds__(256) void k_int4_join(Int4Args a) {
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float r = kGate ? silu(v[j]) * u[j] : v[j];
-    if (n + j < a.N) a.y[row * a.ys + n + j] = to_bf(r);
+    if (n + j < a.N) a.y[row * a.ys + n + j] = result<kGate>(v[j], u[j]);
   }
 }
 
