@@ -59,17 +59,29 @@ def add_rms_norm(x, residual, w, eps):
     return xf.to(x.dtype) * w, res
 
 
+class Int4Projection(nn.Module):
+    """An ops.Int4Weight as a part of a model: its codes and scales are parameters, so
+    parameters(), state_dict() and .to() include them. It has the weight's fields and
+    stands for it in ops.linear_int4."""
+
+    def __init__(self, w: _ops.Int4Weight):
+        super().__init__()
+        self.packed = nn.Parameter(w.packed, requires_grad=False)
+        self.scales = nn.Parameter(w.scales, requires_grad=False)
+        self.out_features, self.in_features, self.group = w.out_features, w.in_features, w.group
+
+
 def _norm_proj(x, norm, eps, w, residual=None, swiglu=False):
     """ops.linear_rmsnorm, or with a 4-bit weight the RMSNorm kernel and its projection
     (the residual is then updated in place)."""
-    if isinstance(w, _ops.Int4Weight):
+    if isinstance(w, Int4Projection):
         xn = _ops.rmsnorm(x, norm, eps, residual=residual)
         return _ops.linear_int4(xn, w, swiglu=swiglu), (x if residual is None else residual)
     return _ops.linear_rmsnorm(x, norm, eps, w, residual=residual, swiglu=swiglu)
 
 
 def _proj(x, w):
-    return _ops.linear_int4(x, w) if isinstance(w, _ops.Int4Weight) else _ops.linear(x, w)
+    return _ops.linear_int4(x, w) if isinstance(w, Int4Projection) else _ops.linear(x, w)
 
 
 class Rope(nn.Module):
@@ -155,14 +167,16 @@ class Qwen3Layer(nn.Module):
         """The four projections to 4-bit weights (ops.quantize_int4)."""
         for name in ("qkv", "o", "gate_up", "down"):
             w = getattr(self, name)
-            if not isinstance(w, _ops.Int4Weight):
-                q = _ops.quantize_int4(w, group)
+            if not isinstance(w, Int4Projection):
+                q = Int4Projection(_ops.quantize_int4(w, group))
                 delattr(self, name)
                 setattr(self, name, q)
 
     def forward_reference(self, positions, h, residual):
         """Eager PyTorch restatement of the same layer (used by tests; bf16 weights)."""
         g = self.g
+        if any(isinstance(w, Int4Projection) for w in (self.qkv, self.o, self.gate_up, self.down)):
+            raise TypeError("the restatement takes bf16 weights; this layer's are in 4 bits")
         if residual is None:
             x, residual = rms_norm(h, self.ln1, g.rms_eps), h
         else:
@@ -228,8 +242,8 @@ class Qwen3Host(nn.Module):
         A model that shares this one's weights keeps those it was built with."""
         for layer in self.layers:
             layer.quantize_int4(group)
-        if lm_head and not isinstance(self.lm_head, _ops.Int4Weight):
-            q = _ops.quantize_int4(self.lm_head, group)
+        if lm_head and not isinstance(self.lm_head, Int4Projection):
+            q = Int4Projection(_ops.quantize_int4(self.lm_head, group))
             del self.lm_head
             self.lm_head = q
         return self
