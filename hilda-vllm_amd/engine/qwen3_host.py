@@ -164,13 +164,14 @@ class Qwen3Layer(nn.Module):
         return h, residual
 
     def quantize_int4(self, group: int = 128):
-        """The four projections to 4-bit weights (ops.quantize_int4)."""
-        for name in ("qkv", "o", "gate_up", "down"):
-            w = getattr(self, name)
-            if not isinstance(w, Int4Projection):
-                q = Int4Projection(_ops.quantize_int4(w, group))
-                delattr(self, name)
-                setattr(self, name, q)
+        """The four projections to 4-bit weights (ops.quantize_int4): all of them, or none
+        where one refuses the group."""
+        new = {name: Int4Projection(_ops.quantize_int4(w, group))
+               for name in ("qkv", "o", "gate_up", "down")
+               if not isinstance(w := getattr(self, name), Int4Projection)}
+        for name, q in new.items():
+            delattr(self, name)
+            setattr(self, name, q)
 
     def forward_reference(self, positions, h, residual):
         """Eager PyTorch restatement of the same layer (used by tests; bf16 weights)."""

@@ -6,9 +6,9 @@ import pytest
 import torch
 
 
-def _layer(seed):
+def _layer(seed, ffn=384):
     q3 = importlib.import_module("hilda-vllm_amd.engine.qwen3_host")
-    g = q3.Qwen3Geometry(num_layers=1, hidden=256, num_heads=2, num_kv_heads=1, ffn=384, vocab=64,
+    g = q3.Qwen3Geometry(num_layers=1, hidden=256, num_heads=2, num_kv_heads=1, ffn=ffn, vocab=64,
                          max_position=64)
     torch.manual_seed(seed)
     return q3.Qwen3Layer(g, "cpu", torch.bfloat16, q3.Rope(128, 64, 1e6, "cpu"))
@@ -68,3 +68,16 @@ def test_the_restatement_refuses_4_bit_weights():
     with pytest.raises(TypeError):
         a.forward_reference(torch.zeros(1, dtype=torch.int64),
                             torch.zeros(1, 256, dtype=torch.bfloat16), None)
+
+
+def test_a_refused_group_changes_nothing():
+    """Inputs of the down projection that the group does not divide: the other three stay
+    as they are too."""
+    a = _layer(6, ffn=192)
+    before = dict(a.named_parameters())
+    with pytest.raises(ValueError):
+        a.quantize_int4(128)
+    after = dict(a.named_parameters())
+    assert set(before) == set(after) and all(before[n] is after[n] for n in before)
+    a.quantize_int4(64)
+    assert a.down.in_features == 192
