@@ -345,6 +345,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     tlp = logits.new_empty((rows, top), dtype=f32) if top else None
     if rows:
         lg, lstride = _rows2d(logits, rows, V)
+        if lstride < V:  # broadcast rows, or the stride of a single one
+            lg, lstride = lg if rows == 1 else lg.contiguous(), V
         nbytes = L.lib().hs_token_logprobs_workspace_size(rows, V, top)
         ws = logits.new_empty(nbytes, dtype=torch.uint8)
 
@@ -550,7 +552,8 @@ def verify_attention_scaled(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
     if bt.dim() != 2 or bt.shape[0] < B:
         raise ValueError("block_tables must be [sequences, blocks]")
-    if bt.stride(1) != 1:
+    W = bt.shape[1]
+    if bt.stride(1) != 1 or bt.stride(0) < W:  # also broadcast rows
         bt = bt.contiguous()
     if out is None:
         out = q.new_empty((N, Hq, D))
@@ -564,7 +567,7 @@ def verify_attention_scaled(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     ost = out.stride()
     _call(dev, "hs_verify_attention_scaled", q.data_ptr(), qst[0], qst[1], k_cache.data_ptr(),
           v_cache.data_ptr(), cst[0], cst[1], cst[2], k_scales.data_ptr(), v_scales.data_ptr(),
-          sst[0], sst[1], sst[2], group, bt.data_ptr(), bt.stride(0), bt.shape[1], nb,
+          sst[0], sst[1], sst[2], group, bt.data_ptr(), max(bt.stride(0), W), W, nb,
           cq.data_ptr(), ck.data_ptr(), B, mq, mk, Hq, Hkv, D, bs, float(softmax_scale),
           out.data_ptr(), ost[0], ost[1], ws.data_ptr() if nbytes else None, nbytes)
     return out
