@@ -7,9 +7,15 @@
 // Codes are decoded exactly to bf16 (every e4m3 value is one) and multiplied on
 // the matrix cores with f32 accumulation; a window of 32 keys lies in one group,
 // so its scales are two scalars: ks joins the softmax scale, and the power of two in vs
-// the decoding of V (what a scale of another producer has besides multiplies the
-// probabilities). The probabilities round to bf16 as the product's second operand;
-// statistics, sums and partial results are f32.
+// the decoding of V (what a scale of another producer has besides is the unit that the
+// outputs are kept in). Statistics, sums and partial results are f32. The probabilities are
+// the product's second operand: in two bf16 parts (16 bits and more) for decode and verify
+// rows and prompts of one tile a wave, where the second product is hidden by the loads (64
+// verify steps 41.9 us, 41.6 us in one part; 32 decodes 85.7 and 85.4; one prompt of 509
+// tokens 18.1 and 17.5). Longer prompts are bound by the vector and matrix pipes and round
+// them to bf16 once (the listed prompts 175 us, 225 us in two parts): their error against
+// 64-bit sums is 1.85e-3 of the outputs' size, root mean square, where the output's own
+// rounding is 1.66e-3. The sum below takes the same rounded ones.
 //
 // A wave works on its own, without LDS in its loop. It takes a window's K rows as
 // the A operand of S^T = K Q^T (lane l: key l % 16, dims 32 (l / 16) .. + 31, two
@@ -213,19 +219,50 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
 
 // The state of 16 QT query rows: per tile the lane's row (l % 16) has its maximum
 // (log2 domain), its sum (in every element of l) and O[d = 32 (l / 16) + 8 j + db] in
-// o[db][j].
+// o[db][j], in units of `unit`.
 template <int QT>
 struct Rows {
   bf16x8_t q[QT][4];
   int lim[QT];  // keys that the row sees
-  float m[QT];
+  float m[QT], unit;
   f32x4_t l[QT], o[QT][8];
 };
+
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+
+// A window's v scale: the power of two in |vs|, which V's decoding takes for nothing, times
+// the outputs' unit, 1 or what else a scale of another producer has (so that no probability
+// is rounded again), times `rest`, which multiplies the probabilities. That is 1 but for
+// scales that are zero, subnormal or not finite.
+struct Split {
+  float scale, unit, rest;
+};
+__device__ __forceinline__ Split split_of(float vs, float unit) {
+  const uint32_t bits = __float_as_uint(vs), size = bits & 0x7fffffffu;
+  if (size >= 0x00800000u && size < 0x7f800000u)
+    return {__uint_as_float(size), __uint_as_float((bits & 0x807fffffu) | 0x3f800000u), 1.0f};
+  if (size && size < 0x00800000u) return {0x1p-100f, unit, uniform(vs * 0x1p100f / unit)};
+  return {1.0f, unit, uniform(vs / unit)};
+}
+
+template <int QT>
+__device__ __forceinline__ void to_unit(float unit, Rows<QT>& R) {
+  const float ratio = uniform(R.unit / unit);
+#pragma unroll
+  for (int u = 0; u < QT; ++u)
+#pragma unroll
+    for (int db = 0; db < 8; ++db) R.o[u][db] *= ratio;
+  R.unit = unit;
+}
 
 template <int QT>
 __device__ __forceinline__ void load_rows(const ScaledAttnArgs& a, const Seq& s, int head, int r0,
                                           int lane, Rows<QT>& R) {
   const int n = lane & 15, g = lane >> 4;
+  R.unit = 1.0f;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = r0 + 16 * t + n;
@@ -265,18 +302,48 @@ __device__ __forceinline__ void scores(const Win& w, const Rows<QT>& R, f32x4_t 
   }
 }
 
-// The softmax step of the scores (times c), and the probabilities times `rest` as P^T.
-// kMask: some row may not see some key. A key that a row does not see takes no part in
-// that row, whatever its codes and scales are: its probability is 0. Bit e of seen[u]:
-// the row sees the lane's e-th key. The sum adds the probabilities as they are
-// multiplied, rounded to bf16, on the matrix cores (a row of ones), so that the weights
-// of an output add up to one.
+// P^T as the product's operand: one bf16 part, or two whose sum is the probability
+template <bool kTwo>
+struct Probs {
+  bf16x8_t part[kTwo ? 2 : 1];
+};
+template <bool kTwo>
+__device__ __forceinline__ Probs<kTwo> probs_of(const float (&y)[8]) {
+  Probs<kTwo> p;
+  Frag f, rest;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    f.u[e >> 1] = pk_bf16(y[e], y[e + 1]);
+    if constexpr (kTwo)
+      rest.u[e >> 1] = pk_bf16(y[e] - __uint_as_float(f.u[e >> 1] << 16),
+                               y[e + 1] - __uint_as_float(f.u[e >> 1] & 0xffff0000u));
+  }
+  p.part[0] = f.v;
+  if constexpr (kTwo) p.part[1] = rest.v;
+  return p;
+}
+// c += a P^T
+template <bool kTwo>
+__device__ __forceinline__ f32x4_t times(bf16x8_t a, const Probs<kTwo>& p, f32x4_t c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p.part[0], c, 0, 0, 0);
+  if constexpr (kTwo) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p.part[1], c, 0, 0, 0);
+  return c;
+}
+template <int QT>
+using WindowProbs = Probs<QT == 1>;
+
+// The softmax step of the scores (times c), and the probabilities as P^T. kMask: some row may
+// not see some key. A key that a row does not see takes no part in that row, whatever its
+// codes and scales are: its probability is 0. Bit e of seen[u]: the row sees the lane's e-th
+// key. The sum adds the probabilities as they are multiplied, in their bf16 parts, on the
+// matrix cores (a row of ones), so that the weights of an output add up to one.
 template <int QT, bool kMask>
-__device__ __forceinline__ void weigh(const f32x4_t (&s)[QT][2], float c, float rest, int ws,
-                                      int rows, int g, Rows<QT>& R, bf16x8_t (&p)[QT],
+__device__ __forceinline__ void weigh(const f32x4_t (&s)[QT][2], float c, int ws,
+                                      int rows, int g, Rows<QT>& R, WindowProbs<QT> (&p)[QT],
                                       uint32_t (&seen)[QT]) {
-  Frag ones;
-  ones.u[0] = ones.u[1] = ones.u[2] = ones.u[3] = 0x3f803f80u;
+  Frag one;
+  one.u[0] = one.u[1] = one.u[2] = one.u[3] = 0x3f803f80u;
+  const bf16x8_t ones = one.v;
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
     seen[u] = 0xff;
@@ -306,33 +373,42 @@ __device__ __forceinline__ void weigh(const f32x4_t (&s)[QT][2], float c, float 
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(y[e] - ref);
-    Frag f;
+    p[u] = probs_of<QT == 1>(y);
+    R.l[u] = times(ones, p[u], R.l[u]);
+  }
+}
+
+// the probabilities times `rest`, where the rows see the keys
+template <int QT>
+__device__ __forceinline__ void multiply(float rest, const uint32_t (&seen)[QT],
+                                         WindowProbs<QT> (&p)[QT]) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) f.u[e >> 1] = pk_bf16(y[e], y[e + 1]);
-    R.l[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, f.v, R.l[u], 0, 0, 0);
-    if (rest != 1.0f) {  // scales of another producer that are no powers of two
+  for (int u = 0; u < QT; ++u) {
+#pragma unroll
+    for (int h = 0; h < (int)(sizeof(p[u].part) / sizeof(bf16x8_t)); ++h) {
+      // a second part is all of nothing where the product is not finite
+      const bool none = h && !(fabsf(rest) < INFINITY);
+      Frag f;
+      f.v = p[u].part[h];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        float z[2] = {y[e] * rest, y[e + 1] * rest};
-        if constexpr (kMask) {
-          if (!((seen[u] >> e) & 1u)) z[0] = 0.0f;
-          if (!((seen[u] >> (e + 1)) & 1u)) z[1] = 0.0f;
-        }
-        f.u[e >> 1] = pk_bf16(z[0], z[1]);
+        const float a = __uint_as_float(f.u[e >> 1] << 16) * rest;
+        const float b = __uint_as_float(f.u[e >> 1] & 0xffff0000u) * rest;
+        f.u[e >> 1] = pk_bf16((seen[u] >> e) & 1u && !none ? a : 0.0f,
+                              (seen[u] >> (e + 1)) & 1u && !none ? b : 0.0f);
       }
+      p[u].part[h] = f.v;
     }
-    p[u] = f.v;
   }
 }
 
 // O^T += V^T P^T
 template <int QT>
-__device__ __forceinline__ void gather(const Win& w, float scale, const bf16x8_t (&p)[QT],
+__device__ __forceinline__ void gather(const Win& w, float scale, const WindowProbs<QT> (&p)[QT],
                                        Rows<QT>& R) {
   transposed(w.v, scale, [&](int db, bf16x8_t va) {
 #pragma unroll
-    for (int u = 0; u < QT; ++u)
-      R.o[u][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[u], R.o[u][db], 0, 0, 0);
+    for (int u = 0; u < QT; ++u) R.o[u][db] = times(va, p[u], R.o[u][db]);
   });
 }
 
@@ -412,24 +488,23 @@ __device__ __forceinline__ void window(const ScaledAttnArgs& a, const Batch& t, 
   const Source next = source(a, t, head, i + 1);
   const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.ks), i));
   const float vs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t.vs), i));
-  // vs as a power of two, which V's decoding takes for nothing, and what is left of it
-  // (all of it where it is zero, negative, subnormal or not finite)
-  const uint32_t bits = __float_as_uint(vs);
-  const bool plain = bits >= 0x00800000u && bits < 0x7f800000u;
-  const float scale = plain ? vs : 1.0f;
-  const float rest = plain ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : vs;
+  // The two steps for scales of another producer stand outside the tiles' loop, where a branch
+  // would keep the tiles' steps from overlapping (the listed prompts: 201 us so).
+  const Split v = split_of(vs, R.unit);
+  if (__float_as_uint(v.unit) != __float_as_uint(R.unit)) to_unit<QT>(v.unit, R);
   f32x4_t s[QT][2];
   scores<QT>(w, R, s);
   load_k(a, next, at_k, w);  // in flight during the rest of this window
-  bf16x8_t p[QT];
+  WindowProbs<QT> p[QT];
   uint32_t seen[QT];
   const int rows = __builtin_amdgcn_readlane(t.blk, i) < 0 ? 0 : kWin;
-  weigh<QT, kMask>(s, a.scale_log2 * ks, rest, ws, rows, lane >> 4, R, p, seen);
+  weigh<QT, kMask>(s, a.scale_log2 * ks, ws, rows, lane >> 4, R, p, seen);
+  if (__float_as_uint(v.rest) != __float_as_uint(1.0f)) multiply<QT>(v.rest, seen, p);
   if constexpr (!kMask) {
-    gather<QT>(w, scale, p, R);
+    gather<QT>(w, v.scale, p, R);
   } else {
     const bool bad = drop_nan(w);
-    gather<QT>(w, scale, p, R);
+    gather<QT>(w, v.scale, p, R);
     if (bad) {
       load_v(a, source(a, t, head, i), at_v, w);
       spread_nan<QT>(w, seen, R);
@@ -463,6 +538,7 @@ __device__ __forceinline__ void walk(const ScaledAttnArgs& a, const int32_t* bt,
     for (; i < free; ++i) window<QT, false>(a, t, head, i, at_k, at_v, lane, w, R);
     for (; i < t.n; ++i) window<QT, true>(a, t, head, i, at_k, at_v, lane, w, R);
   }
+  if (__float_as_uint(R.unit) != __float_as_uint(1.0f)) to_unit<QT>(1.0f, R);
 }
 
 // row r's 8 outputs of dims d .. d + 7
