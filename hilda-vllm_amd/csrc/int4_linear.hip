@@ -160,7 +160,8 @@ __global__ __launch_bounds__(64 * W) void k_int4_rows(Int4Args a) {
 #pragma unroll
   for (int t = 0; t < TN; ++t) y[t] = f32x4_t{0, 0, 0, 0};
   // One step's loads at a time: many waves hide them better than many loads of few waves
-  // (12288 features, SwiGLU, 4 rows: 20.8 us with 8 waves and two steps ahead, 17.3 us so)
+  // (12288 features, SwiGLU, 4 rows: 20.8 us with 8 waves and two steps ahead, 17.3 us so
+  // when that was measured; 16.0 us as the codes are decoded now)
   for (int step = wave; step < a.steps; step += W) {
     bf16x8_t x[4];
     Step<GP> w[TN];
@@ -212,8 +213,9 @@ __device__ __forceinline__ uint4 as_uint4(u32x4_t v) { return make_uint4(v.x, v.
 // are empty and they touch no memory. Two and three steps ahead took the same time or
 // longer; what bounds it is a wave's own chain of operand reads, code shifts and products.
 // H = 2: two sets of waves, each with rows of its own in LDS, take the steps in turn and
-// join their sums in LDS. 64 rows of 12288 inputs, 4096 features: 21.0 us (307 TFLOP/s), 4
-// of them the join's launch; 600 rows of 4096 inputs, 2 x 12288 features: 167 us (723 TFLOP/s).
+// join their sums in LDS. 64 rows of 12288 inputs, 4096 features: 22.1 us (291 TFLOP/s), 4
+// of them the join's launch; 600 rows of 4096 inputs, 2 x 12288 features: 167 us (723 TFLOP/s),
+// 4096 rows 1021 us (808): every 64 rows decode the weights again.
 template <int GP, bool kGate, int H>
 __global__ __launch_bounds__(64 * kTileWaves * H, H == 1 && GP < 4 ? 3 : 2)
 void k_int4_tile(Int4Args a) {

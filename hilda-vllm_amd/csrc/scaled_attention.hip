@@ -15,7 +15,9 @@
 // tokens 18.1 and 17.5). Longer prompts are bound by the vector and matrix pipes and round
 // them to bf16 once (the listed prompts 175 us, 225 us in two parts): their error against
 // 64-bit sums is 1.85e-3 of the outputs' size, root mean square, where the output's own
-// rounding is 1.66e-3. The sum below takes the same rounded ones.
+// rounding is 1.66e-3. The sum below takes the same rounded ones. (Scales that differ by more
+// than powers of two from group to group cost long prompts the change of unit in every
+// group: the listed prompts 209 us, 185 us with a second rounding of the weights instead.)
 //
 // A wave works on its own, without LDS in its loop. It takes a window's K rows as
 // the A operand of S^T = K Q^T (lane l: key l % 16, dims 32 (l / 16) .. + 31, two
@@ -33,11 +35,13 @@
 //    are written before they are read and nothing is counted between the launches,
 //    so the workspace needs no preparation.
 //    It is bound by the cache's stream, which it reads once: 256 decodes of 64 to 2048
-//    keys of 8 heads 123 us (4.6 TB/s), 32 of 2048 to 8192 84 us (4.1), 64 verify steps of
-//    64 to 2048 keys 41.8 us (3.4, of which the join's launch is about 5).
+//    keys of 8 heads 124 us (4.5 TB/s), 32 of 2048 to 8192 86 us (4.0), 64 verify steps of
+//    64 to 2048 keys 41.9 us (3.4, of which the join's launch is about 5).
 //  * k_scaled_rows: prompts. A wave takes 16 QT query rows and all of their keys; bound by
 //    decoding and the softmax beside the products (prompts of up to 2043 tokens behind up
-//    to 1000 keys: 175 us, 636 TFLOP/s).
+//    to 1000 keys: 176 us, 633 TFLOP/s). A call's longest prompt chooses the kernel for all of its
+//    sequences: decodes beside a prompt are not split (31 of 8192 keys with one prompt of 130
+//    tokens: 288 us, 115 us the decodes alone).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -83,7 +87,8 @@ struct ScaledAttnArgs {
   float* part_ml;  // [sequence, kv head, tile, split][16][2]
 };
 
-// Sequence b's bounds, clamped so that a call's odd lengths never index out of it.
+// Sequence b's first query row and lengths, as the caller gives them: its query rows lie
+// within q and out. Its keys go through the block table, which is checked entry by entry.
 struct Seq {
   int qs, Lq, Lk;
 };

@@ -21,7 +21,9 @@
 // Launch: a workgroup per (chunk of tokens, kv head, K or V). It takes the tokens of its
 // chunk whose predecessor in the call lies in another group, looks through the
 // call's whole slot list for the group's other tokens (so the tokens of a group may
-// stand anywhere in the call; the list is a few KB and read from L2), leaves the group to
+// stand anywhere in the call; read from L2, so that the reads grow with the square of the
+// call's tokens: 4000 tokens of 8 heads 13.6 us, 8000 25.8 us, 24000 121 us, five times
+// their bytes' time), leaves the group to
 // the workgroup of its first token, and otherwise does all of the group's work, the rows
 // held in registers from their maximum to their codes. No two workgroups write one group
 // and head, and a slot that occurs twice takes the row of the higher token index, so the

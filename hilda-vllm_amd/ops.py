@@ -316,7 +316,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     likely tokens (hs_token_logprobs), of softmax(logits / temperature).
 
     logits [rows, V] f32/bf16, tokens [rows] integers (outside [0, V): -inf),
-    temperatures [rows] > 0, top 0 .. 32. Returns dict(logprobs=[rows] f32 or None,
+    temperatures [rows] normal f32 > 0, top 0 .. 32. Returns dict(logprobs=[rows] f32 or None,
     entropy=[rows] f32, top_ids=[rows, top] int64 and top_logprobs=[rows, top] f32, None
     with top 0): largest logits first, the lower id first among equal ones. A row with a
     NaN, a +inf or nothing but -inf gives NaN. Calls may overlap on streams and in
@@ -1050,10 +1050,11 @@ def quantize_int4(weight: torch.Tensor, group: int = 128) -> Int4Weight:
 
 def linear_int4(x: torch.Tensor, weight: Int4Weight, *, swiglu: bool = False,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-    """linear with a 4-bit weight (hs_linear_int4): x [rows, K] bf16, any number of
-    rows -> [rows, N] bf16, fp32 accumulation. With swiglu=True the weight is
-    [2F, K] (gate | up), F a multiple of 16, and the result silu(gate) * up
-    [rows, F]. An infinity in a row of x gives NaN in that row."""
+    """linear with a 4-bit weight (hs_linear_int4; an Int4Weight or what has its
+    fields): x [rows, K] bf16, up to 2^20 rows -> [rows, N] bf16, fp32 accumulation.
+    With swiglu=True the weight is [2F, K] (gate | up), F a multiple of 16, and the
+    result silu(gate) * up [rows, F]. Finite inputs may be of any size; an infinity
+    in a row of x gives NaN in that row."""
     w, packed, scales = weight, weight.packed, weight.scales
     dev = _need_cuda(x, packed, scales, out)
     if x.dim() != 2 or x.dtype != torch.bfloat16:

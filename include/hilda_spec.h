@@ -165,10 +165,10 @@ int hs_sampler(const void* logits, int logits_dtype, int64_t logits_row_stride,
 /* lower index first among equal ones (-0 equals 0, NaN is the largest), with */
 /* their log-probabilities. top: 0 .. 32, at most vocab. A row with a NaN, a   */
 /* +inf or nothing but -inf gives NaN log-probabilities and entropy.          */
-/* logits [rows, vocab] HS_F32 or HS_BF16, temperatures [rows] f32 > 0 or     */
-/* NULL (1); tokens and logprobs both or neither; entropy may be NULL. At most */
-/* 65535 rows and 2^21 tokens. The workspace needs no preparation and holds    */
-/* nothing between calls.                                                      */
+/* logits [rows, vocab] HS_F32 or HS_BF16, temperatures [rows] f32, normal     */
+/* numbers > 0, or NULL (1); tokens and logprobs both or neither; entropy may  */
+/* be NULL. At most 65535 rows and 2^21 tokens. The workspace needs no         */
+/* preparation and holds nothing between calls.                                */
 size_t hs_token_logprobs_workspace_size(int rows, int vocab, int top);
 int hs_token_logprobs(const void* logits, int logits_dtype, int64_t logits_row_stride, int rows,
                       int vocab, const int64_t* tokens, const float* temperatures, int top,
@@ -529,13 +529,13 @@ int hs_linear_rmsnorm(const void* x, int64_t x_stride, const void* residual_in,
                       int in_features, int out_features, int epilogue, void* out,
                       int64_t out_stride, void* stream);
 
-/* hs_linear with 4-bit weights and group scales, any number of rows (no       */
+/* hs_linear with 4-bit weights and group scales, up to 2^20 rows (no           */
 /* counterpart in the reference): weight[n, k] = (code[n, k] - 8) *             */
 /* scale[n, k / group], code 0 .. 15, group 32, 64 or 128 (a divisor of        */
 /* in_features), x and out bf16, fp32 accumulation. HS_LINEAR_SWIGLU: weight    */
 /* [2 * out_features, in_features] gate | up, out = silu(gate) * up rounded     */
-/* once; out_features then a multiple of 16. An infinity in a row of x gives    */
-/* NaN there.                                                                  */
+/* once; out_features then a multiple of 16. Finite inputs may be of any size;  */
+/* an infinity in a row of x gives NaN there.                                  */
 /* packed: [tiles][steps][64][4] 32-bit words, tile = 16 weight rows, step =    */
 /* 128 inputs: word i of lane l holds row 16 tile + l % 16, inputs 128 step +   */
 /* 32 i + 8 (l / 16) + e, e = 0 .. 7, input 2 p at bits 4 p and input 2 p + 1   */
