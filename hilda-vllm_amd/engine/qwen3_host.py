@@ -71,17 +71,20 @@ class Int4Projection(nn.Module):
         self.out_features, self.in_features, self.group = w.out_features, w.in_features, w.group
 
 
+_INT4 = (Int4Projection, _ops.Int4Weight)  # the second where a caller has set one itself
+
+
 def _norm_proj(x, norm, eps, w, residual=None, swiglu=False):
     """ops.linear_rmsnorm, or with a 4-bit weight the RMSNorm kernel and its projection
     (the residual is then updated in place)."""
-    if isinstance(w, Int4Projection):
+    if isinstance(w, _INT4):
         xn = _ops.rmsnorm(x, norm, eps, residual=residual)
         return _ops.linear_int4(xn, w, swiglu=swiglu), (x if residual is None else residual)
     return _ops.linear_rmsnorm(x, norm, eps, w, residual=residual, swiglu=swiglu)
 
 
 def _proj(x, w):
-    return _ops.linear_int4(x, w) if isinstance(w, Int4Projection) else _ops.linear(x, w)
+    return _ops.linear_int4(x, w) if isinstance(w, _INT4) else _ops.linear(x, w)
 
 
 class Rope(nn.Module):
@@ -168,7 +171,7 @@ class Qwen3Layer(nn.Module):
         where one refuses the group."""
         new = {name: Int4Projection(_ops.quantize_int4(w, group))
                for name in ("qkv", "o", "gate_up", "down")
-               if not isinstance(w := getattr(self, name), Int4Projection)}
+               if not isinstance(w := getattr(self, name), _INT4)}
         for name, q in new.items():
             delattr(self, name)
             setattr(self, name, q)
@@ -176,7 +179,7 @@ class Qwen3Layer(nn.Module):
     def forward_reference(self, positions, h, residual):
         """Eager PyTorch restatement of the same layer (used by tests; bf16 weights)."""
         g = self.g
-        if any(isinstance(w, Int4Projection) for w in (self.qkv, self.o, self.gate_up, self.down)):
+        if any(isinstance(w, _INT4) for w in (self.qkv, self.o, self.gate_up, self.down)):
             raise TypeError("the restatement takes bf16 weights; this layer's are in 4 bits")
         if residual is None:
             x, residual = rms_norm(h, self.ln1, g.rms_eps), h
@@ -243,7 +246,7 @@ class Qwen3Host(nn.Module):
         A model that shares this one's weights keeps those it was built with."""
         for layer in self.layers:
             layer.quantize_int4(group)
-        if lm_head and not isinstance(self.lm_head, Int4Projection):
+        if lm_head and not isinstance(self.lm_head, _INT4):
             q = Int4Projection(_ops.quantize_int4(self.lm_head, group))
             del self.lm_head
             self.lm_head = q

@@ -28,3 +28,20 @@ def test_state_of_a_quantised_model(cuda):
     shared = q3.Qwen3Host(g, device=cuda, share_from=a, num_layers=1)
     assert torch.equal(shared.compute_logits(h), want)
     assert shared.layers[0].qkv is a.layers[0].qkv
+
+
+def test_packed_weights_set_by_the_caller(hv, cuda):
+    """Codes that come from elsewhere, as plain Int4Weights in the model's places."""
+    q3 = importlib.import_module("hilda-vllm_amd.engine.qwen3_host")
+    print("packed weights set by the caller", flush=True)
+    g = q3.Qwen3Geometry(num_layers=1, hidden=256, num_heads=2, num_kv_heads=1, ffn=384, vocab=301,
+                         max_position=64)
+    a = q3.Qwen3Host(g, device=cuda, seed=1)
+    w = hv.ops.quantize_int4(a.lm_head, 64)
+    h = torch.randn(5, 256, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    want = hv.ops.linear_int4(h, w)
+    del a.lm_head
+    a.lm_head = w
+    assert torch.equal(a.compute_logits(h), want)
+    a.quantize_int4(128, lm_head=True)  # leaves it as it is
+    assert a.lm_head is w
