@@ -562,7 +562,7 @@ def verify_attention_scaled(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if N == 0:
         return out
     # (the bound on the keys sizes the launch alone: with none, all rows get zeros)
-    mq, mk = int(max_seqlen_q), max(int(max_seqlen_k), 1)
+    mq, mk = int(max_seqlen_q), int(max_seqlen_k) or 1
     nbytes = L.lib().hs_verify_attention_scaled_workspace_size(B, Hq, Hkv, mq, mk)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     ost = out.stride()

@@ -19,3 +19,14 @@ def test_rows_without_keys(hv, cuda, rows):
                                                                        device=cuda),
                                          cu, torch.zeros_like(cu), max(rows), 0, 0.1)
     assert bool((out == 0).all())
+
+
+def test_a_negative_bound_is_refused(hv, cuda):
+    print("negative bound on the keys", flush=True)
+    kc = torch.zeros((2, 64, 8, 128), dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn)
+    ks = torch.ones((2, 2, 8), device=cuda)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    with pytest.raises(RuntimeError):
+        hv.ops.verify_attention_scaled(torch.zeros(1, 16, 128, dtype=torch.bfloat16, device=cuda), kc,
+                                       kc, ks, ks, torch.zeros((1, 1), dtype=torch.int32, device=cuda),
+                                       cu, cu, 1, -1, 0.1)
