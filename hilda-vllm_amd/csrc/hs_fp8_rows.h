@@ -1,0 +1,73 @@
+// Rows in 8 bits: e4m3 codes with one power of two for every 128 values of a row, kept as
+// its biased exponent (e8m0: 127 + log2 of the scale; 1 .. 254 here, 255 is NaN).
+//
+// The scale of a group is the smallest power of two s, not below 2^-126, with |v| <= 448 s
+// for the group's finite values; the code is e4m3(v / s), rounded once, from f32, and NaN
+// where v is NaN or infinite. A power of two costs e4m3, itself a floating type, no
+// precision down to its subnormals, v / s is exact, and the matrix instructions apply it
+// (their block exponents), so that a product has no work for it.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "hs_model_dev.h"
+
+namespace hs {
+
+constexpr int kFp8Group = 128;  // values of a scale
+
+// the bits of |v|, 0 where v is NaN or infinite
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// The scale's exponent byte for a group whose largest finite |v| has these bits: 448 is
+// 1.75 2^8, so the exponent of |v| over 2^8, one more where its mantissa is above 1.75.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+  const int e = (int)((amax_bits + 0x1fffffu) >> 23) - 8;
+  return (uint32_t)(e < 1 ? 1 : e);  // at most 247
+}
+// 1 / scale
+__device__ __forceinline__ float scale_inverse(uint32_t byte) {
+  return __uint_as_float((254u - byte) << 23);
+}
+
+// the code of NaN and the infinities is NaN: as NaN itself, whatever the conversion does
+// with infinities
+__device__ __forceinline__ float nan_unless_finite(float v) {
+  return fabsf(v) < __builtin_inff() ? v : __builtin_nanf("");
+}
+
+// codes of four values (v_cvt_pk_fp8_f32: round to nearest even; finite |v / s| <= 448)
+__device__ __forceinline__ uint32_t codes4(const float* v, float inv) {
+  int w = 0;
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(v[0]) * inv, nan_unless_finite(v[1]) * inv,
+                                      w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(v[2]) * inv, nan_unless_finite(v[3]) * inv,
+                                      w, true);
+  return (uint32_t)w;
+}
+
+// the largest of the 16 lanes of a DPP row, in every lane
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, false));
+  return v;
+}
+
+// Codes of 8 values a lane, 16 lanes a group: all lanes of the row take part, lanes past the
+// row's end with zeros. Returns the scale's byte.
+__device__ __forceinline__ uint32_t group_codes8(const float (&v)[8], uint2& codes) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, finite_bits(v[i]));
+  const uint32_t byte = scale_byte(row16_max(m));
+  const float inv = scale_inverse(byte);
+  codes = make_uint2(codes4(v, inv), codes4(v + 4, inv));
+  return byte;
+}
+
+}  // namespace hs

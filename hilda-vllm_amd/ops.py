@@ -1086,3 +1086,195 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, *, swiglu: bool = False,
           M, K, N, w.group, epi, out.data_ptr(), out.stride(0),
           ws.data_ptr() if nbytes else None, nbytes)
     return out
+
+
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits: codes float8_e4m3fn [rows, K] and scales float8_e8m0fnu [rows,
+    ceil(K / 128)], a power of two for every 128 values of a row; value = code * scale.
+    quantize_rows_fp8, rmsnorm_fp8 and linear_fp8(quantize=True) make them."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+class Fp8Weight(NamedTuple):
+    """A projection's weight in e4m3 with a scale for every block of 128 x 128, in the
+    layout of hs_linear_fp8: packed uint8 [tiles, steps, 2, 64, 16] and scales f32 [tiles,
+    steps] over 16-feature tiles and 128-input steps. pack_fp8 and quantize_fp8 make one."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    out_features: int
+    in_features: int
+
+
+def _new_rows_fp8(x: torch.Tensor, rows: int, width: int) -> Fp8Rows:
+    groups = -(-width // 128)
+    scales = x.new_empty((rows, -(-groups // 4) * 4), dtype=torch.float8_e8m0fnu)
+    return Fp8Rows(x.new_empty((rows, width), dtype=torch.float8_e4m3fn),
+                   scales if groups % 4 == 0 else scales[:, :groups])
+
+
+def _bf16_rows(t: torch.Tensor, most: int = 1 << 40) -> torch.Tensor:
+    """t [rows, K] with rows that the kernels can read in 16-byte pieces: t or a copy."""
+    st = t.stride()
+    if st[1] != 1 or st[0] % 8 or not t.shape[1] <= st[0] <= most or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
+    """bf16 rows x [rows, K], K a multiple of 16, in 8 bits (hs_quantize_rows_fp8): for
+    every 128 values of a row the smallest power of two s, at least 2^-126, with |x| <= 448
+    s, and e4m3(x / s). NaN and infinities become NaN and take no part in the scale."""
+    dev = _need_cuda(x)
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] < 1 or x.shape[1] % 16:
+        raise ValueError("quantize_rows_fp8 expects a 2-D bf16 input with a multiple of 16 "
+                         "columns")
+    M, K = x.shape
+    out = _new_rows_fp8(x, M, K)
+    if M:
+        x = _bf16_rows(x)
+        _call(dev, "hs_quantize_rows_fp8", x.data_ptr(), x.stride(0), M, K, out.codes.data_ptr(),
+              K, out.scales.data_ptr(), out.scales.stride(0))
+    return out
+
+
+def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                residual: torch.Tensor | None = None) -> Fp8Rows:
+    """rmsnorm to rows in 8 bits (hs_rmsnorm_fp8): with h = x (+ residual), the residual
+    updated in place to bf16(h), the rows are h * rsqrt(mean(h^2) + eps) * weight in fp32
+    and go to 8 bits as in quantize_rows_fp8, without rounding to bf16 between. x [rows,
+    H] bf16, H a multiple of 16."""
+    dev = _need_cuda(x, weight, residual)
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] < 1 or x.shape[1] % 16:
+        raise ValueError("rmsnorm_fp8 expects a 2-D bf16 input with a multiple of 16 columns")
+    M, H = x.shape
+    if weight.shape != (H,) or weight.dtype != torch.bfloat16:
+        raise ValueError("weight must be bf16 [H]")
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != torch.bfloat16:
+            raise ValueError("residual must be bf16 with x's shape")
+        if M > 1 and residual.stride(0) < H * residual.stride(1) or residual.stride(1) < 1:
+            raise ValueError("residual is updated in place: its rows must not overlap")
+    out = _new_rows_fp8(x, M, H)
+    if not M:
+        return out
+    x = _bf16_rows(x)
+    if weight.stride(0) != 1 or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    res = None if residual is None else _bf16_rows(residual)
+    _call(dev, "hs_rmsnorm_fp8", x.data_ptr(), x.stride(0),
+          None if res is None else res.data_ptr(), 0 if res is None else res.stride(0),
+          weight.data_ptr(), float(eps), M, H, out.codes.data_ptr(), H, out.scales.data_ptr(),
+          out.scales.stride(0))
+    if res is not residual:
+        residual.copy_(res)
+    return out
+
+
+def pack_fp8(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Weight:
+    """Lays out codes float8_e4m3fn [N, K], K a multiple of 16, and scales f32 [ceil(N /
+    128), ceil(K / 128)] (the weight is code * scale of its 128 x 128 block) for linear_fp8.
+    Done once a weight, with torch operations on the tensors' device."""
+    if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise TypeError("codes must be float8_e4m3fn and scales float32")
+    if codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] < 1 or codes.shape[1] % 16:
+        raise ValueError("codes must be [N, K] with K a multiple of 16")
+    N, K = codes.shape
+    if scales.shape != (-(-N // 128), -(-K // 128)):
+        raise ValueError("scales must be [ceil(N / 128), ceil(K / 128)]")
+    tiles, steps = -(-N // 16), -(-K // 128)
+    c = torch.zeros((tiles * 16, steps * 128), dtype=torch.uint8, device=codes.device)
+    c[:N, :K] = codes.view(torch.uint8)
+    # [tile, feature, step, h, g, byte] -> [tile, step, h, lane (g, feature), byte]
+    c = c.view(tiles, 16, steps, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous()
+    s = scales.repeat_interleave(8, 0)[:tiles].contiguous()
+    return Fp8Weight(c.view(tiles, steps, 2, 64, 16), s, N, K)
+
+
+def quantize_fp8(weight: torch.Tensor) -> Fp8Weight:
+    """A float weight [N, K] to e4m3: the scale of a 128 x 128 block is its largest |w|
+    over 448 (at least 2^-126), the codes are the nearest ones."""
+    if weight.dim() != 2 or not weight.is_floating_point() or weight.shape[0] < 1 or \
+            weight.shape[1] < 1 or weight.shape[1] % 16:
+        raise ValueError("weight must be a floating [N, K] tensor with K a multiple of 16")
+    N, K = weight.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    w = torch.nn.functional.pad(weight.float(), (0, kb * 128 - K, 0, nb * 128 - N))
+    w = w.view(nb, 128, kb, 128)
+    scales = (w.abs().amax((1, 3)) / 448).clamp_(min=2.0 ** -126)
+    codes = (w / scales[:, None, :, None]).clamp_(-448, 448).to(torch.float8_e4m3fn)
+    return pack_fp8(codes.view(nb * 128, kb * 128)[:N, :K], scales)
+
+
+def _rows_fp8(x: Fp8Rows) -> Fp8Rows:
+    """Checks rows in 8 bits; returns them, or copies that the kernels can read."""
+    codes, scales = x.codes, x.scales
+    if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu:
+        raise TypeError("rows in 8 bits are float8_e4m3fn codes with float8_e8m0fnu scales")
+    if codes.dim() != 2 or scales.shape != (codes.shape[0], -(-codes.shape[1] // 128)):
+        raise ValueError("rows in 8 bits are codes [rows, K] with scales [rows, ceil(K / 128)]")
+    (M, K), cst, sst = codes.shape, codes.stride(), scales.stride()
+    if cst[1] != 1 or cst[0] % 16 or not K <= cst[0] <= 1 << 22 or codes.data_ptr() % 16:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    groups = scales.shape[1]
+    whole = -(-groups // 4) * 4  # bytes of a row that the kernels may read
+    if sst[1] != 1 or sst[0] % 4 or not whole <= sst[0] <= 1 << 22 or scales.data_ptr() % 4 or (
+            groups != whole and scales.storage_offset() + (M - 1) * sst[0] + whole
+            > scales.untyped_storage().nbytes()):
+        wide = scales.new_empty((M, whole))
+        wide[:, :groups].copy_(scales)
+        scales = wide
+    return Fp8Rows(codes, scales)
+
+
+def linear_fp8(x, weight: Fp8Weight, *, swiglu: bool = False, quantize: bool = False,
+               out: torch.Tensor | None = None):
+    """linear with rows and weight in 8 bits (hs_linear_fp8; weight an Fp8Weight or what
+    has its fields): x Fp8Rows, or [rows, K] bf16, which goes to 8 bits first as in
+    quantize_rows_fp8; up to 2^20 rows -> [rows, N] bf16, fp32 accumulation. With
+    swiglu=True the weight is [2F, K] (gate | up), F a multiple of 16, and the result
+    silu(gate) * up [rows, F]; with quantize=True beside it that result as Fp8Rows, rounded
+    from fp32 once."""
+    rows8 = not isinstance(x, torch.Tensor)
+    xc, xs = (x.codes, x.scales) if rows8 else (x, None)
+    w, packed, scales = weight, weight.packed, weight.scales
+    dev = _need_cuda(xc, xs, packed, scales, out)
+    if rows8:
+        xc, xs = _rows_fp8(x)
+    elif x.dim() != 2 or x.dtype != torch.bfloat16:
+        raise ValueError("linear_fp8 expects Fp8Rows or a 2-D bf16 input")
+    M, K = xc.shape
+    if K != w.in_features or K % 16:
+        raise ValueError("in_features mismatch")
+    if quantize and (not swiglu or out is not None):
+        raise ValueError("quantize goes with swiglu, and returns new rows")
+    if swiglu and w.out_features % 32:
+        raise ValueError("swiglu needs gate and up halves of a multiple of 16 features")
+    tiles, steps = -(-w.out_features // 16), -(-K // 128)
+    if packed.dtype != torch.uint8 or scales.dtype != torch.float32 or \
+            packed.shape != (tiles, steps, 2, 64, 16) or scales.shape != (tiles, steps) or \
+            not packed.is_contiguous() or not scales.is_contiguous():
+        raise ValueError("weight is not laid out as pack_fp8 does")
+    N = w.out_features // 2 if swiglu else w.out_features
+    epi = L.HS_LINEAR_PLAIN
+    if quantize:
+        rows, epi = _new_rows_fp8(xc, M, N), L.HS_LINEAR_SWIGLU_FP8
+        out = rows.codes
+    else:
+        if swiglu:
+            epi = L.HS_LINEAR_SWIGLU
+        if out is None:
+            out = packed.new_empty((M, N), dtype=torch.bfloat16)
+        elif out.shape != (M, N) or out.stride(1) != 1 or out.dtype != torch.bfloat16:
+            raise ValueError("out must be [rows, out_features] bf16 with contiguous rows")
+    if M:
+        if not rows8:
+            xc = _bf16_rows(xc, 1 << 22)
+        nbytes = L.lib().hs_linear_fp8_workspace_size(M, K, N, epi, not rows8)
+        ws = packed.new_empty(nbytes) if nbytes else None
+        _call(dev, "hs_linear_fp8", xc.data_ptr(), xc.stride(0),
+              xs.data_ptr() if rows8 else None, xs.stride(0) if rows8 else 0, packed.data_ptr(),
+              scales.data_ptr(), M, K, N, epi, out.data_ptr(), out.stride(0),
+              rows.scales.data_ptr() if quantize else None,
+              rows.scales.stride(0) if quantize else 0, ws.data_ptr() if nbytes else None, nbytes)
+    return rows if quantize else out

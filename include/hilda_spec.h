@@ -512,6 +512,7 @@ int hs_zero_kv_slots(void* cache, int64_t plane_bytes, int num_planes, int64_t s
 /* elements. Larger row counts are plain library GEMMs.                        */
 #define HS_LINEAR_PLAIN 0
 #define HS_LINEAR_SWIGLU 1
+#define HS_LINEAR_SWIGLU_FP8 2 /* hs_linear_fp8 only */
 int hs_linear(const void* x, int64_t x_stride, const void* weight, int rows, int in_features,
               int out_features, int epilogue, void* out, int64_t out_stride, void* stream);
 
@@ -548,6 +549,48 @@ size_t hs_linear_int4_workspace_size(int rows, int in_features, int out_features
 int hs_linear_int4(const void* x, int64_t x_stride, const void* packed, const void* scales,
                    int rows, int in_features, int out_features, int group, int epilogue, void* out,
                    int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows in 8 bits (no counterpart in the reference): float8_e4m3fn codes [rows,  */
+/* width] with one exponent byte (float8_e8m0fnu, the scale is 2^(byte - 127)) for */
+/* every 128 values of a row, [rows, ceil(width / 128)]: value = code * scale. A   */
+/* group's scale is the smallest power of two s, at least 2^-126, with |v| <= 448 s */
+/* for its finite values; the code is v / s rounded to nearest even, once, from     */
+/* fp32, and NaN for NaN and the infinities. width a multiple of 16, strides in     */
+/* elements: of x a multiple of 8, of codes of 8; x 16-byte, codes 8-byte aligned.  */
+/* hs_quantize_rows_fp8: of bf16 rows x.                                            */
+/* hs_rmsnorm_fp8: of h * rsqrt(mean(h^2) + eps) * weight in fp32, h = x (+         */
+/* residual); with residual != NULL the residual row is replaced by bf16(h) (its    */
+/* stride a multiple of 8, it and weight bf16 and 16-byte aligned).                 */
+int hs_quantize_rows_fp8(const void* x, int64_t x_stride, int rows, int width, void* codes,
+                         int64_t codes_stride, void* scales, int64_t scales_stride, void* stream);
+int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t residual_stride,
+                   const void* weight, float eps, int rows, int hidden, void* codes,
+                   int64_t codes_stride, void* scales, int64_t scales_stride, void* stream);
+
+/* Projection of rows in 8 bits by e4m3 weights with a scale for every block of 128 */
+/* x 128 (no counterpart in the reference), up to 2^20 rows: out[r, n] = sum_k      */
+/* x[r, k] * code[n, k] * scale[n / 128, k / 128], fp32 accumulation, bf16 out.     */
+/* HS_LINEAR_SWIGLU: weight [2 * out_features, in_features] gate | up, out =        */
+/* silu(gate) * up rounded once; HS_LINEAR_SWIGLU_FP8: the same product as rows in  */
+/* 8 bits (out: codes, out_scales: their exponent bytes); out_features a multiple   */
+/* of 16 for both. x: codes with x_scales, or bf16 with x_scales NULL (quantised in  */
+/* the call as hs_quantize_rows_fp8 does). in_features a multiple of 16.             */
+/* packed: bytes [tiles][steps][2][64][16], tile = 16 weight rows, step = 128 inputs: */
+/* byte j at (h, lane) is the code of row 16 tile + lane % 16, input 128 step + 64 h */
+/* + 16 (lane / 16) + j. scales: f32 [tiles][steps], the scale of the tile's block.  */
+/* Rows past the last and inputs past in_features are padded with zeros.             */
+/* Strides in elements: x_stride a multiple of 16 (bf16: 8), at most 2^22;           */
+/* x_scales_stride a multiple of 4, at least ceil(steps / 4) * 4 (the bytes past     */
+/* the last step may hold anything), x_scales 4-byte aligned; x and packed 16-byte   */
+/* aligned; codes of HS_LINEAR_SWIGLU_FP8 16-byte aligned with a stride that is a    */
+/* multiple of 16. The workspace needs no preparation and holds nothing between calls. */
+size_t hs_linear_fp8_workspace_size(int rows, int in_features, int out_features, int epilogue,
+                                    int bf16_rows);
+int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t x_scales_stride,
+                  const void* packed, const float* scales, int rows, int in_features,
+                  int out_features, int epilogue, void* out, int64_t out_stride, void* out_scales,
+                  int64_t out_scales_stride, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 /* out = RMSNorm(x (+ residual)) * weight; with residual != NULL the residual  */
 /* row is replaced by bf16(x + residual) (strides in elements).              */
