@@ -21,6 +21,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/hilda_spec.h"
 #include "hs_fp8_rows.h"
 
@@ -50,6 +52,7 @@ struct Fp8Args {
   int64_t yes;
   float* part;        // [split][rows][tiles * 16]
   int split_steps, nsplit;
+  int cols, rowtiles;  // workgroups of the large tiles
 };
 
 __device__ __forceinline__ i32x8_t operand(uint4 a, uint4 b) {
@@ -58,10 +61,11 @@ __device__ __forceinline__ i32x8_t operand(uint4 a, uint4 b) {
 
 constexpr int kOne = 0x7f7f7f7f;  // block exponents of 2^0
 
-// 16 features by 16 rows, one step; xe: the lane's row's exponent byte in bits 0 .. 7
+// 16 features by 16 rows, one step; the lane's row's exponent is byte B of xe
+template <int B>
 __device__ __forceinline__ f32x4_t mfma(i32x8_t w, i32x8_t x, uint32_t xe) {
   const f32x4_t zero = {0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, kOne, 0, (int)xe);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, kOne, B, (int)xe);
 }
 
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(64 * W) void k_fp8_rows(Fp8Args a) {
     const i32x8_t x = operand(load_x(a, row, step, 0, g), load_x(a, row, step, 1, g));
     const uint32_t e = xe[step];
 #pragma unroll
-    for (int t = 0; t < TN; ++t) y[t] += sw[t] * mfma(w[t], x, e);
+    for (int t = 0; t < TN; ++t) y[t] += sw[t] * mfma<0>(w[t], x, e);
   }
 #pragma unroll
   for (int t = 0; t < TN; ++t) *reinterpret_cast<f32x4_t*>(&s_part[wave][t][m][4 * g]) = y[t];
@@ -135,6 +139,254 @@ __global__ __launch_bounds__(64 * W) void k_fp8_rows(Fp8Args a) {
       if (kGate) a.part[(r0 + r) * width + (int64_t)a.units * 16 + col] = up;
     } else if (col < a.N) {
       a.y[(int64_t)(r0 + r) * a.ys + col] = result<kGate>(v, up);
+    }
+  }
+}
+
+// ---- many rows: 256 features by 256 rows a workgroup -----------------------------------
+
+constexpr int kBig = 256;                   // features and rows of a workgroup
+constexpr int kBigThreads = 512;            // 4 waves over the features, 2 over the rows
+constexpr int kPast = INT32_MAX;            // a byte offset past any buffer: reads zeros
+constexpr int kRange = INT32_MAX - 255;
+constexpr int kStageX = kBig * kStep;       // bytes of a step's rows, and of its weights
+
+// 16 bytes a lane from a buffer straight to LDS, at lds + 16 lane. The compiler does not see
+// the write: the wait before the barrier behind a step covers it. (Through the builtin it
+// would wait for the load before the next read of any shared memory.)
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, int offset, int at,
+                                         uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(lds), "v"(offset), "s"(from), "s"(at)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+// waits for the wave's loads and LDS traffic, then for the other waves
+__device__ __forceinline__ void step_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// the 16-byte piece of a row's step that lies at piece p of the row in LDS, and back
+__device__ __forceinline__ int swizzle(int row, int p) { return p ^ (row & 7); }
+
+template <int kEpilogue>
+__global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
+  constexpr bool kGate = kEpilogue != HS_LINEAR_PLAIN;
+  extern __shared__ uint4 s_all[];  // [stage][x: row, piece | w: tile, half, lane]
+  uint8_t* s_bytes = reinterpret_cast<uint8_t*>(s_all);
+  const uint32_t lds = lds_address(s_all);
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wf = wave & 3, wr = wave >> 2;
+  // the workgroup's tile: each XCD has a stretch of them, 8 row tiles to a column
+  int u0, r0;
+  {
+    const int total = a.cols * a.rowtiles;
+    const int id = blockIdx.x, x = id & 7, q = total >> 3, r = total & 7;
+    const int o = x * q + min(x, r) + (id >> 3);
+    const int group = o / (8 * a.cols), in = o % (8 * a.cols);
+    const int high = min(8, a.rowtiles - 8 * group);
+    r0 = (8 * group + in % high) * kBig;
+    u0 = in / high * (kGate ? 8 : 16);
+  }
+  auto tile_of = [&](int slot) {  // weight tile of one of the workgroup's 16 slots
+    const int f = slot & 3;
+    const int u = kGate ? u0 + (slot >> 2) * 2 + (f & 1) : u0 + slot;
+    return min(u, a.units - 1) + (kGate && f >= 2 ? a.up : 0);
+  };
+  // this wave's loads: 32 rows and two weight tiles
+  const int piece = swizzle(lane >> 3, lane & 7);
+  int xo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 32 * wave + 8 * i + (lane >> 3);
+    xo[i] = r0 + row < a.rows ? row * (int)a.xs + 16 * piece : kPast;
+  }
+  const int64_t tile_bytes = (int64_t)a.steps * (16 * kStep);
+  uint8_t* wp = reinterpret_cast<uint8_t*>(const_cast<uint4*>(a.w));
+  uint8_t* xp = const_cast<uint8_t*>(a.x + (int64_t)r0 * a.xs);
+  uint8_t* wp0 = wp + tile_of(2 * wave) * tile_bytes;
+  uint8_t* wp1 = wp + tile_of(2 * wave + 1) * tile_bytes;
+  // load i of the eight that bring in a step; past the last step none reads memory
+  auto load = [&](int step, int i) {
+    const uint32_t to = lds + (step & 1) * 2 * kStageX;
+    const int range = step < a.steps ? kRange : 0;
+    if (i < 4) {
+      const auto b = __builtin_amdgcn_make_buffer_rsrc(xp, 0, range, 0x00027000);
+      const bool in = kStep * step + 16 * piece < a.K;
+      load_lds(b, in ? xo[i] : kPast, kStep * step, to + (32 * wave + 8 * i) * kStep);
+    } else {
+      const auto b = __builtin_amdgcn_make_buffer_rsrc(i < 6 ? wp0 : wp1, 0, range, 0x00027000);
+      load_lds(b, 16 * lane + 1024 * (i & 1), 16 * kStep * step,
+               to + kStageX + (wave * 4 + i - 4) * 1024);
+    }
+  };
+  // exponents of this lane's 8 rows, four steps a word, and scales of the wave's 4 tiles,
+  // a step a lane
+  uint8_t* ep = const_cast<uint8_t*>(a.xe + (int64_t)r0 * a.xes);
+  const int e_range = (min(a.rows - r0, kBig) - 1) * (int)a.xes + (a.steps + 3) / 4 * 4;
+  uint32_t e4[8], e4n[8];
+  auto load_e4 = [&](int step) {
+    const auto b = __builtin_amdgcn_make_buffer_rsrc(ep, 0, e_range, 0x00027000);
+    const int row = 128 * wr + m;
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      e4n[t] = __builtin_amdgcn_raw_buffer_load_b32(
+          b, step < a.steps ? (row + 16 * t) * (int)a.xes + step : kPast, 0, 0);
+  };
+  float sc[4];
+
+  // operands from LDS
+  const uint8_t* sx0 = s_bytes + (128 * wr + m) * kStep + 16 * swizzle(m, g);
+  const uint8_t* sx1 = s_bytes + (128 * wr + m) * kStep + 16 * swizzle(m, 4 + g);
+  const uint8_t* sw0 = s_bytes + kStageX + wf * 4 * 2048 + 16 * lane;
+  auto read_x = [&](int step, int t) {
+    const int at = (step & 1) * 2 * kStageX + 16 * t * kStep;
+    return operand(*reinterpret_cast<const uint4*>(sx0 + at),
+                   *reinterpret_cast<const uint4*>(sx1 + at));
+  };
+  auto read_w = [&](int step, int f) {
+    const uint8_t* p = sw0 + (step & 1) * 2 * kStageX + 2048 * f;
+    return operand(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 1024));
+  };
+
+  f32x4_t acc[4][8], part[4];
+#pragma unroll
+  for (int f = 0; f < 4; ++f) {
+    part[f] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
+  }
+  load_e4(0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load(0, i);
+  step_barrier();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load(1, i);
+  i32x8_t x[2], w[4];
+  x[0] = read_x(0, 0);
+#pragma unroll
+  for (int f = 0; f < 4; ++f) w[f] = read_w(0, f);
+  float scale[4] = {0, 0, 0, 0};
+  // One step, in an order that the compiler keeps: 32 products, each added three products
+  // later. A row tile's operand is read one tile ahead. The barrier stands before the last
+  // row tile, when all of the step has been read: behind it the next step's first operands
+  // are read in place of the weights that have been used up, and the loads of the step after
+  // it go out into the stage that has become free.
+  auto one = [&](int step, auto quarter) {
+    constexpr int kQ = decltype(quarter)::value;
+    float before[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      before[f] = scale[f];
+      scale[f] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[f]), step & 63));
+    }
+    auto slot = [&](int i) {
+      const int t = i >> 2, f = i & 3, j = (i + 29) & 31;
+      part[f] = mfma<kQ>(w[f], x[t & 1], e4[t]);
+      acc[j & 3][j >> 2] += (i < 3 ? before[j & 3] : scale[j & 3]) * part[j & 3];
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < 28; ++i) {
+      if ((i & 3) == 0) x[((i >> 2) + 1) & 1] = read_x(kQ, (i >> 2) + 1);
+      slot(i);
+    }
+    step_barrier();
+    x[0] = read_x(kQ + 1, 0);
+#pragma unroll
+    for (int i = 28; i < 32; ++i) {
+      slot(i);
+      w[i & 3] = read_w(kQ + 1, i & 3);
+      load(step + 2, 2 * (i & 3));
+      load(step + 2, 2 * (i & 3) + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  for (int first = 0; first < a.steps; first += 64) {
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+      sc[f] = a.sc[(int64_t)tile_of(4 * wf + f) * a.steps + min(first + lane, a.steps - 1)];
+    // (here once, not among the loads in flight at every use)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    // four steps at a time; past the last one the rows are zeros, and so is their exponent
+    for (int step = first; step < min(first + 64, a.steps); step += 4) {
+      const int left = a.steps - step;
+      const uint32_t mask = left < 4 ? (1u << 8 * left) - 1 : ~0u;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) e4[t] = e4n[t] & mask;
+      load_e4(step + 4);
+      one(step, std::integral_constant<int, 0>());
+      one(step + 1, std::integral_constant<int, 1>());
+      one(step + 2, std::integral_constant<int, 2>());
+      one(step + 3, std::integral_constant<int, 3>());
+    }
+  }
+#pragma unroll
+  for (int j = 29; j < 32; ++j) acc[j & 3][j >> 2] += scale[j & 3] * part[j & 3];
+  __syncthreads();
+
+  if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
+    // the workgroup's 128 outputs of a row are one group: 32 of them in each of 4 waves
+    uint32_t* s_max = reinterpret_cast<uint32_t*>(s_all);  // [wf][row]
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const bool live = u0 + 2 * wf + f < a.units;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = live ? silu(acc[f][t][j]) * acc[f + 2][t][j] : 0.0f;
+          acc[f][t][j] = v;
+          most = max(most, finite_bits(v));
+        }
+      }
+      most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+      most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+      if (g == 0) s_max[wf * kBig + 128 * wr + 16 * t + m] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int in = 128 * wr + 16 * t + m, row = r0 + in;
+      if (row >= a.rows) continue;
+      uint32_t most = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) most = max(most, s_max[w * kBig + in]);
+      const uint32_t byte = scale_byte(most);
+      const float inv = scale_inverse(byte);
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const int n = (u0 + 2 * wf + f) * 16 + 4 * g;
+        const float v[4] = {acc[f][t][0], acc[f][t][1], acc[f][t][2], acc[f][t][3]};
+        if (n < a.N)
+          *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.y) + (int64_t)row * a.ys + n) =
+              codes4(v, inv);
+      }
+      if (wf == 0 && g == 0) a.ye[(int64_t)row * a.yes + u0 / 8] = (uint8_t)byte;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int row = r0 + 128 * wr + 16 * t + m;
+      if (row >= a.rows) continue;
+#pragma unroll
+      for (int f = 0; f < (kGate ? 2 : 4); ++f) {
+        const int n = (kGate ? u0 + 2 * wf + f : u0 + 4 * wf + f) * 16 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (n + j < a.N)
+            a.y[(int64_t)row * a.ys + n + j] =
+                result<kGate>(acc[f][t][j], kGate ? acc[f + 2][t][j] : 0.0f);
+        }
+      }
     }
   }
 }
@@ -187,6 +439,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_fp8_join(Fp8Args a) {
 constexpr int kCus = 256;
 
 struct Fp8Plan {
+  bool big;            // k_fp8_big
   int split_steps, nsplit;
   size_t part_bytes;   // sums of split steps
   size_t codes_bytes;  // codes of bf16 rows
@@ -201,7 +454,8 @@ Fp8Plan plan_of(int rows, int K, int N, int epilogue, bool bf16_rows) {
   const int steps = (K + kStep - 1) / kStep, units = (N + 15) / 16;
   p.nsplit = 1;
   p.split_steps = steps;
-  if (epilogue == HS_LINEAR_SWIGLU_FP8)
+  p.big = rows > 128;
+  if (epilogue == HS_LINEAR_SWIGLU_FP8 && !p.big)
     p.part_bytes = padded((size_t)p.nsplit * rows * units * 32 * sizeof(float));
   if (bf16_rows)
     p.codes_bytes = padded((size_t)rows * K) + padded((size_t)rows * scales_row(K));
@@ -222,6 +476,20 @@ void dispatch_rows(const Fp8Args& a, bool gate, hipStream_t s) {
   else if (a.units >= 12 * kCus) launch_rows<4, 4, false>(a, s);
   else if (a.units >= 4 * kCus) launch_rows<4, 2, false>(a, s);
   else launch_rows<8, 1, false>(a, s);
+}
+
+template <int kEpilogue>
+int launch_big(Fp8Args& a, hipStream_t s) {
+  constexpr int kBytes = 4 * kStageX;
+  a.cols = (a.units + (kEpilogue == HS_LINEAR_PLAIN ? 15 : 7)) / (kEpilogue == HS_LINEAR_PLAIN ? 16 : 8);
+  a.rowtiles = (a.rows + kBig - 1) / kBig;
+  static const hipError_t set = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(k_fp8_big<kEpilogue>),
+      hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  if (set != hipSuccess) return HS_ERR_LAUNCH;
+  hipLaunchKernelGGL((k_fp8_big<kEpilogue>), dim3((unsigned)(a.cols * a.rowtiles)),
+                     dim3(kBigThreads), kBytes, s, a);
+  return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 
 int join(const Fp8Args& a, int epilogue, hipStream_t s) {
@@ -318,6 +586,11 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.split_steps = p.split_steps;
   a.nsplit = p.nsplit;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (p.big) {
+    if (epilogue == HS_LINEAR_PLAIN) return launch_big<HS_LINEAR_PLAIN>(a, s);
+    if (epilogue == HS_LINEAR_SWIGLU) return launch_big<HS_LINEAR_SWIGLU>(a, s);
+    return launch_big<HS_LINEAR_SWIGLU_FP8>(a, s);
+  }
   dispatch_rows(a, gate, s);
   if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   return a.part ? join(a, epilogue, s) : HS_OK;
