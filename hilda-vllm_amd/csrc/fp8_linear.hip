@@ -48,6 +48,7 @@ struct Fp8Args {
   int up;             // first tile of the up rows (SwiGLU)
   uint16_t* y;        // bf16, or codes
   int64_t ys;
+  int wide;           // y and ys in 8-byte pieces
   uint8_t* ye;        // exponent bytes of the codes
   int64_t yes;
   float* part;        // [split][rows][tiles * 16]
@@ -68,6 +69,16 @@ __device__ __forceinline__ f32x4_t mfma(i32x8_t w, i32x8_t x, uint32_t xe) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, kOne, B, (int)xe);
 }
 
+__device__ __forceinline__ f32x4_t mfma(i32x8_t w, i32x8_t x) {
+  const f32x4_t zero = {0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+// the scale whose exponent is byte B of e
+template <int B>
+__device__ __forceinline__ float row_scale(uint32_t e) {
+  return __uint_as_float((e >> 8 * B & 255) << 23);
+}
+
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
   return make_uint4(v.x, v.y, v.z, v.w);
@@ -82,11 +93,27 @@ __device__ __forceinline__ uint4 load_x(const Fp8Args& a, int row, int step, int
   return v;
 }
 
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
+// (the reciprocal instruction is good to one unit in f32's last place)
+__device__ __forceinline__ float silu(float g) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+}
 
 template <bool kGate>
 __device__ __forceinline__ uint16_t result(float v, float up) {
   return to_bf(kGate ? silu(v) * up : v);
+}
+
+// 4 features of a row, n a multiple of 4; wide: outputs in 8-byte pieces
+__device__ __forceinline__ void store4(const Fp8Args& a, int64_t row, int n, const uint16_t (&v)[4]) {
+  uint16_t* y = a.y + row * a.ys + n;
+  if (a.wide && n + 4 <= a.N) {
+    *reinterpret_cast<uint2*>(y) = make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (n + j < a.N) y[j] = v[j];
+  }
 }
 
 // 16 rows a workgroup. W: its waves, which share out the steps of its TN weight tiles (with
@@ -149,15 +176,20 @@ constexpr int kBig = 256;                   // features and rows of a workgroup
 constexpr int kBigThreads = 512;            // 4 waves over the features, 2 over the rows
 constexpr int kPast = INT32_MAX;            // a byte offset past any buffer: reads zeros
 constexpr int kRange = INT32_MAX - 255;
-constexpr int kStageX = kBig * kStep;       // bytes of a step's rows, and of its weights
+constexpr int kStage = kBig * kStep;        // bytes of a step's rows, and of its weights
+// shared memory: two stages of rows, two of weights, two of the rows' exponents (four steps)
+constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kBigBytes = kAtE + 2 * 4 * kBig;
 
 // 16 bytes a lane from a buffer straight to LDS, at lds + 16 lane. The compiler does not see
 // the write: the wait before the barrier behind a step covers it. (Through the builtin it
-// would wait for the load before the next read of any shared memory.)
+// would wait for the load before the next read of any shared memory.) kOffset is added to
+// both sides.
+template <int kOffset = 0>
 __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, int offset, int at,
                                          uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :: "s"(lds), "v"(offset), "s"(from), "s"(at)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+               "buffer_load_dwordx4 %1, %2, %3 offen offset:%4 lds"
+               :: "s"(lds), "v"(offset), "s"(from), "s"(at), "n"(kOffset)
                : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
@@ -170,6 +202,9 @@ __device__ __forceinline__ void step_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+
+template <int I>
+using Index = std::integral_constant<int, I>;
 
 // the 16-byte piece of a row's step that lies at piece p of the row in LDS, and back
 __device__ __forceinline__ int swizzle(int row, int p) { return p ^ (row & 7); }
@@ -190,9 +225,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     const int id = blockIdx.x, x = id & 7, q = total >> 3, r = total & 7;
     const int o = x * q + min(x, r) + (id >> 3);
     const int group = o / (8 * a.cols), in = o % (8 * a.cols);
-    const int high = min(8, a.rowtiles - 8 * group);
-    r0 = (8 * group + in % high) * kBig;
-    u0 = in / high * (kGate ? 8 : 16);
+    const int tall = min(8, a.rowtiles - 8 * group);
+    r0 = (8 * group + in % tall) * kBig;
+    u0 = in / tall * (kGate ? 8 : 16);
   }
   auto tile_of = [&](int slot) {  // weight tile of one of the workgroup's 16 slots
     const int f = slot & 3;
@@ -201,58 +236,63 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   };
   // this wave's loads: 32 rows and two weight tiles
   const int piece = swizzle(lane >> 3, lane & 7);
-  int xo[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = 32 * wave + 8 * i + (lane >> 3);
-    xo[i] = r0 + row < a.rows ? row * (int)a.xs + 16 * piece : kPast;
-  }
   const int64_t tile_bytes = (int64_t)a.steps * (16 * kStep);
   uint8_t* wp = reinterpret_cast<uint8_t*>(const_cast<uint4*>(a.w));
   uint8_t* xp = const_cast<uint8_t*>(a.x + (int64_t)r0 * a.xs);
   uint8_t* wp0 = wp + tile_of(2 * wave) * tile_bytes;
   uint8_t* wp1 = wp + tile_of(2 * wave + 1) * tile_bytes;
+  const int high = min(a.rows - r0, kBig);  // rows of the tile
+  const int x_range = (high - 1) * (int)a.xs + a.K;  // rows behind the last one read zeros
+  const int row0 = 32 * wave + (lane >> 3);
   // load i of the eight that bring in a step; past the last step none reads memory
-  auto load = [&](int step, int i) {
-    const uint32_t to = lds + (step & 1) * 2 * kStageX;
-    const int range = step < a.steps ? kRange : 0;
-    if (i < 4) {
-      const auto b = __builtin_amdgcn_make_buffer_rsrc(xp, 0, range, 0x00027000);
-      const bool in = kStep * step + 16 * piece < a.K;
-      load_lds(b, in ? xo[i] : kPast, kStep * step, to + (32 * wave + 8 * i) * kStep);
+  auto load = [&](int step, auto index) {
+    constexpr int i = decltype(index)::value;
+    const uint32_t to = lds + (step & 1) * kStage;
+    if constexpr (i < 4) {
+      const auto b = __builtin_amdgcn_make_buffer_rsrc(xp, 0, x_range, 0x00027000);
+      const int k = kStep * step + 16 * piece;
+      const int at = (row0 + 8 * i) * (int)a.xs + k;
+      load_lds(b, k < a.K ? at : kPast, 0, to + (32 * wave + 8 * i) * kStep);
     } else {
-      const auto b = __builtin_amdgcn_make_buffer_rsrc(i < 6 ? wp0 : wp1, 0, range, 0x00027000);
-      load_lds(b, 16 * lane + 1024 * (i & 1), 16 * kStep * step,
-               to + kStageX + (wave * 4 + i - 4) * 1024);
+      const auto b = __builtin_amdgcn_make_buffer_rsrc(i < 6 ? wp0 : wp1, 0,
+                                                       step < a.steps ? kRange : 0, 0x00027000);
+      load_lds<1024 * (i & 1)>(b, 16 * lane, 16 * kStep * step,
+                               to + kAtW + (wave * 4 + i - 4) * 1024 - 1024 * (i & 1));
     }
   };
-  // exponents of this lane's 8 rows, four steps a word, and scales of the wave's 4 tiles,
-  // a step a lane
-  uint8_t* ep = const_cast<uint8_t*>(a.xe + (int64_t)r0 * a.xes);
-  const int e_range = (min(a.rows - r0, kBig) - 1) * (int)a.xes + (a.steps + 3) / 4 * 4;
-  uint32_t e4[8], e4n[8];
-  auto load_e4 = [&](int step) {
-    const auto b = __builtin_amdgcn_make_buffer_rsrc(ep, 0, e_range, 0x00027000);
-    const int row = 128 * wr + m;
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-      e4n[t] = __builtin_amdgcn_raw_buffer_load_b32(
-          b, step < a.steps ? (row + 16 * t) * (int)a.xes + step : kPast, 0, 0);
+  auto load_all = [&](int step) {
+    load(step, Index<0>()); load(step, Index<1>()); load(step, Index<2>()); load(step, Index<3>());
+    load(step, Index<4>()); load(step, Index<5>()); load(step, Index<6>()); load(step, Index<7>());
   };
-  float sc[4];
+  // the rows' exponents of four steps, a word a row
+  uint8_t* ep = const_cast<uint8_t*>(a.xe + (int64_t)r0 * a.xes);
+  const int e_row = min((int)threadIdx.x & (kBig - 1), high - 1) * (int)a.xes;
+  uint32_t ew;
+  auto load_e = [&](int step) {
+    ew = *reinterpret_cast<const uint32_t*>(ep + (e_row + min(step, a.steps - 1 & ~3)));
+  };
+  auto write_e = [&](int quad) {
+    *reinterpret_cast<uint32_t*>(s_bytes + kAtE + (quad & 1) * 4 * kBig +
+                                 4 * ((int)threadIdx.x & (kBig - 1))) = ew;
+  };
+  float sc[4];  // the scales of the wave's tiles, a step a lane
 
   // operands from LDS
   const uint8_t* sx0 = s_bytes + (128 * wr + m) * kStep + 16 * swizzle(m, g);
   const uint8_t* sx1 = s_bytes + (128 * wr + m) * kStep + 16 * swizzle(m, 4 + g);
-  const uint8_t* sw0 = s_bytes + kStageX + wf * 4 * 2048 + 16 * lane;
+  const uint8_t* sw0 = s_bytes + kAtW + wf * 4 * 2048 + 16 * lane;
+  const uint8_t* se0 = s_bytes + kAtE + 4 * (128 * wr + m);
   auto read_x = [&](int step, int t) {
-    const int at = (step & 1) * 2 * kStageX + 16 * t * kStep;
+    const int at = (step & 1) * kStage + 16 * t * kStep;
     return operand(*reinterpret_cast<const uint4*>(sx0 + at),
                    *reinterpret_cast<const uint4*>(sx1 + at));
   };
   auto read_w = [&](int step, int f) {
-    const uint8_t* p = sw0 + (step & 1) * 2 * kStageX + 2048 * f;
+    const uint8_t* p = sw0 + (step & 1) * kStage + 2048 * f;
     return operand(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 1024));
+  };
+  auto read_e = [&](int quad, int t) {
+    return *reinterpret_cast<const uint32_t*>(se0 + (quad & 1) * 4 * kBig + 64 * t);
   };
 
   f32x4_t acc[4][8], part[4];
@@ -262,51 +302,64 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
 #pragma unroll
     for (int t = 0; t < 8; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
   }
-  load_e4(0);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) load(0, i);
+  load_e(0);
+  write_e(0);
+  load_all(0);
   step_barrier();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) load(1, i);
+  load_all(1);
   i32x8_t x[2], w[4];
+  uint32_t e[2];
   x[0] = read_x(0, 0);
+  e[0] = read_e(0, 0);
 #pragma unroll
   for (int f = 0; f < 4; ++f) w[f] = read_w(0, f);
-  float scale[4] = {0, 0, 0, 0};
+  float factor[2][4] = {};  // of the products, by row tile parity and weight tile
   // One step, in an order that the compiler keeps: 32 products, each added three products
   // later. A row tile's operand is read one tile ahead. The barrier stands before the last
   // row tile, when all of the step has been read: behind it the next step's first operands
   // are read in place of the weights that have been used up, and the loads of the step after
   // it go out into the stage that has become free.
-  auto one = [&](int step, auto quarter) {
+  auto one = [&](int step, uint32_t mask, auto quarter) {
     constexpr int kQ = decltype(quarter)::value;
-    float before[4];
+    const int quad = step >> 2;
+    float row, scale[4];
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      before[f] = scale[f];
+    for (int f = 0; f < 4; ++f)
       scale[f] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[f]), step & 63));
-    }
+    if (kQ == 0) load_e(step + 4);
+    if (kQ == 1) write_e(quad + 1);
     auto slot = [&](int i) {
       const int t = i >> 2, f = i & 3, j = (i + 29) & 31;
-      part[f] = mfma<kQ>(w[f], x[t & 1], e4[t]);
-      acc[j & 3][j >> 2] += (i < 3 ? before[j & 3] : scale[j & 3]) * part[j & 3];
+      part[f] = mfma(w[f], x[t & 1]);
+      if (f == 0) row = row_scale<kQ>(e[t & 1] & mask);
+      // (a pair of tiles of one half is in one block of the weight)
+      factor[t & 1][f] = f == 0 || (kGate && f >= 2) ? row * scale[f] : factor[t & 1][f - 1];
+      acc[j & 3][j >> 2] += factor[(j >> 2) & 1][j & 3] * part[j & 3];
       __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int i = 0; i < 28; ++i) {
-      if ((i & 3) == 0) x[((i >> 2) + 1) & 1] = read_x(kQ, (i >> 2) + 1);
+      if ((i & 3) == 0) {
+        x[((i >> 2) + 1) & 1] = read_x(kQ, (i >> 2) + 1);
+        e[((i >> 2) + 1) & 1] = read_e(quad, (i >> 2) + 1);
+      }
       slot(i);
     }
     step_barrier();
     x[0] = read_x(kQ + 1, 0);
-#pragma unroll
-    for (int i = 28; i < 32; ++i) {
-      slot(i);
-      w[i & 3] = read_w(kQ + 1, i & 3);
-      load(step + 2, 2 * (i & 3));
-      load(step + 2, 2 * (i & 3) + 1);
+    e[0] = read_e(quad + (kQ == 3), 0);
+    auto last = [&](auto index) {
+      constexpr int f = decltype(index)::value;
+      slot(28 + f);
+      w[f] = read_w(kQ + 1, f);
+      load(step + 2, Index<2 * f>());
+      load(step + 2, Index<2 * f + 1>());
       __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    last(Index<0>());
+    last(Index<1>());
+    last(Index<2>());
+    last(Index<3>());
   };
   for (int first = 0; first < a.steps; first += 64) {
 #pragma unroll
@@ -319,18 +372,15 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     for (int step = first; step < min(first + 64, a.steps); step += 4) {
       const int left = a.steps - step;
       const uint32_t mask = left < 4 ? (1u << 8 * left) - 1 : ~0u;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) e4[t] = e4n[t] & mask;
-      load_e4(step + 4);
-      one(step, std::integral_constant<int, 0>());
-      one(step + 1, std::integral_constant<int, 1>());
-      one(step + 2, std::integral_constant<int, 2>());
-      one(step + 3, std::integral_constant<int, 3>());
+      one(step, mask, Index<0>());
+      one(step + 1, mask, Index<1>());
+      one(step + 2, mask, Index<2>());
+      one(step + 3, mask, Index<3>());
     }
   }
 #pragma unroll
-  for (int j = 29; j < 32; ++j) acc[j & 3][j >> 2] += scale[j & 3] * part[j & 3];
-  __syncthreads();
+  for (int j = 29; j < 32; ++j) acc[j & 3][j >> 2] += factor[1][j & 3] * part[j & 3];
+  step_barrier();  // the last loads, which bring zeros, have landed
 
   if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
     // the workgroup's 128 outputs of a row are one group: 32 of them in each of 4 waves
@@ -380,12 +430,11 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
 #pragma unroll
       for (int f = 0; f < (kGate ? 2 : 4); ++f) {
         const int n = (kGate ? u0 + 2 * wf + f : u0 + 4 * wf + f) * 16 + 4 * g;
+        uint16_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (n + j < a.N)
-            a.y[(int64_t)row * a.ys + n + j] =
-                result<kGate>(acc[f][t][j], kGate ? acc[f + 2][t][j] : 0.0f);
-        }
+        for (int j = 0; j < 4; ++j)
+          v[j] = result<kGate>(acc[f][t][j], kGate ? acc[f + 2][t][j] : 0.0f);
+        store4(a, row, n, v);
       }
     }
   }
@@ -480,15 +529,14 @@ void dispatch_rows(const Fp8Args& a, bool gate, hipStream_t s) {
 
 template <int kEpilogue>
 int launch_big(Fp8Args& a, hipStream_t s) {
-  constexpr int kBytes = 4 * kStageX;
   a.cols = (a.units + (kEpilogue == HS_LINEAR_PLAIN ? 15 : 7)) / (kEpilogue == HS_LINEAR_PLAIN ? 16 : 8);
   a.rowtiles = (a.rows + kBig - 1) / kBig;
   static const hipError_t set = hipFuncSetAttribute(
       reinterpret_cast<const void*>(k_fp8_big<kEpilogue>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+      hipFuncAttributeMaxDynamicSharedMemorySize, kBigBytes);
   if (set != hipSuccess) return HS_ERR_LAUNCH;
   hipLaunchKernelGGL((k_fp8_big<kEpilogue>), dim3((unsigned)(a.cols * a.rowtiles)),
-                     dim3(kBigThreads), kBytes, s, a);
+                     dim3(kBigThreads), kBigBytes, s, a);
   return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
 }
 
@@ -580,6 +628,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.up = a.units;
   a.y = static_cast<uint16_t*>(out);
   a.ys = out_stride;
+  a.wide = !((uintptr_t)out & 7) && out_stride % 4 == 0;
   a.ye = static_cast<uint8_t*>(out_scales);
   a.yes = out_scales_stride;
   a.part = p.part_bytes ? reinterpret_cast<float*>(ws) : nullptr;
