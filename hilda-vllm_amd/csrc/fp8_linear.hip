@@ -48,7 +48,7 @@ struct Fp8Args {
   int up;             // first tile of the up rows (SwiGLU)
   uint16_t* y;        // bf16, or codes
   int64_t ys;
-  int wide;           // y and ys in 8-byte pieces
+  int wide;           // y and ys in 16-byte pieces
   uint8_t* ye;        // exponent bytes of the codes
   int64_t yes;
   float* part;        // [split][rows][tiles * 16]
@@ -103,16 +103,18 @@ __device__ __forceinline__ uint16_t result(float v, float up) {
   return to_bf(kGate ? silu(v) * up : v);
 }
 
-// 4 features of a row, n a multiple of 4; wide: outputs in 8-byte pieces
-__device__ __forceinline__ void store4(const Fp8Args& a, int64_t row, int n, const uint16_t (&v)[4]) {
+// 8 features of a row, n a multiple of 8; wide: outputs in 16-byte pieces
+__device__ __forceinline__ void store8(const Fp8Args& a, int64_t row, int n, uint4 v) {
   uint16_t* y = a.y + row * a.ys + n;
-  if (a.wide && n + 4 <= a.N) {
-    *reinterpret_cast<uint2*>(y) = make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+  if (a.wide && n + 8 <= a.N) {
+    *reinterpret_cast<uint4*>(y) = v;
     return;
   }
+  uint16_t h[8];
+  unpack8(v, h);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (n + j < a.N) y[j] = v[j];
+  for (int j = 0; j < 8; ++j) {
+    if (n + j < a.N) y[j] = h[j];
   }
 }
 
@@ -177,8 +179,11 @@ constexpr int kBigThreads = 512;            // 4 waves over the features, 2 over
 constexpr int kPast = INT32_MAX;            // a byte offset past any buffer: reads zeros
 constexpr int kRange = INT32_MAX - 255;
 constexpr int kStage = kBig * kStep;        // bytes of a step's rows, and of its weights
-// shared memory: two stages of rows, two of weights, two of the rows' exponents (four steps)
-constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kBigBytes = kAtE + 2 * 4 * kBig;
+constexpr int kChunk = 64;                  // steps whose exponents and scales are held
+// shared memory: two stages of rows, two of weights, the chunk's exponents [four steps][row]
+// and whether a row has one that is NaN
+constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kAtBad = kAtE + kChunk * kBig;
+constexpr int kBigBytes = kAtBad + 4 * kBig;
 
 // 16 bytes a lane from a buffer straight to LDS, at lds + 16 lane. The compiler does not see
 // the write: the wait before the barrier behind a step covers it. (Through the builtin it
@@ -195,10 +200,11 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, int offset
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
-// waits for the wave's loads and LDS traffic, then for the other waves
+// waits for the wave's LDS traffic and all but its last kLoads loads, then for the other waves
+template <int kLoads>
 __device__ __forceinline__ void step_barrier() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0070 | kLoads);  // vmcnt(kLoads) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -243,38 +249,31 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   uint8_t* wp1 = wp + tile_of(2 * wave + 1) * tile_bytes;
   const int high = min(a.rows - r0, kBig);  // rows of the tile
   const int x_range = (high - 1) * (int)a.xs + a.K;  // rows behind the last one read zeros
-  const int row0 = 32 * wave + (lane >> 3);
-  // load i of the eight that bring in a step; past the last step none reads memory
+  // A wave's eight loads of a step: i 0 and 1 the lower 64 rows of each half, 2 to 5 weights
+  // (group A), 6 and 7 the upper rows (group B). Past the last step none reads memory.
+  const int row0 = (wave >> 2) * 128 + (wave & 3) * 16 + (lane >> 3);
   auto load = [&](int step, auto index) {
     constexpr int i = decltype(index)::value;
     const uint32_t to = lds + (step & 1) * kStage;
-    if constexpr (i < 4) {
+    if constexpr (i < 2 || i >= 6) {
+      constexpr int kRow = i < 2 ? 8 * i : 64 + 8 * (i - 6);
       const auto b = __builtin_amdgcn_make_buffer_rsrc(xp, 0, x_range, 0x00027000);
       const int k = kStep * step + 16 * piece;
-      const int at = (row0 + 8 * i) * (int)a.xs + k;
-      load_lds(b, k < a.K ? at : kPast, 0, to + (32 * wave + 8 * i) * kStep);
+      const int at = (row0 + kRow) * (int)a.xs + k;
+      load_lds(b, k < a.K ? at : kPast, 0,
+               to + ((wave >> 2) * 128 + (wave & 3) * 16 + kRow) * kStep);
     } else {
-      const auto b = __builtin_amdgcn_make_buffer_rsrc(i < 6 ? wp0 : wp1, 0,
+      const auto b = __builtin_amdgcn_make_buffer_rsrc(i < 4 ? wp0 : wp1, 0,
                                                        step < a.steps ? kRange : 0, 0x00027000);
       load_lds<1024 * (i & 1)>(b, 16 * lane, 16 * kStep * step,
-                               to + kAtW + (wave * 4 + i - 4) * 1024 - 1024 * (i & 1));
+                               to + kAtW + (wave * 4 + (i & 2 ? 0 : 2)) * 1024);
     }
   };
-  auto load_all = [&](int step) {
+  auto load_a = [&](int step) {
     load(step, Index<0>()); load(step, Index<1>()); load(step, Index<2>()); load(step, Index<3>());
-    load(step, Index<4>()); load(step, Index<5>()); load(step, Index<6>()); load(step, Index<7>());
+    load(step, Index<4>()); load(step, Index<5>());
   };
-  // the rows' exponents of four steps, a word a row
-  uint8_t* ep = const_cast<uint8_t*>(a.xe + (int64_t)r0 * a.xes);
-  const int e_row = min((int)threadIdx.x & (kBig - 1), high - 1) * (int)a.xes;
-  uint32_t ew;
-  auto load_e = [&](int step) {
-    ew = *reinterpret_cast<const uint32_t*>(ep + (e_row + min(step, a.steps - 1 & ~3)));
-  };
-  auto write_e = [&](int quad) {
-    *reinterpret_cast<uint32_t*>(s_bytes + kAtE + (quad & 1) * 4 * kBig +
-                                 4 * ((int)threadIdx.x & (kBig - 1))) = ew;
-  };
+  auto load_b = [&](int step) { load(step, Index<6>()); load(step, Index<7>()); };
   float sc[4];  // the scales of the wave's tiles, a step a lane
 
   // operands from LDS
@@ -292,7 +291,7 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     return operand(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 1024));
   };
   auto read_e = [&](int quad, int t) {
-    return *reinterpret_cast<const uint32_t*>(se0 + (quad & 1) * 4 * kBig + 64 * t);
+    return *reinterpret_cast<const uint32_t*>(se0 + quad * 4 * kBig + 64 * t);
   };
 
   f32x4_t acc[4][8], part[4];
@@ -302,92 +301,163 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
 #pragma unroll
     for (int t = 0; t < 8; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
   }
-  load_e(0);
-  write_e(0);
-  load_all(0);
-  step_barrier();
-  load_all(1);
-  i32x8_t x[2], w[4];
-  uint32_t e[2];
-  x[0] = read_x(0, 0);
-  e[0] = read_e(0, 0);
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_bytes + kAtBad);
+  if (threadIdx.x < kBig) s_bad[threadIdx.x] = 0;
+  // the chunk's exponents and scales: half of a row's words a thread
+  auto load_chunk = [&](int first) {
+    const int row = threadIdx.x & (kBig - 1), q0 = (int)(threadIdx.x >> 8) * (kChunk / 8);
+    const uint8_t* from = a.xe + (r0 + min(row, high - 1)) * a.xes + first;
+    uint32_t word[kChunk / 8];
 #pragma unroll
-  for (int f = 0; f < 4; ++f) w[f] = read_w(0, f);
-  float factor[2][4] = {};  // of the products, by row tile parity and weight tile
-  // One step, in an order that the compiler keeps: 32 products, each added three products
-  // later. A row tile's operand is read one tile ahead. The barrier stands before the last
-  // row tile, when all of the step has been read: behind it the next step's first operands
-  // are read in place of the weights that have been used up, and the loads of the step after
-  // it go out into the stage that has become free.
-  auto one = [&](int step, uint32_t mask, auto quarter) {
-    constexpr int kQ = decltype(quarter)::value;
-    const int quad = step >> 2;
-    float row, scale[4];
-#pragma unroll
-    for (int f = 0; f < 4; ++f)
-      scale[f] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[f]), step & 63));
-    if (kQ == 0) load_e(step + 4);
-    if (kQ == 1) write_e(quad + 1);
-    auto slot = [&](int i) {
-      const int t = i >> 2, f = i & 3, j = (i + 29) & 31;
-      part[f] = mfma(w[f], x[t & 1]);
-      if (f == 0) row = row_scale<kQ>(e[t & 1] & mask);
-      // (a pair of tiles of one half is in one block of the weight)
-      factor[t & 1][f] = f == 0 || (kGate && f >= 2) ? row * scale[f] : factor[t & 1][f - 1];
-      acc[j & 3][j >> 2] += factor[(j >> 2) & 1][j & 3] * part[j & 3];
-      __builtin_amdgcn_sched_barrier(0);
-    };
-#pragma unroll
-    for (int i = 0; i < 28; ++i) {
-      if ((i & 3) == 0) {
-        x[((i >> 2) + 1) & 1] = read_x(kQ, (i >> 2) + 1);
-        e[((i >> 2) + 1) & 1] = read_e(quad, (i >> 2) + 1);
-      }
-      slot(i);
+    for (int i = 0; i < kChunk / 8; ++i) {
+      const int at = 4 * (q0 + i), left = a.steps - first - at;  // (past the last step: zeros)
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(
+          from + min(at, (a.steps - 1 - first) & ~3));
+      word[i] = left >= 4 ? v : left > 0 ? v & ((1u << 8 * left) - 1) : 0;
     }
-    step_barrier();
-    x[0] = read_x(kQ + 1, 0);
-    e[0] = read_e(quad + (kQ == 3), 0);
-    auto last = [&](auto index) {
-      constexpr int f = decltype(index)::value;
-      slot(28 + f);
-      w[f] = read_w(kQ + 1, f);
-      load(step + 2, Index<2 * f>());
-      load(step + 2, Index<2 * f + 1>());
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    last(Index<0>());
-    last(Index<1>());
-    last(Index<2>());
-    last(Index<3>());
-  };
-  for (int first = 0; first < a.steps; first += 64) {
 #pragma unroll
     for (int f = 0; f < 4; ++f)
       sc[f] = a.sc[(int64_t)tile_of(4 * wf + f) * a.steps + min(first + lane, a.steps - 1)];
-    // (here once, not among the loads in flight at every use)
+    // (waited for here, not at every use among the loads in flight)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    // four steps at a time; past the last one the rows are zeros, and so is their exponent
-    for (int step = first; step < min(first + 64, a.steps); step += 4) {
-      const int left = a.steps - step;
-      const uint32_t mask = left < 4 ? (1u << 8 * left) - 1 : ~0u;
-      one(step, mask, Index<0>());
-      one(step + 1, mask, Index<1>());
-      one(step + 2, mask, Index<2>());
-      one(step + 3, mask, Index<3>());
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < kChunk / 8; ++i) {
+      *reinterpret_cast<uint32_t*>(s_bytes + kAtE + (q0 + i) * 4 * kBig + 4 * row) = word[i];
+      // a byte of ones: its low seven bits carry into the eighth, which is set
+      bad |= ((word[i] & 0x7f7f7f7fu) + 0x01010101u) & word[i] & 0x80808080u;
+    }
+    return bad;
+  };
+  load_a(0);
+  load_b(0);
+  load_a(1);
+  load_b(1);
+  uint32_t bad = load_chunk(0);
+  step_barrier<0>();
+  i32x8_t x[3], w[4];
+  uint32_t e[3];
+  x[2] = read_x(0, 0);
+#pragma unroll
+  for (int f = 0; f < 4; ++f) w[f] = read_w(0, f);
+  float factor[3][4] = {};  // of the products, by row tile's register and weight tile
+  // One step, in an order that the compiler keeps: 32 products, each added three products
+  // later; a row tile's operand is read one tile ahead. At the first barrier the lower rows
+  // and the weights of the step have been read (by all waves): the step after the next loads
+  // into their place (group A). At the second the upper rows have been, too (group B): the
+  // next step's first operands are read in place of those used up. What a barrier waits for
+  // was loaded one and a half steps before.
+  auto one = [&](int step, int quad, auto quarter) {
+    constexpr int kQ = decltype(quarter)::value;
+    constexpr int kReg[8] = {2, 0, 1, 0, 1, 2, 0, 1};  // of the row tiles
+    float row, scale[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+      scale[f] = __uint_as_float(
+          __builtin_amdgcn_readlane(__float_as_uint(sc[f]), step & (kChunk - 1)));
+    // tile and weight of product i: the last two row tiles by weights
+    auto tile = [](int i) { return i < 24 ? i >> 2 : 6 + (i & 1); };
+    auto weight = [](int i) { return i < 24 ? i & 3 : (i - 24) >> 1; };
+    auto read = [&](int t) {
+      x[kReg[t]] = read_x(kQ, t);
+      e[kReg[t]] = read_e(quad, t);
+    };
+    auto product = [&](int i) {
+      const int t = tile(i), f = weight(i), r = kReg[t];
+      part[i & 3] = mfma(w[f], x[r]);
+      if (f == 0) row = row_scale<kQ>(e[r]);
+      // (a pair of tiles of one half is in one block of the weight)
+      if (f == 0) {
+        factor[r][0] = row * scale[0];
+        factor[r][1] = factor[r][0];
+        factor[r][2] = kGate ? row * scale[2] : factor[r][0];
+        factor[r][3] = kGate ? row * scale[3] : factor[r][0];
+      }
+      const int j = (i + 29) & 31, tj = tile(j), fj = weight(j);
+      acc[fj][tj] += factor[kReg[tj]][fj] * part[j & 3];
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < 12; ++i) {
+      if ((i & 3) == 0) read((i >> 2) + 1);
+      product(i);
+    }
+    step_barrier<8>();
+    auto middle = [&](auto index) {
+      constexpr int i = decltype(index)::value;
+      if (i == 12) read(4);
+      if (i == 16) read(5);
+      if (i == 20) {
+        read(6);
+        read(7);
+      }
+      product(i);
+      if constexpr (i < 18) {
+        load(step + 2, Index<i - 12>());
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    middle(Index<12>()); middle(Index<13>()); middle(Index<14>()); middle(Index<15>());
+    middle(Index<16>()); middle(Index<17>()); middle(Index<18>()); middle(Index<19>());
+    middle(Index<20>()); middle(Index<21>()); middle(Index<22>()); middle(Index<23>());
+    step_barrier<8>();
+    x[2] = read_x(kQ + 1, 0);
+    e[2] = read_e((quad + (kQ == 3)) & (kChunk / 4 - 1), 0);
+#pragma unroll
+    for (int i = 24; i < 32; ++i) {
+      product(i);
+      if (i & 1) w[weight(i)] = read_w(kQ + 1, weight(i));
+      if (i == 25) load(step + 2, Index<6>());
+      if (i == 27) load(step + 2, Index<7>());
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  for (int first = 0; first < a.steps; first += kChunk) {
+    if (first) {
+      step_barrier<0>();  // the last chunk's exponents have been read
+      bad |= load_chunk(first);
+      step_barrier<0>();
+    }
+    e[2] = read_e(0, 0);
+    // four steps at a time; past the last one the rows are zeros, and so is their scale
+    const int until = min(first + kChunk, a.steps);
+    for (int step = first; step < until; step += 4) {
+      const int quad = (step & (kChunk - 1)) >> 2;
+      one(step, quad, Index<0>());
+      one(step + 1, quad, Index<1>());
+      one(step + 2, quad, Index<2>());
+      one(step + 3, quad, Index<3>());
     }
   }
 #pragma unroll
-  for (int j = 29; j < 32; ++j) acc[j & 3][j >> 2] += factor[1][j & 3] * part[j & 3];
-  step_barrier();  // the last loads, which bring zeros, have landed
+  for (int j = 29; j < 32; ++j)
+    acc[(j - 24) >> 1][6 + (j & 1)] += factor[j & 1][(j - 24) >> 1] * part[j & 3];
+  if (bad) s_bad[threadIdx.x & (kBig - 1)] = 1;
+  step_barrier<0>();  // the last loads, which bring zeros, have landed
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    if (s_bad[128 * wr + 16 * t + m]) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[f][t][j] = __builtin_nanf("");
+    }
+  }
 
+
+  // Through shared memory, so that whole lines go out: rows of kRow bytes and a pad
+  constexpr int kRow = kEpilogue == HS_LINEAR_PLAIN ? 2 * kBig : kGate && kEpilogue == HS_LINEAR_SWIGLU ? kBig : kBig / 2;
+  constexpr int kPitch = kRow + 16;
+  static_assert(kBig * kPitch <= kAtBad, "");
+  uint8_t* s_out = s_bytes;
+  uint32_t bytes[8];  // exponents of the rows' codes
   if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
     // the workgroup's 128 outputs of a row are one group: 32 of them in each of 4 waves
-    uint32_t* s_max = reinterpret_cast<uint32_t*>(s_all);  // [wf][row]
+    uint32_t* s_max = reinterpret_cast<uint32_t*>(s_bytes + kBig * kPitch);  // [wf][row]
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      uint32_t most = 0;
+      float most = 0;
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const bool live = u0 + 2 * wf + f < a.units;
@@ -395,46 +465,75 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
         for (int j = 0; j < 4; ++j) {
           const float v = live ? silu(acc[f][t][j]) * acc[f + 2][t][j] : 0.0f;
           acc[f][t][j] = v;
-          most = max(most, finite_bits(v));
+          most = fmaxf(most, fabsf(v));  // (passes over NaN)
         }
       }
-      most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
-      most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
-      if (g == 0) s_max[wf * kBig + 128 * wr + 16 * t + m] = most;
+      if (__any(most == __builtin_inff())) {  // the scale is that of the finite values
+        uint32_t bits = 0;
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            bits = max(bits, finite_bits(acc[f][t][j]));
+            acc[f][t][j] = nan_unless_finite(acc[f][t][j]);
+          }
+        most = __uint_as_float(bits);
+      }
+      most = quad_max(most);
+      if (g == 0) s_max[wf * kBig + 128 * wr + 16 * t + m] = __float_as_uint(most);
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const int in = 128 * wr + 16 * t + m, row = r0 + in;
-      if (row >= a.rows) continue;
       uint32_t most = 0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) most = max(most, s_max[w * kBig + in]);
-      const uint32_t byte = scale_byte(most);
-      const float inv = scale_inverse(byte);
+      for (int w = 0; w < 4; ++w) most = max(most, s_max[w * kBig + 128 * wr + 16 * t + m]);
+      bytes[t] = scale_byte(most);
+      const float inv = scale_inverse(bytes[t]);
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const int n = (u0 + 2 * wf + f) * 16 + 4 * g;
         const float v[4] = {acc[f][t][0], acc[f][t][1], acc[f][t][2], acc[f][t][3]};
-        if (n < a.N)
-          *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.y) + (int64_t)row * a.ys + n) =
-              codes4(v, inv);
+        *reinterpret_cast<uint32_t*>(s_out + (128 * wr + 16 * t + m) * kPitch + 32 * wf + 16 * f +
+                                     4 * g) = finite_codes4(v, inv);
       }
-      if (wf == 0 && g == 0) a.ye[(int64_t)row * a.yes + u0 / 8] = (uint8_t)byte;
     }
   } else {
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const int row = r0 + 128 * wr + 16 * t + m;
-      if (row >= a.rows) continue;
 #pragma unroll
       for (int f = 0; f < (kGate ? 2 : 4); ++f) {
-        const int n = (kGate ? u0 + 2 * wf + f : u0 + 4 * wf + f) * 16 + 4 * g;
         uint16_t v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           v[j] = result<kGate>(acc[f][t][j], kGate ? acc[f + 2][t][j] : 0.0f);
-        store4(a, row, n, v);
+        *reinterpret_cast<uint2*>(s_out + (128 * wr + 16 * t + m) * kPitch +
+                                  (kGate ? 64 : 128) * wf + 32 * f + 8 * g) =
+            make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int kLanes = kRow / 16;  // of a row
+#pragma unroll
+  for (int i = 0; i < 32 * kLanes / 64; ++i) {
+    const int in = 32 * wave + (64 * i + lane) / kLanes, at = lane % kLanes;
+    const int64_t row = r0 + in;
+    if (in >= high) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(s_out + in * kPitch + 16 * at);
+    if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
+      const int n = 16 * (u0 + at);
+      if (n < a.N)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + row * a.ys + n) = v;
+    } else {
+      store8(a, row, 16 * u0 + 8 * at, v);
+    }
+  }
+  if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
+    if (wf == 0 && g == 0) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int in = 128 * wr + 16 * t + m;
+        if (in < high) a.ye[(int64_t)(r0 + in) * a.yes + u0 / 8] = (uint8_t)bytes[t];
       }
     }
   }
@@ -628,7 +727,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.up = a.units;
   a.y = static_cast<uint16_t*>(out);
   a.ys = out_stride;
-  a.wide = !((uintptr_t)out & 7) && out_stride % 4 == 0;
+  a.wide = !((uintptr_t)out & 15) && out_stride % 8 == 0;
   a.ye = static_cast<uint8_t*>(out_scales);
   a.yes = out_scales_stride;
   a.part = p.part_bytes ? reinterpret_cast<float*>(ws) : nullptr;

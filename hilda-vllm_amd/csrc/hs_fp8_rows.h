@@ -39,6 +39,22 @@ __device__ __forceinline__ float nan_unless_finite(float v) {
   return fabsf(v) < __builtin_inff() ? v : __builtin_nanf("");
 }
 
+// codes of four values that are finite or NaN
+__device__ __forceinline__ uint32_t finite_codes4(const float* v, float inv) {
+  int w = 0;
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
+  return (uint32_t)w;
+}
+
+// the largest of the lanes l, l ^ 16, l ^ 32 and l ^ 48
+__device__ __forceinline__ float quad_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // codes of four values (v_cvt_pk_fp8_f32: round to nearest even; finite |v / s| <= 448)
 __device__ __forceinline__ uint32_t codes4(const float* v, float inv) {
   int w = 0;
