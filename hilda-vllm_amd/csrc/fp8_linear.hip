@@ -435,17 +435,18 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     acc[(j - 24) >> 1][6 + (j & 1)] += factor[j & 1][(j - 24) >> 1] * part[j & 3];
   if (bad) s_bad[threadIdx.x & (kBig - 1)] = 1;
   step_barrier<0>();  // the last loads, which bring zeros, have landed
+  uint32_t nan_rows = 0;
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    if (s_bad[128 * wr + 16 * t + m]) {
+  for (int t = 0; t < 8; ++t) nan_rows |= s_bad[128 * wr + 16 * t + m] << t;
+  if (__any(nan_rows)) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
 #pragma unroll
       for (int f = 0; f < 4; ++f)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[f][t][j] = __builtin_nanf("");
-    }
+        for (int j = 0; j < 4; ++j)
+          acc[f][t][j] = nan_rows >> t & 1 ? __builtin_nanf("") : acc[f][t][j];
   }
-
-
   // Through shared memory, so that whole lines go out: rows of kRow bytes and a pad
   constexpr int kRow = kEpilogue == HS_LINEAR_PLAIN ? 2 * kBig : kGate && kEpilogue == HS_LINEAR_SWIGLU ? kBig : kBig / 2;
   constexpr int kPitch = kRow + 16;
@@ -460,13 +461,13 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
       float most = 0;
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const bool live = u0 + 2 * wf + f < a.units;
+        float here = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float v = live ? silu(acc[f][t][j]) * acc[f + 2][t][j] : 0.0f;
-          acc[f][t][j] = v;
-          most = fmaxf(most, fabsf(v));  // (passes over NaN)
+          acc[f][t][j] = silu(acc[f][t][j]) * acc[f + 2][t][j];
+          here = fmaxf(here, fabsf(acc[f][t][j]));  // (passes over NaN)
         }
+        most = fmaxf(most, u0 + 2 * wf + f < a.units ? here : 0.0f);
       }
       if (__any(most == __builtin_inff())) {  // the scale is that of the finite values
         uint32_t bits = 0;
