@@ -69,16 +69,6 @@ __device__ __forceinline__ f32x4_t mfma(i32x8_t w, i32x8_t x, uint32_t xe) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, kOne, B, (int)xe);
 }
 
-__device__ __forceinline__ f32x4_t mfma(i32x8_t w, i32x8_t x) {
-  const f32x4_t zero = {0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
-}
-// the scale whose exponent is byte B of e
-template <int B>
-__device__ __forceinline__ float row_scale(uint32_t e) {
-  return __uint_as_float((e >> 8 * B & 255) << 23);
-}
-
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
   const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
   return make_uint4(v.x, v.y, v.z, v.w);
@@ -181,9 +171,7 @@ constexpr int kRange = INT32_MAX - 255;
 constexpr int kStage = kBig * kStep;        // bytes of a step's rows, and of its weights
 constexpr int kChunk = 64;                  // steps whose exponents and scales are held
 // shared memory: two stages of rows, two of weights, the chunk's exponents [four steps][row]
-// and whether a row has one that is NaN
-constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kAtBad = kAtE + kChunk * kBig;
-constexpr int kBigBytes = kAtBad + 4 * kBig;
+constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kBigBytes = kAtE + kChunk * kBig;
 
 // 16 bytes a lane from a buffer straight to LDS, at lds + 16 lane. The compiler does not see
 // the write: the wait before the barrier behind a step covers it. (Through the builtin it
@@ -215,6 +203,120 @@ using Index = std::integral_constant<int, I>;
 // the 16-byte piece of a row's step that lies at piece p of the row in LDS, and back
 __device__ __forceinline__ int swizzle(int row, int p) { return p ^ (row & 7); }
 
+// The end of a workgroup of WF x WR waves, each with 16 FT features (with SwiGLU half gate and
+// half up) by 16 RT rows, from its first output tile u0 and row r0, `high` of its rows in the
+// matrix: outputs through shared memory, so that whole lines go out.
+template <int kEpilogue, int FT, int RT, int WF, int WR>
+__device__ __forceinline__ void finish(const Fp8Args& a, f32x4_t (&acc)[FT][RT], uint8_t* s_bytes,
+                                       int u0, int r0, int high) {
+  constexpr bool kGate = kEpilogue != HS_LINEAR_PLAIN, kEight = kEpilogue == HS_LINEAR_SWIGLU_FP8;
+  constexpr int OT = kGate ? FT / 2 : FT;  // output tiles of a wave
+  constexpr int kRows = 16 * RT * WR, kTileRows = 16 * RT;
+  constexpr int kRow = 16 * OT * WF * (kEight ? 1 : 2), kPitch = kRow + 16;  // bytes of a row
+  static_assert(!kEight || kRow == kFp8Group, "a row's outputs are one group");
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wf = wave % WF, first = kTileRows * (wave / WF) + m;
+  uint32_t bytes[RT];  // exponents of the rows' codes
+  if constexpr (kEight) {
+    uint32_t* s_max = reinterpret_cast<uint32_t*>(s_bytes + kRows * kPitch);  // [wf][row]
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float most = 0;
+#pragma unroll
+      for (int f = 0; f < OT; ++f) {
+        float here = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[f][t][j] = silu(acc[f][t][j]) * acc[f + OT][t][j];
+          here = fmaxf(here, fabsf(acc[f][t][j]));  // (passes over NaN)
+        }
+        most = fmaxf(most, u0 + OT * wf + f < a.units ? here : 0.0f);
+      }
+      if (__any(most == __builtin_inff())) {  // the scale is that of the finite values
+        uint32_t bits = 0;
+#pragma unroll
+        for (int f = 0; f < OT; ++f)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (u0 + OT * wf + f < a.units) bits = max(bits, finite_bits(acc[f][t][j]));
+            acc[f][t][j] = nan_unless_finite(acc[f][t][j]);
+          }
+        most = __uint_as_float(bits);
+      }
+      most = quad_max(most);
+      if (g == 0) s_max[wf * kRows + first + 16 * t] = __float_as_uint(most);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int w = 0; w < WF; ++w) most = max(most, s_max[w * kRows + first + 16 * t]);
+      bytes[t] = scale_byte(most);
+      const float inv = scale_inverse(bytes[t]);
+#pragma unroll
+      for (int f = 0; f < OT; ++f) {
+        const float v[4] = {acc[f][t][0], acc[f][t][1], acc[f][t][2], acc[f][t][3]};
+        *reinterpret_cast<uint32_t*>(s_bytes + (first + 16 * t) * kPitch + 16 * (OT * wf + f) +
+                                     4 * g) = finite_codes4(v, inv);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+#pragma unroll
+      for (int f = 0; f < OT; ++f) {
+        uint16_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = result<kGate>(acc[f][t][j], kGate ? acc[f + FT - OT][t][j] : 0.0f);
+        *reinterpret_cast<uint2*>(s_bytes + (first + 16 * t) * kPitch + 32 * (OT * wf + f) +
+                                  8 * g) =
+            make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int kLanes = kRow / 16;  // of a row
+#pragma unroll
+  for (int i = 0; i < kRows * kLanes / (64 * WF * WR); ++i) {
+    const int e = (i * WF * WR + wave) * 64 + lane, in = e / kLanes, at = e % kLanes;
+    const int64_t row = r0 + in;
+    if (in >= high) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(s_bytes + in * kPitch + 16 * at);
+    if constexpr (kEight) {
+      const int n = 16 * (u0 + at);
+      if (n < a.N)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + row * a.ys + n) = v;
+    } else {
+      store8(a, row, 16 * u0 + 8 * at, v);
+    }
+  }
+  if constexpr (kEight) {
+    if (wf == 0 && g == 0) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        if (first + 16 * t < high)
+          a.ye[(int64_t)(r0 + first + 16 * t) * a.yes + u0 / 8] = (uint8_t)bytes[t];
+      }
+    }
+  }
+}
+
+// The workgroup's place in the order of the tiles: each XCD (workgroups go to them in turn)
+// has a stretch of it, so that what its L2 holds is shared: 8 row tiles to a column.
+__device__ __forceinline__ int order_of(int total) {
+  const int id = blockIdx.x, x = id & 7, q = total >> 3, r = total & 7;
+  return x * q + min(x, r) + (id >> 3);
+}
+__device__ __forceinline__ void place_of(const Fp8Args& a, int o, int& col, int& row) {
+  const int group = o / (8 * a.cols), in = o % (8 * a.cols);
+  const int tall = min(8, a.rowtiles - 8 * group);
+  row = 8 * group + in % tall;
+  col = in / tall;
+}
+
 template <int kEpilogue>
 __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   constexpr bool kGate = kEpilogue != HS_LINEAR_PLAIN;
@@ -224,17 +326,10 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wf = wave & 3, wr = wave >> 2;
-  // the workgroup's tile: each XCD has a stretch of them, 8 row tiles to a column
   int u0, r0;
-  {
-    const int total = a.cols * a.rowtiles;
-    const int id = blockIdx.x, x = id & 7, q = total >> 3, r = total & 7;
-    const int o = x * q + min(x, r) + (id >> 3);
-    const int group = o / (8 * a.cols), in = o % (8 * a.cols);
-    const int tall = min(8, a.rowtiles - 8 * group);
-    r0 = (8 * group + in % tall) * kBig;
-    u0 = in / tall * (kGate ? 8 : 16);
-  }
+  place_of(a, order_of(a.cols * a.rowtiles), u0, r0);
+  r0 *= kBig;
+  u0 *= kGate ? 8 : 16;
   auto tile_of = [&](int slot) {  // weight tile of one of the workgroup's 16 slots
     const int f = slot & 3;
     const int u = kGate ? u0 + (slot >> 2) * 2 + (f & 1) : u0 + slot;
@@ -301,8 +396,6 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
 #pragma unroll
     for (int t = 0; t < 8; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
   }
-  uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_bytes + kAtBad);
-  if (threadIdx.x < kBig) s_bad[threadIdx.x] = 0;
   // the chunk's exponents and scales: half of a row's words a thread
   auto load_chunk = [&](int first) {
     const int row = threadIdx.x & (kBig - 1), q0 = (int)(threadIdx.x >> 8) * (kChunk / 8);
@@ -321,27 +414,22 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     // (waited for here, not at every use among the loads in flight)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    uint32_t bad = 0;
 #pragma unroll
-    for (int i = 0; i < kChunk / 8; ++i) {
+    for (int i = 0; i < kChunk / 8; ++i)
       *reinterpret_cast<uint32_t*>(s_bytes + kAtE + (q0 + i) * 4 * kBig + 4 * row) = word[i];
-      // a byte of ones: its low seven bits carry into the eighth, which is set
-      bad |= ((word[i] & 0x7f7f7f7fu) + 0x01010101u) & word[i] & 0x80808080u;
-    }
-    return bad;
   };
   load_a(0);
   load_b(0);
   load_a(1);
   load_b(1);
-  uint32_t bad = load_chunk(0);
+  load_chunk(0);
   step_barrier<0>();
   i32x8_t x[3], w[4];
   uint32_t e[3];
   x[2] = read_x(0, 0);
 #pragma unroll
   for (int f = 0; f < 4; ++f) w[f] = read_w(0, f);
-  float factor[3][4] = {};  // of the products, by row tile's register and weight tile
+  float scale[4] = {0, 0, 0, 0};
   // One step, in an order that the compiler keeps: 32 products, each added three products
   // later; a row tile's operand is read one tile ahead. At the first barrier the lower rows
   // and the weights of the step have been read (by all waves): the step after the next loads
@@ -351,11 +439,13 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   auto one = [&](int step, int quad, auto quarter) {
     constexpr int kQ = decltype(quarter)::value;
     constexpr int kReg[8] = {2, 0, 1, 0, 1, 2, 0, 1};  // of the row tiles
-    float row, scale[4];
+    float before[4];
 #pragma unroll
-    for (int f = 0; f < 4; ++f)
+    for (int f = 0; f < 4; ++f) {
+      before[f] = scale[f];
       scale[f] = __uint_as_float(
           __builtin_amdgcn_readlane(__float_as_uint(sc[f]), step & (kChunk - 1)));
+    }
     // tile and weight of product i: the last two row tiles by weights
     auto tile = [](int i) { return i < 24 ? i >> 2 : 6 + (i & 1); };
     auto weight = [](int i) { return i < 24 ? i & 3 : (i - 24) >> 1; };
@@ -365,17 +455,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     };
     auto product = [&](int i) {
       const int t = tile(i), f = weight(i), r = kReg[t];
-      part[i & 3] = mfma(w[f], x[r]);
-      if (f == 0) row = row_scale<kQ>(e[r]);
-      // (a pair of tiles of one half is in one block of the weight)
-      if (f == 0) {
-        factor[r][0] = row * scale[0];
-        factor[r][1] = factor[r][0];
-        factor[r][2] = kGate ? row * scale[2] : factor[r][0];
-        factor[r][3] = kGate ? row * scale[3] : factor[r][0];
-      }
-      const int j = (i + 29) & 31, tj = tile(j), fj = weight(j);
-      acc[fj][tj] += factor[kReg[tj]][fj] * part[j & 3];
+      part[i & 3] = mfma<kQ>(w[f], x[r], e[r]);
+      const int j = (i + 29) & 31;
+      acc[weight(j)][tile(j)] += (i < 3 ? before : scale)[weight(j)] * part[j & 3];
       __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
@@ -416,7 +498,7 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   for (int first = 0; first < a.steps; first += kChunk) {
     if (first) {
       step_barrier<0>();  // the last chunk's exponents have been read
-      bad |= load_chunk(first);
+      load_chunk(first);
       step_barrier<0>();
     }
     e[2] = read_e(0, 0);
@@ -432,112 +514,199 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   }
 #pragma unroll
   for (int j = 29; j < 32; ++j)
-    acc[(j - 24) >> 1][6 + (j & 1)] += factor[j & 1][(j - 24) >> 1] * part[j & 3];
-  if (bad) s_bad[threadIdx.x & (kBig - 1)] = 1;
+    acc[(j - 24) >> 1][6 + (j & 1)] += scale[(j - 24) >> 1] * part[j & 3];
   step_barrier<0>();  // the last loads, which bring zeros, have landed
-  uint32_t nan_rows = 0;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) nan_rows |= s_bad[128 * wr + 16 * t + m] << t;
-  if (__any(nan_rows)) {
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-#pragma unroll
-      for (int f = 0; f < 4; ++f)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[f][t][j] = nan_rows >> t & 1 ? __builtin_nanf("") : acc[f][t][j];
-  }
-  // Through shared memory, so that whole lines go out: rows of kRow bytes and a pad
-  constexpr int kRow = kEpilogue == HS_LINEAR_PLAIN ? 2 * kBig : kGate && kEpilogue == HS_LINEAR_SWIGLU ? kBig : kBig / 2;
-  constexpr int kPitch = kRow + 16;
-  static_assert(kBig * kPitch <= kAtBad, "");
-  uint8_t* s_out = s_bytes;
-  uint32_t bytes[8];  // exponents of the rows' codes
-  if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
-    // the workgroup's 128 outputs of a row are one group: 32 of them in each of 4 waves
-    uint32_t* s_max = reinterpret_cast<uint32_t*>(s_bytes + kBig * kPitch);  // [wf][row]
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      float most = 0;
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        float here = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[f][t][j] = silu(acc[f][t][j]) * acc[f + 2][t][j];
-          here = fmaxf(here, fabsf(acc[f][t][j]));  // (passes over NaN)
-        }
-        most = fmaxf(most, u0 + 2 * wf + f < a.units ? here : 0.0f);
-      }
-      if (__any(most == __builtin_inff())) {  // the scale is that of the finite values
-        uint32_t bits = 0;
-#pragma unroll
-        for (int f = 0; f < 2; ++f)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            bits = max(bits, finite_bits(acc[f][t][j]));
-            acc[f][t][j] = nan_unless_finite(acc[f][t][j]);
-          }
-        most = __uint_as_float(bits);
-      }
-      most = quad_max(most);
-      if (g == 0) s_max[wf * kBig + 128 * wr + 16 * t + m] = __float_as_uint(most);
+  finish<kEpilogue, 4, 8, 4, 2>(a, acc, s_bytes, u0, r0, high);
+}
+
+// ---- fewer rows: smaller tiles, more stages, the steps split where there are few tiles ----
+
+// The sizes of a workgroup: WF x WR waves, each with 16 FT features by 16 RT rows; S stages.
+template <int kFT, int kRT, int kWF, int kWR, int kS>
+struct Tile {
+  static constexpr int FT = kFT, RT = kRT, WF = kWF, WR = kWR, S = kS;
+  static constexpr int kWaves = WF * WR, kThreads = 64 * kWaves;
+  static constexpr int kRows = 16 * RT * WR, kSlots = FT * WF;  // rows, 16-feature tiles
+  static constexpr int kXLoads = kRows / 8 / kWaves, kWLoads = 2 * kSlots / kWaves;  // a wave's
+  static constexpr int kXBytes = kRows * kStep, kStageBytes = kXBytes + kSlots * 16 * kStep;
+  static constexpr int kAtE = S * kStageBytes, kBytes = kAtE + kChunk * kRows;
+  static_assert(kXLoads * 8 * kWaves == kRows && (kWLoads == 2 || kWLoads == 4) &&
+                kWLoads * kWaves == 2 * kSlots, "");
+  static_assert(kRows * (32 * kSlots + 16) <= kBytes && kBytes <= 160 * 1024, "");
+};
+
+template <int kEpilogue, class T>
+__global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
+  constexpr bool kGate = kEpilogue != HS_LINEAR_PLAIN;
+  constexpr int FT = T::FT, RT = T::RT, OT = kGate ? FT / 2 : FT;
+  extern __shared__ uint4 s_all[];  // [stage][x: row, piece | w: tile, half, lane], exponents, bad
+  uint8_t* s_bytes = reinterpret_cast<uint8_t*>(s_all);
+  const uint32_t lds = lds_address(s_all);
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wf = wave % T::WF, wr = wave / T::WF;
+  const int tiles = a.cols * a.rowtiles, order = order_of(tiles * a.nsplit);
+  const int split = order / tiles;
+  int u0, r0;
+  place_of(a, order % tiles, u0, r0);
+  r0 *= T::kRows;
+  u0 *= OT * T::WF;
+  const int begin = split * a.split_steps, end = min(a.steps, begin + a.split_steps);
+  auto tile_of = [&](int slot) {  // weight tile of one of the workgroup's slots
+    const int f = slot % FT, u = u0 + slot / FT * OT + f % OT;
+    return min(u, a.units - 1) + f / OT * a.up;
+  };
+  const int64_t tile_bytes = (int64_t)a.steps * (16 * kStep);
+  uint8_t* wp = reinterpret_cast<uint8_t*>(const_cast<uint4*>(a.w));
+  uint8_t* xp = const_cast<uint8_t*>(a.x + (int64_t)r0 * a.xs);
+  constexpr int kWLoads = T::kWLoads;
+  uint8_t* wp0 = wp + tile_of(kWLoads / 2 * wave) * tile_bytes;
+  uint8_t* wp1 = wp + tile_of(kWLoads / 2 * (wave + 1) - 1) * tile_bytes;
+  const int high = min(a.rows - r0, T::kRows), k_end = min(a.K, kStep * end);
+  const int x_range = (high - 1) * (int)a.xs + a.K;  // rows behind the last one read zeros
+  const int piece = swizzle(lane >> 3, lane & 7);
+  // load i of a step's into stage `to`; past the last step none reads memory
+  constexpr int kLoads = T::kXLoads + kWLoads;
+  auto load = [&](int step, uint32_t to, int i) {
+    if (i < T::kXLoads) {
+      const auto b = __builtin_amdgcn_make_buffer_rsrc(xp, 0, x_range, 0x00027000);
+      const int k = kStep * step + 16 * piece, row = 8 * (T::kXLoads * wave + i);
+      load_lds(b, k < k_end ? (row + (lane >> 3)) * (int)a.xs + k : kPast, 0,
+               to + row * kStep);
+      return;
     }
-    __syncthreads();
+    i -= T::kXLoads;
+    const auto b = __builtin_amdgcn_make_buffer_rsrc(i < 2 ? wp0 : wp1, 0, step < end ? kRange : 0,
+                                                     0x00027000);
+    const uint32_t tw = to + T::kXBytes + 1024 * (kWLoads * wave + (i & 2));
+    if (i & 1) load_lds<1024>(b, 16 * lane, 16 * kStep * step, tw);
+    else load_lds<0>(b, 16 * lane, 16 * kStep * step, tw);
+  };
+  auto stage = [&](int i) { return lds + i * T::kStageBytes; };
+  float sc[FT];
+  auto load_chunk = [&](int first) {
+    constexpr int kWords = kChunk / 4 * T::kRows / T::kThreads;
+    const int row = threadIdx.x % T::kRows, q0 = (int)threadIdx.x / T::kRows * kWords;
+    const uint8_t* from = a.xe + (r0 + min(row, high - 1)) * a.xes + first;
+    uint32_t word[kWords];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      uint32_t most = 0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) most = max(most, s_max[w * kBig + 128 * wr + 16 * t + m]);
-      bytes[t] = scale_byte(most);
-      const float inv = scale_inverse(bytes[t]);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float v[4] = {acc[f][t][0], acc[f][t][1], acc[f][t][2], acc[f][t][3]};
-        *reinterpret_cast<uint32_t*>(s_out + (128 * wr + 16 * t + m) * kPitch + 32 * wf + 16 * f +
-                                     4 * g) = finite_codes4(v, inv);
-      }
+    for (int i = 0; i < kWords; ++i) {
+      const int at = 4 * (q0 + i), left = a.steps - first - at;  // (past the last step: zeros)
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(
+          from + min(at, (a.steps - 1 - first) & ~3));
+      word[i] = left >= 4 ? v : left > 0 ? v & ((1u << 8 * left) - 1) : 0;
     }
-  } else {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
+    for (int f = 0; f < FT; ++f)
+      sc[f] = a.sc[(int64_t)tile_of(FT * wf + f) * a.steps + min(first + lane, a.steps - 1)];
+    // (waited for here, not at every use among the loads in flight)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
 #pragma unroll
-      for (int f = 0; f < (kGate ? 2 : 4); ++f) {
-        uint16_t v[4];
+    for (int i = 0; i < kWords; ++i)
+      *reinterpret_cast<uint32_t*>(s_bytes + T::kAtE + ((q0 + i) * T::kRows + row) * 4) = word[i];
+  };
+
+  f32x4_t acc[FT][RT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[j] = result<kGate>(acc[f][t][j], kGate ? acc[f + 2][t][j] : 0.0f);
-        *reinterpret_cast<uint2*>(s_out + (128 * wr + 16 * t + m) * kPitch +
-                                  (kGate ? 64 : 128) * wf + 32 * f + 8 * g) =
-            make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
-      }
-    }
-  }
-  __syncthreads();
-  constexpr int kLanes = kRow / 16;  // of a row
+  for (int f = 0; f < FT; ++f)
 #pragma unroll
-  for (int i = 0; i < 32 * kLanes / 64; ++i) {
-    const int in = 32 * wave + (64 * i + lane) / kLanes, at = lane % kLanes;
-    const int64_t row = r0 + in;
-    if (in >= high) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(s_out + in * kPitch + 16 * at);
-    if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
-      const int n = 16 * (u0 + at);
-      if (n < a.N)
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.y) + row * a.ys + n) = v;
+    for (int t = 0; t < RT; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < T::S * kLoads; ++i) load(begin + i / kLoads, stage(i / kLoads), i % kLoads);
+  const int in_rows = 16 * RT * wr + m;
+  const uint8_t* sx0 = s_bytes + in_rows * kStep + 16 * swizzle(m, g);
+  const uint8_t* sx1 = s_bytes + in_rows * kStep + 16 * swizzle(m, 4 + g);
+  const uint8_t* sw = s_bytes + T::kXBytes + wf * FT * 2048 + 16 * lane;
+  const uint8_t* se = s_bytes + T::kAtE + 4 * in_rows;
+  struct Operands {
+    i32x8_t x[RT], w[FT];
+  };
+  constexpr int kReads = FT + RT;
+  auto read = [&](int at, Operands& o, int i) {  // operand i: the weights', then the rows'
+    if (i < FT) {
+      o.w[i] = operand(*reinterpret_cast<const uint4*>(sw + at + 2048 * i),
+                       *reinterpret_cast<const uint4*>(sw + at + 2048 * i + 1024));
     } else {
-      store8(a, row, 16 * u0 + 8 * at, v);
+      o.x[i - FT] = operand(*reinterpret_cast<const uint4*>(sx0 + at + 16 * (i - FT) * kStep),
+                            *reinterpret_cast<const uint4*>(sx1 + at + 16 * (i - FT) * kStep));
+    }
+  };
+  load_chunk(begin);
+  step_barrier<(T::S - 1) * kLoads>();
+  Operands even, odd;
+#pragma unroll
+  for (int i = 0; i < kReads; ++i) read(0, even, i);
+  int now = 0;  // the step's stage
+  // A step, whose operands are in registers. Between its products the next one's are read
+  // and the loads of the step that takes its stage go out: a wave issues in order, and there
+  // may be one to a SIMD (all of them before the products: 0.64 us a step of 128 x 128, TIME
+  // so). The barrier sees that the next step has landed and that all waves have read this one.
+  auto one = [&](int step, int in_chunk, const Operands& o, Operands& next) {
+    step_barrier<(T::S - 2) * kLoads>();
+    uint32_t e[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      e[t] = *reinterpret_cast<const uint32_t*>(se + (in_chunk >> 2) * 4 * T::kRows + 64 * t);
+    const uint32_t to = stage(now);
+    now = now == T::S - 1 ? 0 : now + 1;
+    const int shift = 8 * (in_chunk & 3);
+    float scale[FT];
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+      scale[f] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[f]), in_chunk));
+    // products, each added three products later
+    f32x4_t part[4];
+    auto add = [&](int j) { acc[j % FT][j / FT] += scale[j % FT] * part[j & 3]; };
+#pragma unroll
+    for (int i = 0; i < FT * RT; ++i) {
+      const int t = i / FT, f = i % FT;
+      if (f == 0) e[t] >>= shift;
+      if (i >= 3) add(i - 3);
+      part[i & 3] = mfma<0>(o.w[f], o.x[t], e[t]);
+      constexpr int P = FT * RT;
+#pragma unroll
+      for (int j = i * kReads / P; j < (i + 1) * kReads / P; ++j)
+        read(now * T::kStageBytes, next, j);
+#pragma unroll
+      for (int j = i * kLoads / P; j < (i + 1) * kLoads / P; ++j) load(step + T::S, to, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = FT * RT - 3; j < FT * RT; ++j) add(j);
+  };
+  for (int first = begin; first < end; first += kChunk) {
+    if (first != begin) {
+      step_barrier<0>();  // the last chunk's exponents have been read
+      load_chunk(first);
+    }
+    // two steps at a time: past the last one the rows are zeros, and so is their scale
+    const int count = min(kChunk, end - first);
+    for (int i = 0; i < count; i += 2) {
+      one(first + i, i, even, odd);
+      one(first + i + 1, i + 1, odd, even);
     }
   }
-  if constexpr (kEpilogue == HS_LINEAR_SWIGLU_FP8) {
-    if (wf == 0 && g == 0) {
+  step_barrier<0>();  // the last loads, which bring zeros, have landed
+  if (a.part) {
+    const int64_t width = (int64_t)a.units * (kGate ? 32 : 16);
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const int in = 128 * wr + 16 * t + m;
-        if (in < high) a.ye[(int64_t)(r0 + in) * a.yes + u0 / 8] = (uint8_t)bytes[t];
+    for (int t = 0; t < RT; ++t) {
+      if (in_rows + 16 * t >= high) continue;
+      float* to = a.part + ((int64_t)split * a.rows + r0 + in_rows + 16 * t) * width;
+#pragma unroll
+      for (int f = 0; f < FT; ++f) {
+        const int u = u0 + wf * OT + f % OT;
+        if (u < a.units)
+          *reinterpret_cast<f32x4_t*>(to + (int64_t)(u + f / OT * a.units) * 16 + 4 * g) = acc[f][t];
       }
     }
+    return;
   }
+  if constexpr (kEpilogue != HS_LINEAR_SWIGLU_FP8)
+    finish<kEpilogue, FT, RT, T::WF, T::WR>(a, acc, s_bytes, u0, r0, high);
+  else if constexpr (OT * T::WF == 8)
+    finish<kEpilogue, FT, RT, T::WF, T::WR>(a, acc, s_bytes, u0, r0, high);
 }
 
 constexpr int kJoinThreads = 256;
@@ -587,8 +756,15 @@ __global__ __launch_bounds__(kJoinThreads) void k_fp8_join(Fp8Args a) {
 
 constexpr int kCus = 256;
 
+using Tile256x128 = Tile<4, 4, 4, 2, 3>;  // features by rows
+using Tile128x128 = Tile<2, 4, 4, 2, 4>;
+using Tile128x64 = Tile<2, 2, 4, 2, 3>;
+using Tile128x32 = Tile<2, 2, 4, 1, 3>;
+
+enum Kernel { kRowsOf16, k128x32, k128x64, k128x128, k256x128, k256x256 };
+
 struct Fp8Plan {
-  bool big;            // k_fp8_big
+  Kernel kernel;
   int split_steps, nsplit;
   size_t part_bytes;   // sums of split steps
   size_t codes_bytes;  // codes of bf16 rows
@@ -600,12 +776,15 @@ int64_t scales_row(int K) { return ((K + kStep - 1) / kStep + 3) / 4 * 4; }
 
 Fp8Plan plan_of(int rows, int K, int N, int epilogue, bool bf16_rows) {
   Fp8Plan p = {};
+  const bool gate = epilogue != HS_LINEAR_PLAIN, eight = epilogue == HS_LINEAR_SWIGLU_FP8;
   const int steps = (K + kStep - 1) / kStep, units = (N + 15) / 16;
   p.nsplit = 1;
   p.split_steps = steps;
-  p.big = rows > 128;
-  if (epilogue == HS_LINEAR_SWIGLU_FP8 && !p.big)
-    p.part_bytes = padded((size_t)p.nsplit * rows * units * 32 * sizeof(float));
+  p.kernel = rows > 128 ? k256x256 : kRowsOf16;
+  //PLAN
+  const bool whole = p.kernel == k256x256 || p.kernel == k256x128;  // of a group of outputs
+  if (p.nsplit > 1 || (eight && !whole))
+    p.part_bytes = padded((size_t)p.nsplit * rows * units * (gate ? 32 : 16) * sizeof(float));
   if (bf16_rows)
     p.codes_bytes = padded((size_t)rows * K) + padded((size_t)rows * scales_row(K));
   p.bytes = p.part_bytes + p.codes_bytes;
@@ -627,17 +806,34 @@ void dispatch_rows(const Fp8Args& a, bool gate, hipStream_t s) {
   else launch_rows<8, 1, false>(a, s);
 }
 
-template <int kEpilogue>
-int launch_big(Fp8Args& a, hipStream_t s) {
-  a.cols = (a.units + (kEpilogue == HS_LINEAR_PLAIN ? 15 : 7)) / (kEpilogue == HS_LINEAR_PLAIN ? 16 : 8);
-  a.rowtiles = (a.rows + kBig - 1) / kBig;
-  static const hipError_t set = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(k_fp8_big<kEpilogue>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, kBigBytes);
-  if (set != hipSuccess) return HS_ERR_LAUNCH;
-  hipLaunchKernelGGL((k_fp8_big<kEpilogue>), dim3((unsigned)(a.cols * a.rowtiles)),
-                     dim3(kBigThreads), kBigBytes, s, a);
+// a kernel of more than 64 KB of shared memory
+template <class F>
+int launch(F kernel, int blocks, int threads, int bytes, const Fp8Args& a, hipStream_t s) {
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return HS_ERR_LAUNCH;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), bytes, s, a);
   return hipGetLastError() == hipSuccess ? HS_OK : HS_ERR_LAUNCH;
+}
+
+template <int kEpilogue>
+int launch_tiles(Fp8Args& a, Kernel kernel, hipStream_t s) {
+  constexpr int kHalf = kEpilogue == HS_LINEAR_PLAIN ? 1 : 2;
+  auto tiles = [&](int slots, int rows) {
+    a.cols = (a.units + slots / kHalf - 1) / (slots / kHalf);
+    a.rowtiles = (a.rows + rows - 1) / rows;
+    return a.cols * a.rowtiles * a.nsplit;
+  };
+  auto go = [&](auto tile) {
+    using T = decltype(tile);
+    return launch(k_fp8_tile<kEpilogue, T>, tiles(T::kSlots, T::kRows), T::kThreads, T::kBytes, a, s);
+  };
+  if (kernel == k256x256)
+    return launch(k_fp8_big<kEpilogue>, tiles(16, kBig), kBigThreads, kBigBytes, a, s);
+  if (kernel == k256x128) return go(Tile256x128());
+  if (kernel == k128x128) return go(Tile128x128());
+  if (kernel == k128x64) return go(Tile128x64());
+  return go(Tile128x32());
 }
 
 int join(const Fp8Args& a, int epilogue, hipStream_t s) {
@@ -735,13 +931,18 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.split_steps = p.split_steps;
   a.nsplit = p.nsplit;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (p.big) {
-    if (epilogue == HS_LINEAR_PLAIN) return launch_big<HS_LINEAR_PLAIN>(a, s);
-    if (epilogue == HS_LINEAR_SWIGLU) return launch_big<HS_LINEAR_SWIGLU>(a, s);
-    return launch_big<HS_LINEAR_SWIGLU_FP8>(a, s);
+  int status = HS_OK;
+  if (p.kernel == kRowsOf16) {
+    dispatch_rows(a, gate, s);
+    if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
+  } else if (epilogue == HS_LINEAR_PLAIN) {
+    status = launch_tiles<HS_LINEAR_PLAIN>(a, p.kernel, s);
+  } else if (epilogue == HS_LINEAR_SWIGLU) {
+    status = launch_tiles<HS_LINEAR_SWIGLU>(a, p.kernel, s);
+  } else {
+    status = launch_tiles<HS_LINEAR_SWIGLU_FP8>(a, p.kernel, s);
   }
-  dispatch_rows(a, gate, s);
-  if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
+  if (status != HS_OK) return status;
   return a.part ? join(a, epilogue, s) : HS_OK;
 }
 
