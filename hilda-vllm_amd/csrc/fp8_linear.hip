@@ -30,13 +30,12 @@ namespace hs {
 namespace {
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = kFp8Group;  // inputs of a step
 
 struct Fp8Args {
-  const uint8_t* x;
+  const uint8_t* x;   // codes, or bf16 (k_fp8_rows)
   int64_t xs;
   const uint8_t* xe;  // exponent bytes [rows][xes]
   int64_t xes;
@@ -74,15 +73,6 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-// inputs 128 step + 64 h + 16 g .. + 15 of a row; zeros past the row or K
-__device__ __forceinline__ uint4 load_x(const Fp8Args& a, int row, int step, int h, int g) {
-  const int k = kStep * step + 64 * h + 16 * g;
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (row < a.rows && k < a.K)
-    v = *reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.xs + k);
-  return v;
-}
-
 // (the reciprocal instruction is good to one unit in f32's last place)
 __device__ __forceinline__ float silu(float g) {
   return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));
@@ -108,40 +98,120 @@ __device__ __forceinline__ void store8(const Fp8Args& a, int64_t row, int n, uin
   }
 }
 
-// 16 rows a workgroup. W: its waves, which share out the steps of its TN weight tiles (with
-// SwiGLU half of them gate and half up tiles) and join their sums in LDS.
-template <int W, int TN, bool kGate>
+// The lane's 32 values of a bf16 row's step (inputs 64 h + 16 g .. + 15, h = 0 and 1) as codes
+// under the scale of the step's 128, which the four lanes of a row share; its exponent's byte.
+__device__ __forceinline__ i32x8_t row_codes(const uint4 (&raw)[4], uint32_t& byte) {
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  uint32_t v[16] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w,
+                    raw[2].x, raw[2].y, raw[2].z, raw[2].w, raw[3].x, raw[3].y, raw[3].z, raw[3].w};
+  // the bits of |v| order bf16 numbers
+  auto most_of = [&] {
+    u16x2_t most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu));
+    uint32_t m = max((uint32_t)most[0], (uint32_t)most[1]);
+    const auto p = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(p[0], p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return max(q[0], q[1]);
+  };
+  uint32_t most = most_of();
+  if (__any(most >= 0x7f80u)) {  // NaN and infinities take no part in the scale, and are NaN
+    uint32_t nan[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      nan[i] = ((v[i] & 0x7f80u) == 0x7f80u ? 0x7fc0u : 0) |
+               ((v[i] & 0x7f800000u) == 0x7f800000u ? 0x7fc00000u : 0);
+      if (nan[i] & 0xffffu) v[i] &= 0xffff0000u;
+      if (nan[i] >> 16) v[i] &= 0xffffu;
+    }
+    most = most_of();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] |= nan[i];
+  }
+  byte = scale_byte(most << 16);
+  return scaled_codes32(v, byte);
+}
+
+// RT * 16 rows a workgroup. W: its waves, which share out the steps of its TN weight tiles
+// (with SwiGLU half of them gate and half up tiles), U of a wave's steps at once, and join
+// their sums in LDS. kBf16: the rows are bf16 and go to 8 bits here, in every workgroup.
+template <int W, int TN, int RT, int U, bool kGate, bool kBf16>
 __global__ __launch_bounds__(64 * W) void k_fp8_rows(Fp8Args a) {
   constexpr int kOut = kGate ? TN / 2 : TN;
-  __shared__ float s_part[W][TN][16][16];  // [wave][tile][row][feature]
+  __shared__ float s_part[W][TN][16 * RT][16];  // [wave][tile][row][feature]
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u0 = blockIdx.x * kOut, r0 = blockIdx.y * 16, row = r0 + m;
+  const int u0 = blockIdx.x * kOut, r0 = blockIdx.y * 16 * RT;
   int tile[TN];
 #pragma unroll
   for (int t = 0; t < TN; ++t) tile[t] = min(u0 + t % kOut, a.units - 1) + t / kOut * a.up;
-  const uint8_t* xe = a.xe + (int64_t)min(row, a.rows - 1) * a.xes;
-  f32x4_t y[TN];
+  f32x4_t y[TN][RT];
 #pragma unroll
-  for (int t = 0; t < TN; ++t) y[t] = f32x4_t{0, 0, 0, 0};
-  for (int step = wave; step < a.steps; step += W) {
-    i32x8_t w[TN];
-    float sw[TN];
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) y[t][r] = f32x4_t{0, 0, 0, 0};
+  constexpr int kRaw = kBf16 ? 4 : 2;  // 16-byte pieces of a row's step in a lane
+  struct Step {
+    uint4 w[TN][2], x[RT][kRaw];
+    uint32_t e[RT];
+    float sc[TN];
+  };
+  auto load = [&](int step, Step& s) {
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
       const int64_t at = (int64_t)tile[t] * a.steps + step;
-      w[t] = operand(load_once(a.w + at * 128 + lane), load_once(a.w + at * 128 + 64 + lane));
-      sw[t] = a.sc[at];
+      s.w[t][0] = load_once(a.w + at * 128 + lane);
+      s.w[t][1] = load_once(a.w + at * 128 + 64 + lane);
+      s.sc[t] = a.sc[at];
     }
-    const i32x8_t x = operand(load_x(a, row, step, 0, g), load_x(a, row, step, 1, g));
-    const uint32_t e = xe[step];
 #pragma unroll
-    for (int t = 0; t < TN; ++t) y[t] += sw[t] * mfma<0>(w[t], x, e);
+    for (int r = 0; r < RT; ++r) {
+      const int row = r0 + 16 * r + m;
+#pragma unroll
+      for (int i = 0; i < kRaw; ++i) {
+        const int k = kStep * step + 64 * (2 * i / kRaw) + 16 * g + (kBf16 ? 8 * (i & 1) : 0);
+        s.x[r][i] = make_uint4(0, 0, 0, 0);
+        if (row < a.rows && k < a.K)
+          s.x[r][i] = *reinterpret_cast<const uint4*>(a.x + ((int64_t)row * a.xs + k) *
+                                                                (kBf16 ? 2 : 1));
+      }
+      if (!kBf16) s.e[r] = a.xe[(int64_t)min(row, a.rows - 1) * a.xes + step];
+    }
+  };
+  auto multiply = [&](const Step& s) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      uint32_t e = s.e[r];
+      i32x8_t x;
+      if constexpr (kBf16) x = row_codes(s.x[r], e);
+      else x = operand(s.x[r][0], s.x[r][1]);
+#pragma unroll
+      for (int t = 0; t < TN; ++t)
+        y[t][r] += s.sc[t] * mfma<0>(operand(s.w[t][0], s.w[t][1]), x, e);
+    }
+  };
+  int step = wave;
+  for (; step + (U - 1) * W < a.steps; step += U * W) {
+    Step s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(step + u * W, s[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) multiply(s[u]);
+  }
+  for (; step < a.steps; step += W) {
+    Step s;
+    load(step, s);
+    multiply(s);
   }
 #pragma unroll
-  for (int t = 0; t < TN; ++t) *reinterpret_cast<f32x4_t*>(&s_part[wave][t][m][4 * g]) = y[t];
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+      *reinterpret_cast<f32x4_t*>(&s_part[wave][t][16 * r + m][4 * g]) = y[t][r];
   __syncthreads();
-  const int rows = min(16, a.rows - r0);
+  const int rows = min(16 * RT, a.rows - r0);
   for (int e = threadIdx.x; e < 16 * rows * kOut; e += 64 * W) {
     const int n = e & 15, t = (e >> 4) % kOut, r = (e >> 4) / kOut;
     float v = 0.0f, up = 0.0f;
@@ -785,25 +855,30 @@ Fp8Plan plan_of(int rows, int K, int N, int epilogue, bool bf16_rows) {
   const bool whole = p.kernel == k256x256 || p.kernel == k256x128;  // of a group of outputs
   if (p.nsplit > 1 || (eight && !whole))
     p.part_bytes = padded((size_t)p.nsplit * rows * units * (gate ? 32 : 16) * sizeof(float));
-  if (bf16_rows)
+  if (bf16_rows && p.kernel != kRowsOf16)
     p.codes_bytes = padded((size_t)rows * K) + padded((size_t)rows * scales_row(K));
   p.bytes = p.part_bytes + p.codes_bytes;
   return p;
 }
 
-template <int W, int TN, bool kGate>
-void launch_rows(const Fp8Args& a, hipStream_t s) {
+template <int W, int TN, int RT, int U, bool kGate>
+void launch_rows(const Fp8Args& a, bool bf16_rows, hipStream_t s) {
   constexpr int kOut = kGate ? TN / 2 : TN;
-  hipLaunchKernelGGL((k_fp8_rows<W, TN, kGate>),
-                     dim3((unsigned)((a.units + kOut - 1) / kOut), (unsigned)((a.rows + 15) / 16)),
-                     dim3(64 * W), 0, s, a);
+  const dim3 grid((unsigned)((a.units + kOut - 1) / kOut), (unsigned)((a.rows + 16 * RT - 1) / (16 * RT)));
+  if (bf16_rows) {
+    if constexpr (RT == 1)
+      hipLaunchKernelGGL((k_fp8_rows<W, TN, RT, U, kGate, true>), grid, dim3(64 * W), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((k_fp8_rows<W, TN, RT, U, kGate, false>), grid, dim3(64 * W), 0, s, a);
+  }
 }
 
-void dispatch_rows(const Fp8Args& a, bool gate, hipStream_t s) {
-  if (gate) launch_rows<4, 2, true>(a, s);
-  else if (a.units >= 12 * kCus) launch_rows<4, 4, false>(a, s);
-  else if (a.units >= 4 * kCus) launch_rows<4, 2, false>(a, s);
-  else launch_rows<8, 1, false>(a, s);
+void dispatch_rows(const Fp8Args& a, bool gate, bool bf16_rows, hipStream_t s) {
+  //ROWS
+  if (gate) launch_rows<4, 2, 1, 2, true>(a, bf16_rows, s);
+  else if (a.units >= 12 * kCus) launch_rows<4, 4, 1, 1, false>(a, bf16_rows, s);
+  else if (a.units >= 4 * kCus) launch_rows<4, 2, 1, 2, false>(a, bf16_rows, s);
+  else launch_rows<8, 1, 1, 4, false>(a, bf16_rows, s);
 }
 
 // a kernel of more than 64 KB of shared memory
@@ -903,7 +978,8 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.xs = x_stride;
   a.xe = static_cast<const uint8_t*>(x_scales);
   a.xes = x_scales_stride;
-  if (bf16_rows) {
+  const bool fused = bf16_rows && p.kernel == kRowsOf16;  // with the quantisation
+  if (bf16_rows && !fused) {
     uint8_t* codes = ws + p.part_bytes;
     uint8_t* exps = codes + padded((size_t)rows * in_features);
     const int status = hs_quantize_rows_fp8(x, x_stride, rows, in_features, codes, in_features,
@@ -933,7 +1009,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   int status = HS_OK;
   if (p.kernel == kRowsOf16) {
-    dispatch_rows(a, gate, s);
+    dispatch_rows(a, gate, fused, s);
     if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   } else if (epilogue == HS_LINEAR_PLAIN) {
     status = launch_tiles<HS_LINEAR_PLAIN>(a, p.kernel, s);

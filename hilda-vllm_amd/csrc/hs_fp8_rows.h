@@ -16,6 +16,8 @@ namespace hs {
 
 constexpr int kFp8Group = 128;  // values of a scale
 
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
 // the bits of |v|, 0 where v is NaN or infinite
 __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
@@ -45,6 +47,25 @@ __device__ __forceinline__ uint32_t finite_codes4(const float* v, float inv) {
   w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, w, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
   return (uint32_t)w;
+}
+
+// codes of 32 bf16 values (in pairs; finite or NaN) under the scale of exponent `byte`
+// (v_cvt_scalef32_pk_fp8_bf16: the quotient by the scale, to nearest even)
+__device__ __forceinline__ i32x8_t scaled_codes32(const uint32_t (&v)[16], uint32_t byte) {
+  typedef short i16x2_t __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const float scale = __uint_as_float(byte << 23);
+  i32x8_t codes;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    i16x2_t w = {0, 0};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2_t, v[2 * i]), scale,
+                                                  false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2_t, v[2 * i + 1]),
+                                                  scale, true);
+    codes[i] = __builtin_bit_cast(int, w);
+  }
+  return codes;
 }
 
 // the largest of the lanes l, l ^ 16, l ^ 32 and l ^ 48
