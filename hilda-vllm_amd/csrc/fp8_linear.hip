@@ -135,9 +135,9 @@ __device__ __forceinline__ i32x8_t row_codes(const uint4 (&raw)[4], uint32_t& by
 }
 
 // RT * 16 rows a workgroup. W: its waves, which share out the steps of its TN weight tiles
-// (with SwiGLU half of them gate and half up tiles), U of a wave's steps at once, and join
-// their sums in LDS. kBf16: the rows are bf16 and go to 8 bits here, in every workgroup.
-template <int W, int TN, int RT, int U, bool kGate, bool kBf16>
+// (with SwiGLU half of them gate and half up tiles) and join their sums in LDS. kBf16: the
+// rows are bf16 and go to 8 bits here, in every workgroup.
+template <int W, int TN, int RT, bool kGate, bool kBf16>
 __global__ __launch_bounds__(64 * W) void k_fp8_rows(Fp8Args a) {
   constexpr int kOut = kGate ? TN / 2 : TN;
   __shared__ float s_part[W][TN][16 * RT][16];  // [wave][tile][row][feature]
@@ -192,15 +192,9 @@ __global__ __launch_bounds__(64 * W) void k_fp8_rows(Fp8Args a) {
         y[t][r] += s.sc[t] * mfma<0>(operand(s.w[t][0], s.w[t][1]), x, e);
     }
   };
-  int step = wave;
-  for (; step + (U - 1) * W < a.steps; step += U * W) {
-    Step s[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(step + u * W, s[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) multiply(s[u]);
-  }
-  for (; step < a.steps; step += W) {
+  // one step's loads at a time: many waves hide them as well as many loads (16 waves 5.0 us, 8
+  // waves with four steps' loads 5.1 us for a row of 4096, 4096 features)
+  for (int step = wave; step < a.steps; step += W) {
     Step s;
     load(step, s);
     multiply(s);
@@ -831,7 +825,22 @@ using Tile128x128 = Tile<2, 4, 4, 2, 4>;
 using Tile128x64 = Tile<2, 2, 4, 2, 3>;
 using Tile128x32 = Tile<2, 2, 4, 1, 3>;
 
-enum Kernel { kRowsOf16, k128x32, k128x64, k128x128, k256x128, k256x256 };
+enum Kernel { kRows, k128x32, k128x64, k128x128, k256x128, k256x256 };
+
+// What a workgroup of a tile kernel takes, in us: a step, alone and with all CUs at work, and
+// everything beside the steps. Fitted to 135 shapes (17 to 3000 rows, 1024 to 12288 inputs, 1024
+// to 24576 features) with every kernel and up to 16 splits: the choices by these figures take
+// 0.5% longer than the best ones on average, 14% at most.
+struct TileTime {
+  int features, rows;
+  float step, full_step, rest;
+};
+constexpr TileTime kTileTimes[] = {{0, 0, 0, 0, 0},
+                                   {128, 32, 0.23f, 0.28f, 3.4f},
+                                   {128, 64, 0.30f, 0.38f, 3.5f},
+                                   {128, 128, 0.37f, 0.54f, 4.1f},
+                                   {256, 128, 0.66f, 0.78f, 6.7f},
+                                   {256, 256, 1.12f, 1.35f, 6.7f}};
 
 struct Fp8Plan {
   Kernel kernel;
@@ -844,41 +853,96 @@ struct Fp8Plan {
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 int64_t scales_row(int K) { return ((K + kStep - 1) / kStep + 3) / 4 * 4; }
 
+// The few-row kernel's sizes for a call, none (0 waves) where the tiles serve it. Up to 16 rows
+// take it always: 16 waves for a tile of a weight of up to 256 (4096 features, 4 rows: 5.1 us,
+// 5.7 us with 8), 8 for more than 8 rows, whose operands weigh more (12288 inputs, 16 rows: 12.7
+// us, 14.2 us with 16); two tiles to a workgroup that shares their rows for wider ones (6144
+// features, 4 rows: 6.3 us, 6.9 us with one), and four of very wide ones with many rows (151936
+// features, 16 bf16 rows: 100 us, 116 us with two). More rows take it where the workgroups still
+// fit the CUs: then each weight is read once or twice and nothing has to be joined (64 rows of
+// 4096, 4096 features: 9.2 us, 11.7 us in tiles; 32 rows 6.8 and 10.7 us); with 32 rows a
+// workgroup only up to 56 steps, past which the rows' reads cost more (12288 inputs, 64 rows: 23
+// us, 19 us in tiles).
+struct RowsKernel {
+  int waves, tiles, row_tiles;
+};
+RowsKernel rows_of(int rows, int steps, int units, bool gate) {
+  const int r16 = (rows + 15) / 16, r32 = (rows + 31) / 32;
+  const int pairs = gate ? units : (units + 1) / 2;
+  if (!gate && (int64_t)units * r16 <= kCus) return {rows <= 8 ? 16 : 8, 1, 1};
+  if (rows <= 16 && !gate && units >= 12 * kCus && rows > 8) return {4, 4, 1};
+  if (rows <= 16 || (int64_t)pairs * r16 <= kCus) return {8, 2, 1};
+  if ((int64_t)pairs * r32 <= kCus && steps <= 56) return {8, 2, 2};
+  if (rows <= 32 && !gate && units >= 12 * kCus) return {4, 4, 2};
+  return {0, 0, 0};
+}
+
 Fp8Plan plan_of(int rows, int K, int N, int epilogue, bool bf16_rows) {
   Fp8Plan p = {};
   const bool gate = epilogue != HS_LINEAR_PLAIN, eight = epilogue == HS_LINEAR_SWIGLU_FP8;
   const int steps = (K + kStep - 1) / kStep, units = (N + 15) / 16;
   p.nsplit = 1;
   p.split_steps = steps;
-  p.kernel = rows > 128 ? k256x256 : kRowsOf16;
-  //PLAN
+  p.kernel = rows_of(rows, steps, units, gate).waves ? kRows : k128x32;
+  if (p.kernel != kRows) {
+    float best = 0;
+    for (int k = k128x32; k <= k256x256; ++k) {
+      const TileTime& t = kTileTimes[k];
+      const int64_t tiles = (int64_t)((units * (gate ? 2 : 1) * 16 + t.features - 1) / t.features) *
+                            ((rows + t.rows - 1) / t.rows);
+      for (int want : {1, 2, 3, 4, 6, 8, 12, 16}) {
+        // (exponents are read four steps at a time)
+        const int split_steps = ((steps + want - 1) / want + 3) / 4 * 4;
+        const int n = (steps + split_steps - 1) / split_steps;
+        if (want > 1 && (k == k256x256 || tiles * n > 2 * kCus || split_steps >= steps)) break;
+        const int64_t groups = tiles * n, rounds = (groups + kCus - 1) / kCus;
+        const float fill = groups < kCus ? (float)groups / kCus : 1.0f;
+        const float step = t.step + (t.full_step - t.step) * fill;
+        float time = rounds * ((want > 1 ? split_steps : steps) * step + t.rest);
+        // the weights' stream, from memory or the cache before it
+        time = fmaxf(time, (float)units * (gate ? 2 : 1) * 16 * K / 8e6f + 2.0f);
+        // sums that go through memory, and the launch that joins them
+        if (n > 1 || (eight && k < k256x128))
+          time += 3.6f + (float)n * rows * units * (gate ? 2 : 1) * 64 / 2.25e6f;
+        if (best != 0 && time >= best) continue;
+        best = time;
+        p.kernel = (Kernel)k;
+        p.nsplit = n;
+        p.split_steps = n > 1 ? split_steps : steps;
+      }
+    }
+  }
   const bool whole = p.kernel == k256x256 || p.kernel == k256x128;  // of a group of outputs
   if (p.nsplit > 1 || (eight && !whole))
     p.part_bytes = padded((size_t)p.nsplit * rows * units * (gate ? 32 : 16) * sizeof(float));
-  if (bf16_rows && p.kernel != kRowsOf16)
+  if (bf16_rows && !(p.kernel == kRows && rows <= 16))
     p.codes_bytes = padded((size_t)rows * K) + padded((size_t)rows * scales_row(K));
   p.bytes = p.part_bytes + p.codes_bytes;
   return p;
 }
 
-template <int W, int TN, int RT, int U, bool kGate>
+template <int W, int TN, int RT, bool kGate>
 void launch_rows(const Fp8Args& a, bool bf16_rows, hipStream_t s) {
   constexpr int kOut = kGate ? TN / 2 : TN;
   const dim3 grid((unsigned)((a.units + kOut - 1) / kOut), (unsigned)((a.rows + 16 * RT - 1) / (16 * RT)));
   if (bf16_rows) {
     if constexpr (RT == 1)
-      hipLaunchKernelGGL((k_fp8_rows<W, TN, RT, U, kGate, true>), grid, dim3(64 * W), 0, s, a);
+      hipLaunchKernelGGL((k_fp8_rows<W, TN, RT, kGate, true>), grid, dim3(64 * W), 0, s, a);
   } else {
-    hipLaunchKernelGGL((k_fp8_rows<W, TN, RT, U, kGate, false>), grid, dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((k_fp8_rows<W, TN, RT, kGate, false>), grid, dim3(64 * W), 0, s, a);
   }
 }
 
 void dispatch_rows(const Fp8Args& a, bool gate, bool bf16_rows, hipStream_t s) {
-  //ROWS
-  if (gate) launch_rows<4, 2, 1, 2, true>(a, bf16_rows, s);
-  else if (a.units >= 12 * kCus) launch_rows<4, 4, 1, 1, false>(a, bf16_rows, s);
-  else if (a.units >= 4 * kCus) launch_rows<4, 2, 1, 2, false>(a, bf16_rows, s);
-  else launch_rows<8, 1, 1, 4, false>(a, bf16_rows, s);
+  const RowsKernel k = rows_of(a.rows, a.steps, a.units, gate);
+  if (gate && k.row_tiles == 1) launch_rows<8, 2, 1, true>(a, bf16_rows, s);
+  else if (gate) launch_rows<8, 2, 2, true>(a, bf16_rows, s);
+  else if (k.waves == 16) launch_rows<16, 1, 1, false>(a, bf16_rows, s);
+  else if (k.tiles == 1) launch_rows<8, 1, 1, false>(a, bf16_rows, s);
+  else if (k.tiles == 2 && k.row_tiles == 1) launch_rows<8, 2, 1, false>(a, bf16_rows, s);
+  else if (k.tiles == 2) launch_rows<8, 2, 2, false>(a, bf16_rows, s);
+  else if (k.row_tiles == 1) launch_rows<4, 4, 1, false>(a, bf16_rows, s);
+  else launch_rows<4, 4, 2, false>(a, bf16_rows, s);
 }
 
 // a kernel of more than 64 KB of shared memory
@@ -978,7 +1042,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.xs = x_stride;
   a.xe = static_cast<const uint8_t*>(x_scales);
   a.xes = x_scales_stride;
-  const bool fused = bf16_rows && p.kernel == kRowsOf16;  // with the quantisation
+  const bool fused = bf16_rows && p.kernel == kRows && rows <= 16;  // with the quantisation
   if (bf16_rows && !fused) {
     uint8_t* codes = ws + p.part_bytes;
     uint8_t* exps = codes + padded((size_t)rows * in_features);
@@ -1008,7 +1072,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.nsplit = p.nsplit;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   int status = HS_OK;
-  if (p.kernel == kRowsOf16) {
+  if (p.kernel == kRows) {
     dispatch_rows(a, gate, fused, s);
     if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   } else if (epilogue == HS_LINEAR_PLAIN) {
