@@ -1107,16 +1107,18 @@ class Fp8Weight(NamedTuple):
 
 
 def _new_rows_fp8(x: torch.Tensor, rows: int, width: int) -> Fp8Rows:
+    codes = x.new_empty((rows, width), dtype=torch.float8_e4m3fn)
     groups = -(-width // 128)
+    if groups % 4 == 0:
+        return Fp8Rows(codes, x.new_empty((rows, groups), dtype=torch.float8_e8m0fnu))
     scales = x.new_empty((rows, -(-groups // 4) * 4), dtype=torch.float8_e8m0fnu)
-    return Fp8Rows(x.new_empty((rows, width), dtype=torch.float8_e4m3fn),
-                   scales if groups % 4 == 0 else scales[:, :groups])
+    return Fp8Rows(codes, scales[:, :groups])
 
 
 def _bf16_rows(t: torch.Tensor, most: int = 1 << 40) -> torch.Tensor:
     """t [rows, K] with rows that the kernels can read in 16-byte pieces: t or a copy."""
-    st = t.stride()
-    if st[1] != 1 or st[0] % 8 or not t.shape[1] <= st[0] <= most or t.data_ptr() % 16:
+    row, col = t.stride()
+    if col != 1 or row % 8 or not t.shape[1] <= row <= most or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -1126,15 +1128,17 @@ def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
     every 128 values of a row the smallest power of two s, at least 2^-126, with |x| <= 448
     s, and e4m3(x / s). NaN and infinities become NaN and take no part in the scale."""
     dev = _need_cuda(x)
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] < 1 or x.shape[1] % 16:
+    shape = x.shape
+    if len(shape) != 2 or x.dtype != torch.bfloat16 or shape[1] < 1 or shape[1] % 16:
         raise ValueError("quantize_rows_fp8 expects a 2-D bf16 input with a multiple of 16 "
                          "columns")
-    M, K = x.shape
+    M, K = shape
     out = _new_rows_fp8(x, M, K)
     if M:
         x = _bf16_rows(x)
-        _call(dev, "hs_quantize_rows_fp8", x.data_ptr(), x.stride(0), M, K, out.codes.data_ptr(),
-              K, out.scales.data_ptr(), out.scales.stride(0))
+        codes, scales = out
+        _call(dev, "hs_quantize_rows_fp8", x.data_ptr(), x.stride(0), M, K, codes.data_ptr(), K,
+              scales.data_ptr(), scales.stride(0))
     return out
 
 
@@ -1145,27 +1149,30 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     and go to 8 bits as in quantize_rows_fp8, without rounding to bf16 between. x [rows,
     H] bf16, H a multiple of 16."""
     dev = _need_cuda(x, weight, residual)
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] < 1 or x.shape[1] % 16:
+    shape = x.shape
+    if len(shape) != 2 or x.dtype != torch.bfloat16 or shape[1] < 1 or shape[1] % 16:
         raise ValueError("rmsnorm_fp8 expects a 2-D bf16 input with a multiple of 16 columns")
-    M, H = x.shape
+    M, H = shape
     if weight.shape != (H,) or weight.dtype != torch.bfloat16:
         raise ValueError("weight must be bf16 [H]")
+    res = residual
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != torch.bfloat16:
+        if residual.shape != shape or residual.dtype != torch.bfloat16:
             raise ValueError("residual must be bf16 with x's shape")
-        if M > 1 and residual.stride(0) < H * residual.stride(1) or residual.stride(1) < 1:
+        row, col = residual.stride()
+        if col < 1 or M > 1 and row < H * col:
             raise ValueError("residual is updated in place: its rows must not overlap")
+        res = _bf16_rows(residual)
     out = _new_rows_fp8(x, M, H)
     if not M:
         return out
     x = _bf16_rows(x)
     if weight.stride(0) != 1 or weight.data_ptr() % 16:
         weight = weight.clone(memory_format=torch.contiguous_format)
-    res = None if residual is None else _bf16_rows(residual)
+    codes, scales = out
     _call(dev, "hs_rmsnorm_fp8", x.data_ptr(), x.stride(0),
           None if res is None else res.data_ptr(), 0 if res is None else res.stride(0),
-          weight.data_ptr(), float(eps), M, H, out.codes.data_ptr(), H, out.scales.data_ptr(),
-          out.scales.stride(0))
+          weight.data_ptr(), eps, M, H, codes.data_ptr(), H, scales.data_ptr(), scales.stride(0))
     if res is not residual:
         residual.copy_(res)
     return out
@@ -1206,25 +1213,26 @@ def quantize_fp8(weight: torch.Tensor) -> Fp8Weight:
     return pack_fp8(codes.view(nb * 128, kb * 128)[:N, :K], scales)
 
 
-def _rows_fp8(x: Fp8Rows) -> Fp8Rows:
+def _rows_fp8(codes: torch.Tensor, scales: torch.Tensor):
     """Checks rows in 8 bits; returns them, or copies that the kernels can read."""
-    codes, scales = x.codes, x.scales
     if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu:
         raise TypeError("rows in 8 bits are float8_e4m3fn codes with float8_e8m0fnu scales")
-    if codes.dim() != 2 or scales.shape != (codes.shape[0], -(-codes.shape[1] // 128)):
+    shape = codes.shape
+    if len(shape) != 2 or scales.shape != (shape[0], -(-shape[1] // 128)):
         raise ValueError("rows in 8 bits are codes [rows, K] with scales [rows, ceil(K / 128)]")
-    (M, K), cst, sst = codes.shape, codes.stride(), scales.stride()
-    if cst[1] != 1 or cst[0] % 16 or not K <= cst[0] <= 1 << 22 or codes.data_ptr() % 16:
+    row, col = codes.stride()
+    if col != 1 or row % 16 or not shape[1] <= row <= 1 << 22 or codes.data_ptr() % 16:
         codes = codes.clone(memory_format=torch.contiguous_format)
     groups = scales.shape[1]
     whole = -(-groups // 4) * 4  # bytes of a row that the kernels may read
-    if sst[1] != 1 or sst[0] % 4 or not whole <= sst[0] <= 1 << 22 or scales.data_ptr() % 4 or (
-            groups != whole and scales.storage_offset() + (M - 1) * sst[0] + whole
+    row, col = scales.stride()
+    if col != 1 or row % 4 or not whole <= row <= 1 << 22 or scales.data_ptr() % 4 or (
+            groups != whole and scales.storage_offset() + (shape[0] - 1) * row + whole
             > scales.untyped_storage().nbytes()):
-        wide = scales.new_empty((M, whole))
+        wide = scales.new_empty((shape[0], whole))
         wide[:, :groups].copy_(scales)
         scales = wide
-    return Fp8Rows(codes, scales)
+    return codes, scales
 
 
 def linear_fp8(x, weight: Fp8Weight, *, swiglu: bool = False, quantize: bool = False,
@@ -1235,46 +1243,46 @@ def linear_fp8(x, weight: Fp8Weight, *, swiglu: bool = False, quantize: bool = F
     swiglu=True the weight is [2F, K] (gate | up), F a multiple of 16, and the result
     silu(gate) * up [rows, F]; with quantize=True beside it that result as Fp8Rows, rounded
     from fp32 once."""
-    rows8 = not isinstance(x, torch.Tensor)
-    xc, xs = (x.codes, x.scales) if rows8 else (x, None)
-    w, packed, scales = weight, weight.packed, weight.scales
-    dev = _need_cuda(xc, xs, packed, scales, out)
-    if rows8:
-        xc, xs = _rows_fp8(x)
-    elif x.dim() != 2 or x.dtype != torch.bfloat16:
-        raise ValueError("linear_fp8 expects Fp8Rows or a 2-D bf16 input")
-    M, K = xc.shape
-    if K != w.in_features or K % 16:
+    packed, scales, features = weight.packed, weight.scales, weight.out_features
+    if isinstance(x, torch.Tensor):
+        dev = _need_cuda(x, packed, scales, out)
+        codes, exps = x, None
+        if x.dim() != 2 or x.dtype != torch.bfloat16:
+            raise ValueError("linear_fp8 expects Fp8Rows or a 2-D bf16 input")
+    else:
+        dev = _need_cuda(x.codes, x.scales, packed, scales, out)
+        codes, exps = _rows_fp8(x.codes, x.scales)
+    M, K = codes.shape
+    if K != weight.in_features or K % 16:
         raise ValueError("in_features mismatch")
-    if quantize and (not swiglu or out is not None):
-        raise ValueError("quantize goes with swiglu, and returns new rows")
-    if swiglu and w.out_features % 32:
-        raise ValueError("swiglu needs gate and up halves of a multiple of 16 features")
-    tiles, steps = -(-w.out_features // 16), -(-K // 128)
+    tiles, steps = -(-features // 16), -(-K // 128)
     if packed.dtype != torch.uint8 or scales.dtype != torch.float32 or \
             packed.shape != (tiles, steps, 2, 64, 16) or scales.shape != (tiles, steps) or \
             not packed.is_contiguous() or not scales.is_contiguous():
         raise ValueError("weight is not laid out as pack_fp8 does")
-    N = w.out_features // 2 if swiglu else w.out_features
-    epi = L.HS_LINEAR_PLAIN
+    N, epi, exps_out, exps_row = features, L.HS_LINEAR_PLAIN, None, 0
+    if swiglu:
+        if features % 32:
+            raise ValueError("swiglu needs gate and up halves of a multiple of 16 features")
+        N, epi = features // 2, L.HS_LINEAR_SWIGLU
     if quantize:
-        rows, epi = _new_rows_fp8(xc, M, N), L.HS_LINEAR_SWIGLU_FP8
-        out = rows.codes
-    else:
-        if swiglu:
-            epi = L.HS_LINEAR_SWIGLU
-        if out is None:
-            out = packed.new_empty((M, N), dtype=torch.bfloat16)
-        elif out.shape != (M, N) or out.stride(1) != 1 or out.dtype != torch.bfloat16:
-            raise ValueError("out must be [rows, out_features] bf16 with contiguous rows")
+        if not swiglu or out is not None:
+            raise ValueError("quantize goes with swiglu, and returns new rows")
+        epi, rows = L.HS_LINEAR_SWIGLU_FP8, _new_rows_fp8(packed, M, N)
+        out, exps_out, exps_row = rows.codes, rows.scales.data_ptr(), rows.scales.stride(0)
+    elif out is None:
+        out = packed.new_empty((M, N), dtype=torch.bfloat16)
+    elif out.shape != (M, N) or out.stride(1) != 1 or out.dtype != torch.bfloat16:
+        raise ValueError("out must be [rows, out_features] bf16 with contiguous rows")
     if M:
-        if not rows8:
-            xc = _bf16_rows(xc, 1 << 22)
-        nbytes = L.lib().hs_linear_fp8_workspace_size(M, K, N, epi, not rows8)
+        if exps is None:
+            codes = _bf16_rows(codes, 1 << 22)
+        # (16 rows without quantize need no workspace)
+        nbytes = 0 if M <= 16 and not quantize else \
+            L.lib().hs_linear_fp8_workspace_size(M, K, N, epi, exps is None)
         ws = packed.new_empty(nbytes) if nbytes else None
-        _call(dev, "hs_linear_fp8", xc.data_ptr(), xc.stride(0),
-              xs.data_ptr() if rows8 else None, xs.stride(0) if rows8 else 0, packed.data_ptr(),
-              scales.data_ptr(), M, K, N, epi, out.data_ptr(), out.stride(0),
-              rows.scales.data_ptr() if quantize else None,
-              rows.scales.stride(0) if quantize else 0, ws.data_ptr() if nbytes else None, nbytes)
+        _call(dev, "hs_linear_fp8", codes.data_ptr(), codes.stride(0),
+              None if exps is None else exps.data_ptr(), 0 if exps is None else exps.stride(0),
+              packed.data_ptr(), scales.data_ptr(), M, K, N, epi, out.data_ptr(), out.stride(0),
+              exps_out, exps_row, ws.data_ptr() if nbytes else None, nbytes)
     return rows if quantize else out
