@@ -8,7 +8,9 @@ gate_up epilogue, q/k-norm + RoPE fused with the KV-cache store, and the paged
 attention; prefill-sized projections are hipBLASLt GEMMs through torch behind
 the standalone RMSNorm kernel. Weights are N(0, 0.02^2) in bf16 (no checkpoint
 is loaded); Qwen3Host.quantize_int4 turns the projections into 4-bit weights with
-group scales, which run behind the standalone RMSNorm kernel at every size.
+group scales, which run behind the standalone RMSNorm kernel at every size, and
+Qwen3Host.quantize_fp8 into e4m3 weights with a scale for every 128 x 128, which
+multiply rows in 8 bits: the RMSNorm and SwiGLU kernels write those.
 """
 from __future__ import annotations
 
@@ -71,12 +73,32 @@ class Int4Projection(nn.Module):
         self.out_features, self.in_features, self.group = w.out_features, w.in_features, w.group
 
 
-_INT4 = (Int4Projection, _ops.Int4Weight)  # the second where a caller has set one itself
+class Fp8Projection(nn.Module):
+    """An ops.Fp8Weight as a part of a model, as Int4Projection is an Int4Weight; it stands
+    for it in ops.linear_fp8."""
+
+    def __init__(self, w: _ops.Fp8Weight):
+        super().__init__()
+        self.packed = nn.Parameter(w.packed, requires_grad=False)
+        self.scales = nn.Parameter(w.scales, requires_grad=False)
+        self.out_features, self.in_features = w.out_features, w.in_features
 
 
-def _norm_proj(x, norm, eps, w, residual=None, swiglu=False):
-    """ops.linear_rmsnorm, or with a 4-bit weight the RMSNorm kernel and its projection
-    (the residual is then updated in place)."""
+# the second of each where a caller has set one itself
+_INT4 = (Int4Projection, _ops.Int4Weight)
+_FP8 = (Fp8Projection, _ops.Fp8Weight)
+
+
+def _norm_proj(x, norm, eps, w, residual=None, swiglu=False, quantize=False):
+    """ops.linear_rmsnorm, or with a 4- or 8-bit weight the RMSNorm kernel and its
+    projection (the residual is then updated in place). quantize: the result may be rows in
+    8 bits, which an e4m3 weight behind it takes."""
+    if isinstance(w, _FP8):
+        xn = _ops.rmsnorm_fp8(x, norm, eps, residual=residual)
+        # up to 16 rows the next projection's kernel takes them to 8 bits by itself
+        quantize = quantize and swiglu and x.shape[0] > 16
+        return (_ops.linear_fp8(xn, w, swiglu=swiglu, quantize=quantize),
+                x if residual is None else residual)
     if isinstance(w, _INT4):
         xn = _ops.rmsnorm(x, norm, eps, residual=residual)
         return _ops.linear_int4(xn, w, swiglu=swiglu), (x if residual is None else residual)
@@ -84,7 +106,18 @@ def _norm_proj(x, norm, eps, w, residual=None, swiglu=False):
 
 
 def _proj(x, w):
+    if isinstance(w, _FP8):
+        return _ops.linear_fp8(x, w)
     return _ops.linear_int4(x, w) if isinstance(w, _INT4) else _ops.linear(x, w)
+
+
+def _replace(module, names, kinds, make):
+    """module's weights of these names by make(weight), but those of `kinds`: all, or none
+    where one is refused."""
+    new = {name: make(w) for name in names if not isinstance(w := getattr(module, name), kinds)}
+    for name, q in new.items():
+        delattr(module, name)
+        setattr(module, name, q)
 
 
 class Rope(nn.Module):
@@ -108,6 +141,9 @@ class Rope(nn.Module):
             return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], -1).to(x.dtype)
 
         return rot(q), rot(k)
+
+
+_PROJECTIONS = ("qkv", "o", "gate_up", "down")
 
 
 class Qwen3Layer(nn.Module):
@@ -162,25 +198,28 @@ class Qwen3Layer(nn.Module):
             o = attn.attend_qkv(qkv, self.q_norm, self.k_norm, self.rope.cos_sin, positions,
                                 g.rms_eps)
         h = _proj(o.reshape(o.shape[0], -1), self.o)
-        x, residual = _norm_proj(h, self.ln2, g.rms_eps, self.gate_up, residual, swiglu=True)
+        x, residual = _norm_proj(h, self.ln2, g.rms_eps, self.gate_up, residual, swiglu=True,
+                                 quantize=isinstance(self.down, _FP8))
         h = _proj(x, self.down)
         return h, residual
 
     def quantize_int4(self, group: int = 128):
-        """The four projections to 4-bit weights (ops.quantize_int4): all of them, or none
-        where one refuses the group."""
-        new = {name: Int4Projection(_ops.quantize_int4(w, group))
-               for name in ("qkv", "o", "gate_up", "down")
-               if not isinstance(w := getattr(self, name), _INT4)}
-        for name, q in new.items():
-            delattr(self, name)
-            setattr(self, name, q)
+        """The four projections to 4-bit weights (ops.quantize_int4): all of them that are
+        in bf16, or none where one refuses the group."""
+        _replace(self, _PROJECTIONS, _INT4 + _FP8,
+                 lambda w: Int4Projection(_ops.quantize_int4(w, group)))
+
+    def quantize_fp8(self):
+        """The four projections to e4m3 weights (ops.quantize_fp8): all of them that are in
+        bf16, or none where one is refused."""
+        _replace(self, _PROJECTIONS, _INT4 + _FP8,
+                 lambda w: Fp8Projection(_ops.quantize_fp8(w)))
 
     def forward_reference(self, positions, h, residual):
         """Eager PyTorch restatement of the same layer (used by tests; bf16 weights)."""
         g = self.g
-        if any(isinstance(w, _INT4) for w in (self.qkv, self.o, self.gate_up, self.down)):
-            raise TypeError("the restatement takes bf16 weights; this layer's are in 4 bits")
+        if any(isinstance(getattr(self, name), _INT4 + _FP8) for name in _PROJECTIONS):
+            raise TypeError("the restatement takes bf16 weights; this layer's are in 4 or 8 bits")
         if residual is None:
             x, residual = rms_norm(h, self.ln1, g.rms_eps), h
         else:
@@ -246,10 +285,20 @@ class Qwen3Host(nn.Module):
         A model that shares this one's weights keeps those it was built with."""
         for layer in self.layers:
             layer.quantize_int4(group)
-        if lm_head and not isinstance(self.lm_head, _INT4):
-            q = Int4Projection(_ops.quantize_int4(self.lm_head, group))
-            del self.lm_head
-            self.lm_head = q
+        if lm_head:
+            _replace(self, ("lm_head",), _INT4 + _FP8,
+                     lambda w: Int4Projection(_ops.quantize_int4(w, group)))
+        return self
+
+    def quantize_fp8(self, lm_head: bool = False) -> "Qwen3Host":
+        """Every layer's bf16 projections (and with lm_head=True the LM head; a tied
+        embedding stays as it is) to e4m3 weights with one scale per 128 x 128. A model that
+        shares this one's weights keeps those it was built with."""
+        for layer in self.layers:
+            layer.quantize_fp8()
+        if lm_head:
+            _replace(self, ("lm_head",), _INT4 + _FP8,
+                     lambda w: Fp8Projection(_ops.quantize_fp8(w)))
         return self
 
     def attention_layers(self):
