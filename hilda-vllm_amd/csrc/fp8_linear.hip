@@ -234,8 +234,9 @@ constexpr int kPast = INT32_MAX;            // a byte offset past any buffer: re
 constexpr int kRange = INT32_MAX - 255;
 constexpr int kStage = kBig * kStep;        // bytes of a step's rows, and of its weights
 constexpr int kChunk = 64;                  // steps whose exponents and scales are held
-// shared memory: two stages of rows, two of weights, the chunk's exponents [four steps][row]
-constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kBigBytes = kAtE + kChunk * kBig;
+// shared memory: two stages of rows, two of weights, the chunk's exponents and scales
+constexpr int kAtW = 2 * kStage, kAtE = 4 * kStage, kAtS = kAtE + kChunk * kBig;
+constexpr int kBigBytes = kAtS + kChunk * 4 * 16;
 
 // 16 bytes a lane from a buffer straight to LDS, at lds + 16 lane. The compiler does not see
 // the write: the wait before the barrier behind a step covers it. (Through the builtin it
@@ -249,12 +250,19 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, int offset
                :: "s"(lds), "v"(offset), "s"(from), "s"(at), "n"(kOffset)
                : "memory");
 }
+// 4 bytes a lane, at lds + 4 lane
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t from, int offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(offset), "s"(from)
+               : "memory");
+}
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 // waits for the wave's LDS traffic and all but its last kLoads loads, then for the other waves
 template <int kLoads>
 __device__ __forceinline__ void step_barrier() {
+  static_assert(kLoads < 16, "the count's low four bits");
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0070 | kLoads);  // vmcnt(kLoads) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
@@ -381,6 +389,64 @@ __device__ __forceinline__ void place_of(const Fp8Args& a, int o, int& col, int&
   col = in / tall;
 }
 
+// A chunk's exponents to shared memory at `e`, a word of four steps a row, [four steps][row], and
+// its weights' scales at `s`, [gate, up][step][output tile]: SLOTS weight tiles from output tile
+// u0, ROWS rows from r0 (the last ones are `high`), of WAVES waves. Past the last step both are
+// zeros, but for bytes of a word that it ends in (trim).
+template <bool kGate, int ROWS, int SLOTS, int WAVES>
+__device__ __forceinline__ void load_chunk(const Fp8Args& a, int first, int u0, int r0, int high,
+                                           uint32_t e, uint32_t s) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const auto eb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.xe + r0 * a.xes), 0, (high - 1) * (int)a.xes + (a.steps + 3) / 4 * 4,
+      0x00027000);
+  static_assert(ROWS / 4 % WAVES == 0, "");
+#pragma unroll
+  for (int i = 0; i < ROWS / 4 / WAVES; ++i) {
+    const int j = i * WAVES + wave, d = 64 * j + lane, step = first + d / ROWS * 4;
+    load_lds4(eb, step < a.steps ? d % ROWS * (int)a.xes + step : kPast, e + 256 * j);
+  }
+  constexpr int OUT = kGate ? SLOTS / 2 : SLOTS;
+#pragma unroll
+  for (int i = 0; i < (SLOTS + WAVES - 1) / WAVES; ++i) {
+    const int j = i * WAVES + wave;
+    if (SLOTS % WAVES && j >= SLOTS) break;
+    const int half = kGate ? j / OUT : 0, d = 64 * (j - half * OUT) + lane;
+    const int step = first + d / OUT;
+    const auto sb = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(a.sc + (u0 + half * (int64_t)a.up) * a.steps), 0, kRange, 0x00027000);
+    const int tile = min(d % OUT, a.units - 1 - u0);
+    load_lds4(sb, step < a.steps ? 4 * (tile * a.steps + step) : kPast, s + 256 * j);
+  }
+}
+// after the chunk has landed and all waves know: zeros for what follows the last step in its word
+template <int ROWS>
+__device__ __forceinline__ void trim_chunk(const Fp8Args& a, int first, uint8_t* e) {
+  const int left = a.steps - first;
+  if (left >= kChunk || left % 4 == 0) return;
+  if (threadIdx.x < ROWS)
+    reinterpret_cast<uint32_t*>(e)[left / 4 * ROWS + threadIdx.x] &= (1u << 8 * (left % 4)) - 1;
+  __syncthreads();
+}
+// N consecutive scales of a wave's tiles at p
+template <int N>
+__device__ __forceinline__ void read_scales(const uint8_t* p, float* out) {
+  static_assert(N == 1 || N == 2 || N == 4, "");
+  if constexpr (N == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    out[0] = v.x; out[1] = v.y; out[2] = v.z; out[3] = v.w;
+  } else if constexpr (N == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    out[0] = v.x; out[1] = v.y;
+  } else {
+    out[0] = *reinterpret_cast<const float*>(p);
+  }
+}
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+
 template <int kEpilogue>
 __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   constexpr bool kGate = kEpilogue != HS_LINEAR_PLAIN;
@@ -433,7 +499,6 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     load(step, Index<4>()); load(step, Index<5>());
   };
   auto load_b = [&](int step) { load(step, Index<6>()); load(step, Index<7>()); };
-  float sc[4];  // the scales of the wave's tiles, a step a lane
 
   // operands from LDS
   const uint8_t* sx0 = s_bytes + (128 * wr + m) * kStep + 16 * swizzle(m, g);
@@ -460,34 +525,26 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
 #pragma unroll
     for (int t = 0; t < 8; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
   }
-  // the chunk's exponents and scales: half of a row's words a thread
-  auto load_chunk = [&](int first) {
-    const int row = threadIdx.x & (kBig - 1), q0 = (int)(threadIdx.x >> 8) * (kChunk / 8);
-    const uint8_t* from = a.xe + (r0 + min(row, high - 1)) * a.xes + first;
-    uint32_t word[kChunk / 8];
-#pragma unroll
-    for (int i = 0; i < kChunk / 8; ++i) {
-      const int at = 4 * (q0 + i), left = a.steps - first - at;  // (past the last step: zeros)
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(
-          from + min(at, (a.steps - 1 - first) & ~3));
-      word[i] = left >= 4 ? v : left > 0 ? v & ((1u << 8 * left) - 1) : 0;
+  // the scales of the wave's tiles
+  const uint8_t* ss = s_bytes + kAtS + 4 * (kGate ? 2 : 4) * wf;
+  auto read_scale = [&](int in_chunk, float (&v)[4]) {
+    if constexpr (kGate) {
+      read_scales<2>(ss + 32 * in_chunk, v);
+      read_scales<2>(ss + 32 * kChunk + 32 * in_chunk, v + 2);
+    } else {
+      read_scales<4>(ss + 64 * in_chunk, v);
     }
-#pragma unroll
-    for (int f = 0; f < 4; ++f)
-      sc[f] = a.sc[(int64_t)tile_of(4 * wf + f) * a.steps + min(first + lane, a.steps - 1)];
-    // (waited for here, not at every use among the loads in flight)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-#pragma unroll
-    for (int i = 0; i < kChunk / 8; ++i)
-      *reinterpret_cast<uint32_t*>(s_bytes + kAtE + (q0 + i) * 4 * kBig + 4 * row) = word[i];
   };
+  auto chunk = [&](int first) {
+    load_chunk<kGate, kBig, 16, 8>(a, first, u0, r0, high, lds + kAtE, lds + kAtS);
+  };
+  chunk(0);
   load_a(0);
   load_b(0);
   load_a(1);
   load_b(1);
-  load_chunk(0);
-  step_barrier<0>();
+  step_barrier<8>();
+  trim_chunk<kBig>(a, 0, s_bytes + kAtE);
   i32x8_t x[3], w[4];
   uint32_t e[3];
   x[2] = read_x(0, 0);
@@ -503,13 +560,10 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   auto one = [&](int step, int quad, auto quarter) {
     constexpr int kQ = decltype(quarter)::value;
     constexpr int kReg[8] = {2, 0, 1, 0, 1, 2, 0, 1};  // of the row tiles
-    float before[4];
+    float before[4], next[4];
+    read_scale(step & (kChunk - 1), next);
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      before[f] = scale[f];
-      scale[f] = __uint_as_float(
-          __builtin_amdgcn_readlane(__float_as_uint(sc[f]), step & (kChunk - 1)));
-    }
+    for (int f = 0; f < 4; ++f) before[f] = scale[f];
     // tile and weight of product i: the last two row tiles by weights
     auto tile = [](int i) { return i < 24 ? i >> 2 : 6 + (i & 1); };
     auto weight = [](int i) { return i < 24 ? i & 3 : (i - 24) >> 1; };
@@ -520,6 +574,10 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
     auto product = [&](int i) {
       const int t = tile(i), f = weight(i), r = kReg[t];
       part[i & 3] = mfma<kQ>(w[f], x[r], e[r]);
+      if (i == 2) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) scale[q] = uniform(next[q]);
+      }
       const int j = (i + 29) & 31;
       acc[weight(j)][tile(j)] += (i < 3 ? before : scale)[weight(j)] * part[j & 3];
       __builtin_amdgcn_sched_barrier(0);
@@ -562,8 +620,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_fp8_big(Fp8Args a) {
   for (int first = 0; first < a.steps; first += kChunk) {
     if (first) {
       step_barrier<0>();  // the last chunk's exponents have been read
-      load_chunk(first);
+      chunk(first);
       step_barrier<0>();
+      trim_chunk<kBig>(a, first, s_bytes + kAtE);
     }
     e[2] = read_e(0, 0);
     // four steps at a time; past the last one the rows are zeros, and so is their scale
@@ -593,7 +652,8 @@ struct Tile {
   static constexpr int kRows = 16 * RT * WR, kSlots = FT * WF;  // rows, 16-feature tiles
   static constexpr int kXLoads = kRows / 8 / kWaves, kWLoads = 2 * kSlots / kWaves;  // a wave's
   static constexpr int kXBytes = kRows * kStep, kStageBytes = kXBytes + kSlots * 16 * kStep;
-  static constexpr int kAtE = S * kStageBytes, kBytes = kAtE + kChunk * kRows;
+  static constexpr int kAtE = S * kStageBytes, kAtS = kAtE + kChunk * kRows;
+  static constexpr int kBytes = kAtS + kChunk * 4 * kSlots;
   static_assert(kXLoads * 8 * kWaves == kRows && (kWLoads == 2 || kWLoads == 4) &&
                 kWLoads * kWaves == 2 * kSlots, "");
   static_assert(kRows * (32 * kSlots + 16) <= kBytes && kBytes <= 160 * 1024, "");
@@ -647,28 +707,11 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
     else load_lds<0>(b, 16 * lane, 16 * kStep * step, tw);
   };
   auto stage = [&](int i) { return lds + i * T::kStageBytes; };
-  float sc[FT];
-  auto load_chunk = [&](int first) {
-    constexpr int kWords = kChunk / 4 * T::kRows / T::kThreads;
-    const int row = threadIdx.x % T::kRows, q0 = (int)threadIdx.x / T::kRows * kWords;
-    const uint8_t* from = a.xe + (r0 + min(row, high - 1)) * a.xes + first;
-    uint32_t word[kWords];
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      const int at = 4 * (q0 + i), left = a.steps - first - at;  // (past the last step: zeros)
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(
-          from + min(at, (a.steps - 1 - first) & ~3));
-      word[i] = left >= 4 ? v : left > 0 ? v & ((1u << 8 * left) - 1) : 0;
-    }
-#pragma unroll
-    for (int f = 0; f < FT; ++f)
-      sc[f] = a.sc[(int64_t)tile_of(FT * wf + f) * a.steps + min(first + lane, a.steps - 1)];
-    // (waited for here, not at every use among the loads in flight)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-#pragma unroll
-    for (int i = 0; i < kWords; ++i)
-      *reinterpret_cast<uint32_t*>(s_bytes + T::kAtE + ((q0 + i) * T::kRows + row) * 4) = word[i];
+  const uint8_t* ss = s_bytes + T::kAtS + 4 * OT * wf;  // the scales of the wave's tiles
+  constexpr int kOutTiles = OT * T::WF;
+  auto chunk = [&](int first) {
+    load_chunk<kGate, T::kRows, T::kSlots, T::kWaves>(a, first, u0, r0, high, lds + T::kAtE,
+                                                      lds + T::kAtS);
   };
 
   f32x4_t acc[FT][RT];
@@ -676,6 +719,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[f][t] = f32x4_t{0, 0, 0, 0};
+  chunk(begin);
 #pragma unroll
   for (int i = 0; i < T::S * kLoads; ++i) load(begin + i / kLoads, stage(i / kLoads), i % kLoads);
   const int in_rows = 16 * RT * wr + m;
@@ -696,8 +740,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
                             *reinterpret_cast<const uint4*>(sx1 + at + 16 * (i - FT) * kStep));
     }
   };
-  load_chunk(begin);
   step_barrier<(T::S - 1) * kLoads>();
+  trim_chunk<T::kRows>(a, begin, s_bytes + T::kAtE);
   Operands even, odd;
 #pragma unroll
   for (int i = 0; i < kReads; ++i) read(0, even, i);
@@ -716,9 +760,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
     now = now == T::S - 1 ? 0 : now + 1;
     const int shift = 8 * (in_chunk & 3);
     float scale[FT];
-#pragma unroll
-    for (int f = 0; f < FT; ++f)
-      scale[f] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc[f]), in_chunk));
+    read_scales<OT>(ss + 4 * kOutTiles * in_chunk, scale);
+    if constexpr (kGate)
+      read_scales<OT>(ss + 4 * kOutTiles * (kChunk + in_chunk), scale + OT);
     // products, each added three products later
     f32x4_t part[4];
     auto add = [&](int j) { acc[j % FT][j / FT] += scale[j % FT] * part[j & 3]; };
@@ -742,7 +786,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
   for (int first = begin; first < end; first += kChunk) {
     if (first != begin) {
       step_barrier<0>();  // the last chunk's exponents have been read
-      load_chunk(first);
+      chunk(first);
+      step_barrier<0>();
+      trim_chunk<T::kRows>(a, first, s_bytes + T::kAtE);
     }
     // two steps at a time: past the last one the rows are zeros, and so is their scale
     const int count = min(kChunk, end - first);
