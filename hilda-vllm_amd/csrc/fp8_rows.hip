@@ -176,10 +176,12 @@ void launch_norm(const NormArgs& a, hipStream_t s) {
                      dim3(T < 256 ? 256 : T), 0, s, a);
 }
 
+constexpr int kMaxRows = 1 << 22;  // 1024 threads each in one grid
+
 // the limits that both entry points share: whole 16-byte pieces of bf16, 8-byte pieces of codes
 int rows_status(const void* x, int64_t xs, int rows, int width, const void* codes, int64_t cs,
                 int64_t ss) {
-  if (width % 16 || width > (1 << 24) || rows > (1 << 24)) return HS_ERR_UNSUPPORTED;
+  if (width % 16 || width > (1 << 24) || rows > kMaxRows) return HS_ERR_UNSUPPORTED;
   if ((xs % 8) || (cs % 8) || xs < width || cs < width || ss < (width + kFp8Group - 1) / kFp8Group)
     return HS_ERR_UNSUPPORTED;
   if (((uintptr_t)x & 15) || ((uintptr_t)codes & 7)) return HS_ERR_UNSUPPORTED;
@@ -201,7 +203,7 @@ int hs_quantize_rows_fp8(const void* x, int64_t x_stride, int rows, int width, v
   if (status != HS_OK) return status;
   const int groups = (width + kFp8Group - 1) / kFp8Group;
   const int64_t blocks = ((int64_t)rows * groups * 16 + kQuantThreads - 1) / kQuantThreads;
-  if (blocks > INT32_MAX) return HS_ERR_UNSUPPORTED;
+  if (blocks * kQuantThreads > UINT32_MAX) return HS_ERR_UNSUPPORTED;  // a grid's threads
   hipLaunchKernelGGL(k_quantize_rows, dim3((unsigned)blocks), dim3(kQuantThreads), 0,
                      reinterpret_cast<hipStream_t>(stream), static_cast<const uint16_t*>(x),
                      x_stride, rows, width, groups, static_cast<uint8_t*>(codes), codes_stride,

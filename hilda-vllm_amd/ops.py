@@ -1147,7 +1147,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     """rmsnorm to rows in 8 bits (hs_rmsnorm_fp8): with h = x (+ residual), the residual
     updated in place to bf16(h), the rows are h * rsqrt(mean(h^2) + eps) * weight in fp32
     and go to 8 bits as in quantize_rows_fp8, without rounding to bf16 between. x [rows,
-    H] bf16, H a multiple of 16."""
+    H] bf16, H a multiple of 16; x and residual may be the same rows, but not overlap
+    otherwise."""
     dev = _need_cuda(x, weight, residual)
     shape = x.shape
     if len(shape) != 2 or x.dtype != torch.bfloat16 or shape[1] < 1 or shape[1] % 16:
@@ -1172,7 +1173,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     codes, scales = out
     _call(dev, "hs_rmsnorm_fp8", x.data_ptr(), x.stride(0),
           None if res is None else res.data_ptr(), 0 if res is None else res.stride(0),
-          weight.data_ptr(), eps, M, H, codes.data_ptr(), H, scales.data_ptr(), scales.stride(0))
+          weight.data_ptr(), float(eps), M, H, codes.data_ptr(), H, scales.data_ptr(),
+          scales.stride(0))
     if res is not residual:
         residual.copy_(res)
     return out

@@ -555,12 +555,14 @@ int hs_linear_int4(const void* x, int64_t x_stride, const void* packed, const vo
 /* every 128 values of a row, [rows, ceil(width / 128)]: value = code * scale. A   */
 /* group's scale is the smallest power of two s, at least 2^-126, with |v| <= 448 s */
 /* for its finite values; the code is v / s rounded to nearest even, once, from     */
-/* fp32, and NaN for NaN and the infinities. width a multiple of 16, strides in     */
-/* elements: of x a multiple of 8, of codes of 8; x 16-byte, codes 8-byte aligned.  */
+/* fp32, and NaN for NaN and the infinities. Up to 2^22 rows (and 2^35 values for    */
+/* hs_quantize_rows_fp8), width a multiple of 16, strides in elements: of x a        */
+/* multiple of 8, of codes of 8; x 16-byte, codes 8-byte aligned.                    */
 /* hs_quantize_rows_fp8: of bf16 rows x.                                            */
 /* hs_rmsnorm_fp8: of h * rsqrt(mean(h^2) + eps) * weight in fp32, h = x (+         */
 /* residual); with residual != NULL the residual row is replaced by bf16(h) (its    */
-/* stride a multiple of 8, it and weight bf16 and 16-byte aligned).                 */
+/* stride a multiple of 8, it and weight bf16 and 16-byte aligned; x and residual    */
+/* are the same rows or do not overlap).                                            */
 int hs_quantize_rows_fp8(const void* x, int64_t x_stride, int rows, int width, void* codes,
                          int64_t codes_stride, void* scales, int64_t scales_stride, void* stream);
 int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t residual_stride,

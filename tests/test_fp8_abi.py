@@ -120,6 +120,7 @@ def test_refusals(hv):
         assert f(rows=0, x=None) == 0
         assert f(x=None) == f(c=None) == f(s=None) == f(rows=-1) == f(k=0) == -1
         assert f(k=248) == f(xs=248) == f(xs=260) == f(cs=248) == f(cs=260) == f(ss=1) == -4
-        assert f(x=p + 8) == f(c=p + 4) == f(rows=(1 << 24) + 1) == -4
+        assert f(x=p + 8) == f(c=p + 4) == f(rows=(1 << 22) + 1) == -4
+    assert quantize(rows=1 << 22, k=1 << 20, xs=1 << 20, cs=1 << 20, ss=1 << 13) == -4
     assert norm(w=None) == -1
     assert norm(w=p + 8) == norm(res=p + 8) == norm(rs=248) == norm(rs=260) == -4

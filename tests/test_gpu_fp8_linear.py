@@ -144,6 +144,50 @@ def test_rows_of_any_size(hv, cuda, rows):
     assert bool(((got - y).abs() <= tol + 2.0 ** -8 * (y.abs() + tol)).all())
 
 
+@pytest.mark.parametrize("rows", [3, 40, 200, 1100])
+def test_scales_at_their_ends(hv, cuda, rows):
+    """A scale that is NaN (byte 255) makes its row NaN and no other; the least ones (bytes 0
+    and 1) stand for less than 2^-100 here; bytes behind a row's last scale are not read as
+    scales. (640 inputs are five scales, kept in eight bytes.)"""
+    gen = torch.Generator().manual_seed(rows)
+    codes, scales = _weights(gen, 200, 640)
+    w = hv.ops.pack_fp8(codes.to(cuda), scales.to(cuda))
+    xc = torch.randn(rows, 640, generator=gen).mul(100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    e = torch.full((rows, 8), 255, dtype=torch.uint8)
+    e[:, :5] = 120 + torch.randint(0, 9, (rows, 5), generator=gen).to(torch.uint8)
+
+    def run():
+        es = e.to(cuda).view(torch.float8_e8m0fnu)[:, :5]
+        return hv.ops.linear_fp8(hv.ops.Fp8Rows(xc.to(cuda), es), w)
+
+    want = run()
+    assert bool(torch.isfinite(want).all())
+    e[1, 4] = 255
+    e[rows - 1, 0] = 255
+    e[0, :5] = torch.tensor([0, 1, 0, 1, 0], dtype=torch.uint8)
+    got = run()
+    assert bool(got[[1, rows - 1]].isnan().all())
+    assert bool((got[0].abs() < 2.0 ** -100).all())
+    rest = [r for r in range(2, rows - 1)]
+    assert torch.equal(got[rest], want[rest])
+
+
+def test_one_row_of_many_sizes(hv, cuda):
+    """A row's result is the same in every batch that one kernel serves, and near itself in all
+    (the sums' order differs): the first rows of batches around the kernels' limits."""
+    gen = torch.Generator().manual_seed(77)
+    codes, scales = _weights(gen, 528, 1040)
+    w = hv.ops.pack_fp8(codes.to(cuda), scales.to(cuda))
+    x = _rows(gen, 2100, 1040)
+    rows = hv.ops.quantize_rows_fp8(x.to(cuda))
+    y, tol = _reference(ref.values(*ref.rows(x[:1])), codes, scales, "plain", 528)
+    for m in (1, 8, 9, 16, 17, 32, 33, 64, 65, 127, 129, 256, 300, 512, 513, 1024, 2100):
+        part = hv.ops.Fp8Rows(rows.codes[:m], rows.scales[:m])
+        got = hv.ops.linear_fp8(part, w)
+        assert bool(((got[:1].double().cpu() - y).abs() <= tol + 2.0 ** -8 * (y.abs() + tol)).all())
+        assert bool(torch.isfinite(got).all()), m
+
+
 def test_quantize_fp8(hv, cuda):
     """The product is that of the weight the codes stand for, at most half a step off."""
     gen = torch.Generator().manual_seed(5)

@@ -107,6 +107,17 @@ def test_rmsnorm_fp8(hv, cuda, size, residual):
                     assert bool((wide[:, :at] == 7).all() and (wide[:, at + k:] == 7).all())
 
 
+def test_rmsnorm_fp8_of_its_own_residual(hv, cuda):
+    """x and the residual the same rows: h = 2 x, in place."""
+    x = torch.randn(9, 1040, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16)
+    w = torch.ones(1040, dtype=torch.bfloat16)
+    h, y, tol = _norm(x, x, w, 1e-6)
+    both = x.to(cuda)
+    got = hv.ops.rmsnorm_fp8(both, w.to(cuda), 1e-6, residual=both)
+    ref.check_rows(got.codes, got.scales, y, tol)
+    assert torch.equal(both.cpu(), (2 * x.float()).to(torch.bfloat16))
+
+
 def test_rmsnorm_fp8_limits(hv, cuda):
     """Rows of zeros, one that holds a NaN and one with an infinity: the others stay."""
     gen = torch.Generator().manual_seed(4)
