@@ -890,6 +890,7 @@ constexpr TileTime kTileTimes[] = {{0, 0, 0, 0, 0},
 
 struct Fp8Plan {
   Kernel kernel;
+  bool fused;          // bf16 rows go to 8 bits in the projection's kernel
   int split_steps, nsplit;
   size_t part_bytes;   // sums of split steps
   size_t codes_bytes;  // codes of bf16 rows
@@ -961,7 +962,8 @@ Fp8Plan plan_of(int rows, int K, int N, int epilogue, bool bf16_rows) {
   const bool whole = p.kernel == k256x256 || p.kernel == k256x128;  // of a group of outputs
   if (p.nsplit > 1 || (eight && !whole))
     p.part_bytes = padded((size_t)p.nsplit * rows * units * (gate ? 32 : 16) * sizeof(float));
-  if (bf16_rows && !(p.kernel == kRows && rows <= 16))
+  p.fused = bf16_rows && p.kernel == kRows && rows_of(rows, steps, units, gate).row_tiles == 1;
+  if (bf16_rows && !p.fused)
     p.codes_bytes = padded((size_t)rows * K) + padded((size_t)rows * scales_row(K));
   p.bytes = p.part_bytes + p.codes_bytes;
   return p;
@@ -1090,8 +1092,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   a.xs = x_stride;
   a.xe = static_cast<const uint8_t*>(x_scales);
   a.xes = x_scales_stride;
-  const bool fused = bf16_rows && p.kernel == kRows && rows <= 16;  // with the quantisation
-  if (bf16_rows && !fused) {
+  if (bf16_rows && !p.fused) {
     uint8_t* codes = ws + p.part_bytes;
     uint8_t* exps = codes + padded((size_t)rows * in_features);
     const int status = hs_quantize_rows_fp8(x, x_stride, rows, in_features, codes, in_features,
@@ -1121,7 +1122,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   int status = HS_OK;
   if (p.kernel == kRows) {
-    dispatch_rows(a, gate, fused, s);
+    dispatch_rows(a, gate, p.fused, s);
     if (hipGetLastError() != hipSuccess) return HS_ERR_LAUNCH;
   } else if (epilogue == HS_LINEAR_PLAIN) {
     status = launch_tiles<HS_LINEAR_PLAIN>(a, p.kernel, s);
