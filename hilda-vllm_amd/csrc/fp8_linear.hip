@@ -857,10 +857,10 @@ __global__ __launch_bounds__(kJoinThreads) void k_fp8_join(Fp8Args a) {
     if (n < a.N) *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.y) + row * a.ys + n) = c;
     if ((e & 15) == 0) a.ye[row * a.yes + group] = (uint8_t)byte;
   } else {
+    uint16_t h[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (n + i < a.N) a.y[row * a.ys + n + i] = result<kGate>(v[i], u[i]);
-    }
+    for (int i = 0; i < 8; ++i) h[i] = result<kGate>(v[i], u[i]);
+    store8(a, row, n, pack8(h));
   }
 }
 
