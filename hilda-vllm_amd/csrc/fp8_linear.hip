@@ -663,7 +663,7 @@ template <int kEpilogue, class T>
 __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
   constexpr bool kGate = kEpilogue != HS_LINEAR_PLAIN;
   constexpr int FT = T::FT, RT = T::RT, OT = kGate ? FT / 2 : FT;
-  extern __shared__ uint4 s_all[];  // [stage][x: row, piece | w: tile, half, lane], exponents, bad
+  extern __shared__ uint4 s_all[];  // [stage][x: row, piece | w: tile, half, lane], exponents, scales
   uint8_t* s_bytes = reinterpret_cast<uint8_t*>(s_all);
   const uint32_t lds = lds_address(s_all);
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -1043,6 +1043,10 @@ bool sizes_ok(int rows, int K, int N, int epilogue) {
   return rows >= 1 && K >= 1 && N >= 1 && epilogue >= HS_LINEAR_PLAIN &&
          epilogue <= HS_LINEAR_SWIGLU_FP8;
 }
+// grids and 32-bit offsets of the kernels
+bool sizes_fit(int rows, int K, int N) {
+  return rows <= kMaxRows && K <= 1 << 22 && N <= 1 << 24;
+}
 
 }  // namespace
 }  // namespace hs
@@ -1053,7 +1057,9 @@ extern "C" {
 
 size_t hs_linear_fp8_workspace_size(int rows, int in_features, int out_features, int epilogue,
                                     int bf16_rows) {
-  if (!sizes_ok(rows, in_features, out_features, epilogue) || rows > kMaxRows) return 0;
+  if (!sizes_ok(rows, in_features, out_features, epilogue) ||
+      !sizes_fit(rows, in_features, out_features))
+    return 0;
   return plan_of(rows, in_features, out_features, epilogue, bf16_rows != 0).bytes;
 }
 
@@ -1069,9 +1075,7 @@ int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t
   if (in_features % 16) return HS_ERR_UNSUPPORTED;
   // gate and up halves start at a tile each
   if (gate && out_features % 16) return HS_ERR_UNSUPPORTED;
-  // grids and 32-bit offsets of the kernels
-  if (rows > kMaxRows || in_features > (1 << 22) || out_features > (1 << 24))
-    return HS_ERR_UNSUPPORTED;
+  if (!sizes_fit(rows, in_features, out_features)) return HS_ERR_UNSUPPORTED;
   const bool bf16_rows = !x_scales;
   if ((x_stride % (bf16_rows ? 8 : 16)) || x_stride < in_features || x_stride > (1 << 22))
     return HS_ERR_UNSUPPORTED;

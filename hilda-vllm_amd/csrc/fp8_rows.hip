@@ -176,7 +176,7 @@ void launch_norm(const NormArgs& a, hipStream_t s) {
                      dim3(T < 256 ? 256 : T), 0, s, a);
 }
 
-constexpr int kMaxRows = 1 << 22;  // 1024 threads each in one grid
+constexpr int kMaxRows = (1 << 22) - 1;  // 1024 threads each in a grid of less than 2^32
 
 // the limits that both entry points share: whole 16-byte pieces of bf16, 8-byte pieces of codes
 int rows_status(const void* x, int64_t xs, int rows, int width, const void* codes, int64_t cs,

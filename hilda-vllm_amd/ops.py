@@ -5,7 +5,7 @@ current HIP stream to libhilda_spec.so and raises RuntimeError on any non-zero
 status. Workspaces are allocated once per (device, kind) and reused, and calls on
 one device are ordered by the current stream; the entry points whose workspace
 needs no preparation (store_kvcache_scaled, verify_attention_scaled, linear_int4,
-token_logprobs) take one of the call's own.
+linear_fp8, token_logprobs) take one of the call's own.
 """
 from __future__ import annotations
 

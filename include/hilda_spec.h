@@ -555,7 +555,7 @@ int hs_linear_int4(const void* x, int64_t x_stride, const void* packed, const vo
 /* every 128 values of a row, [rows, ceil(width / 128)]: value = code * scale. A   */
 /* group's scale is the smallest power of two s, at least 2^-126, with |v| <= 448 s */
 /* for its finite values; the code is v / s rounded to nearest even, once, from     */
-/* fp32, and NaN for NaN and the infinities. Up to 2^22 rows (and 2^35 values for    */
+/* fp32, and NaN for NaN and the infinities. Less than 2^22 rows (and 2^35 values in */
 /* hs_quantize_rows_fp8), width a multiple of 16, strides in elements: of x a        */
 /* multiple of 8, of codes of 8; x 16-byte, codes 8-byte aligned.                    */
 /* hs_quantize_rows_fp8: of bf16 rows x.                                            */
@@ -570,8 +570,9 @@ int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t resi
                    int64_t codes_stride, void* scales, int64_t scales_stride, void* stream);
 
 /* Projection of rows in 8 bits by e4m3 weights with a scale for every block of 128 */
-/* x 128 (no counterpart in the reference), up to 2^20 rows: out[r, n] = sum_k      */
-/* x[r, k] * code[n, k] * scale[n / 128, k / 128], fp32 accumulation, bf16 out.     */
+/* x 128 (no counterpart in the reference), up to 2^20 rows, 2^22 inputs and 2^24    */
+/* outputs: out[r, n] = sum_k x[r, k] * code[n, k] * scale[n / 128, k / 128], fp32   */
+/* accumulation, bf16 out.                                                          */
 /* HS_LINEAR_SWIGLU: weight [2 * out_features, in_features] gate | up, out =        */
 /* silu(gate) * up rounded once; HS_LINEAR_SWIGLU_FP8: the same product as rows in  */
 /* 8 bits (out: codes, out_scales: their exponent bytes); out_features a multiple   */
@@ -582,10 +583,11 @@ int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t resi
 /* + 16 (lane / 16) + j. scales: f32 [tiles][steps], the scale of the tile's block.  */
 /* Rows past the last and inputs past in_features are padded with zeros.             */
 /* Strides in elements: x_stride a multiple of 16 (bf16: 8), at most 2^22;           */
-/* x_scales_stride a multiple of 4, at least ceil(steps / 4) * 4 (the bytes past     */
-/* the last step may hold anything), x_scales 4-byte aligned; x and packed 16-byte   */
-/* aligned; codes of HS_LINEAR_SWIGLU_FP8 16-byte aligned with a stride that is a    */
-/* multiple of 16. The workspace needs no preparation and holds nothing between calls. */
+/* x_scales_stride a multiple of 4, at least ceil(steps / 4) * 4 and at most 2^22     */
+/* (the bytes past the last step are read in every row, and may hold anything),      */
+/* x_scales 4-byte aligned; x and packed 16-byte aligned; codes of                   */
+/* HS_LINEAR_SWIGLU_FP8 16-byte aligned with a stride that is a multiple of 16. The  */
+/* workspace needs no preparation and holds nothing between calls.                   */
 size_t hs_linear_fp8_workspace_size(int rows, int in_features, int out_features, int epilogue,
                                     int bf16_rows);
 int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t x_scales_stride,

@@ -109,6 +109,8 @@ def test_refusals(hv):
         assert linear(rows=rows, xe=xe, epi=epi, ws=p + 8, ws_bytes=need) == -4
     assert lib.hs_linear_fp8_workspace_size(0, 4096, 4096, 0, 0) == 0
     assert lib.hs_linear_fp8_workspace_size(4, 4096, 4096, 3, 0) == 0
+    for sizes in (((1 << 20) + 1, 4096, 4096), (64, (1 << 31) - 1, 4096), (64, 4096, (1 << 31) - 1)):
+        assert lib.hs_linear_fp8_workspace_size(*sizes, 2, 1) == 0
 
     def quantize(x=p, xs=256, rows=2, k=256, c=p, cs=256, s=p, ss=2):
         return lib.hs_quantize_rows_fp8(x, xs, rows, k, c, cs, s, ss, None)
@@ -120,7 +122,7 @@ def test_refusals(hv):
         assert f(rows=0, x=None) == 0
         assert f(x=None) == f(c=None) == f(s=None) == f(rows=-1) == f(k=0) == -1
         assert f(k=248) == f(xs=248) == f(xs=260) == f(cs=248) == f(cs=260) == f(ss=1) == -4
-        assert f(x=p + 8) == f(c=p + 4) == f(rows=(1 << 22) + 1) == -4
-    assert quantize(rows=1 << 22, k=1 << 20, xs=1 << 20, cs=1 << 20, ss=1 << 13) == -4
+        assert f(x=p + 8) == f(c=p + 4) == f(rows=1 << 22) == -4
+    assert quantize(rows=(1 << 22) - 1, k=1 << 20, xs=1 << 20, cs=1 << 20, ss=1 << 13) == -4
     assert norm(w=None) == -1
     assert norm(w=p + 8) == norm(res=p + 8) == norm(rs=248) == norm(rs=260) == -4

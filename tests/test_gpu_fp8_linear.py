@@ -233,6 +233,75 @@ def test_captured_calls_share_nothing(hv, cuda):
             assert _same(beside[i], want[i])
 
 
+@pytest.mark.parametrize("rows,features", [(3, 256), (40, 256), (300, 4096), (1100, 2048),
+                                           (2048, 4096)])
+def test_swiglu_leaves_nonfinite_values_to_themselves(hv, cuda, rows, features):
+    """silu(gate) * up = 2^57 * 2^57 but for one feature whose product overflows and one with
+    a negative gate (silu(-2^57) is 0): the overflow is NaN and takes no part in the scale. A
+    row with a NaN is NaN, with the least scale."""
+    ops = hv.ops
+    codes = torch.ones(2 * features, 128)
+    codes[5] = codes[features + 5] = 448.0
+    codes[7] = -1
+    w = ops.pack_fp8(codes.to(torch.float8_e4m3fn).to(cuda),
+                     torch.ones(features // 64, 1, device=cuda))
+    xc = torch.ones(rows, 128)
+    xc[1, 99] = float("nan")
+    e = torch.full((rows, 4), 127 + 50, dtype=torch.uint8, device=cuda)
+    x = ops.Fp8Rows(xc.to(torch.float8_e4m3fn).to(cuda), e.view(torch.float8_e8m0fnu)[:, :1])
+    got = ops.linear_fp8(x, w, swiglu=True, quantize=True)
+    c, s = got.codes.float().cpu(), got.scales.float().cpu()
+    rest = [r for r in range(rows) if r != 1]
+    assert bool(c[1].isnan().all()) and bool((s[1] == 2.0 ** -126).all())
+    assert bool((s[rest] == 2.0 ** 106).all())  # 2^114 <= 448 * 2^106
+    assert bool(c[rest, 5].isnan().all()) and bool((c[rest, 7] == 0).all())
+    assert bool((c[rest][:, [j for j in range(features) if j not in (5, 7)]] == 256).all())
+
+
+def _units(gen, n, k, cuda):
+    """-1, 0 and 1, whose products are summed without rounding."""
+    return torch.randint(-1, 2, (n, k), generator=gen).to(torch.float8_e4m3fn).to(cuda)
+
+
+def _rows_of_one(codes):
+    steps = -(-codes.shape[1] // 128)
+    e = torch.full((codes.shape[0], -(-steps // 4) * 4), 127, dtype=torch.uint8,
+                   device=codes.device)
+    return e.view(torch.float8_e8m0fnu)[:, :steps]
+
+
+def _exact(x, w):
+    return (x.cpu().double() @ w.cpu().double().t()).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("k,n", [(4352, 16), (16, 2064)])
+def test_offsets_past_32_bits_of_rows(hv, cuda, k, n):
+    """2^20 rows: codes or outputs of more than 2^32 bytes."""
+    ops, gen, rows = hv.ops, torch.Generator().manual_seed(k), 1 << 20
+    codes = _units(gen, n, k, cuda)
+    w = ops.pack_fp8(codes, torch.ones(-(-n // 128), -(-k // 128), device=cuda))
+    last = _units(gen, 40, k, cuda)
+    x = torch.zeros(rows, k, dtype=torch.float8_e4m3fn, device=cuda)
+    x[-40:] = last
+    got = ops.linear_fp8(ops.Fp8Rows(x, _rows_of_one(x)), w)
+    assert torch.equal(got[-40:].cpu(), _exact(last, codes))
+    assert not bool(got[:-40].any())
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_offsets_past_32_bits_of_weights(hv, cuda, rows):
+    ops, gen, k, n = hv.ops, torch.Generator().manual_seed(rows), 4352, 1 << 20
+    codes = _units(gen, 48, k, cuda)
+    tail = ops.pack_fp8(codes, torch.ones(1, 34, device=cuda))
+    packed = torch.zeros(n // 16, 34, 2, 64, 16, dtype=torch.uint8, device=cuda)
+    packed[-3:] = tail.packed
+    w = ops.Fp8Weight(packed, torch.ones(n // 16, 34, device=cuda), n, k)
+    x = _units(gen, rows, k, cuda)
+    got = ops.linear_fp8(ops.Fp8Rows(x, _rows_of_one(x)), w)
+    assert torch.equal(got[:, -48:].cpu(), _exact(x, codes))
+    assert not bool(got[:, :-48].any())
+
+
 def test_linear_refusals(hv, cuda):
     ops = hv.ops
     w = ops.quantize_fp8(torch.ones(40, 160, device=cuda))

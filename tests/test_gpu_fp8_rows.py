@@ -137,6 +137,24 @@ def test_rmsnorm_fp8_limits(hv, cuda):
     assert bool(got.codes[3, 500].float().isnan())
 
 
+def test_offsets_past_32_bits(hv, cuda):
+    """2^20 rows of 4112: more than 2^32 codes, and 2^33 bytes of bf16."""
+    gen = torch.Generator().manual_seed(6)
+    x = torch.zeros(1 << 20, 4112, dtype=torch.bfloat16, device=cuda)
+    last = torch.randn(30, 4112, generator=gen).to(torch.bfloat16).to(cuda)
+    x[-30:] = last
+    w = torch.ones(4112, dtype=torch.bfloat16, device=cuda)
+    res = x.clone()
+    for got, want in ((hv.ops.quantize_rows_fp8(x), hv.ops.quantize_rows_fp8(last)),
+                      (hv.ops.rmsnorm_fp8(x, w, 1e-6, residual=res),
+                       hv.ops.rmsnorm_fp8(last, w, 1e-6, residual=last.clone()))):
+        for a, b in zip(got, want):
+            assert torch.equal(a[-30:].view(torch.uint8), b.view(torch.uint8))
+        assert not bool(got.codes[:-30].view(torch.uint8).any())
+        assert bool((got.scales[:-30].view(torch.uint8) == 1).all())
+    assert torch.equal(res[-30:], last + last) and not bool(res[:-30].any())
+
+
 def test_rows_refusals(hv, cuda):
     ops = hv.ops
     x = torch.zeros(3, 160, dtype=torch.bfloat16, device=cuda)
