@@ -574,6 +574,9 @@ int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t resi
 /* outputs: out[r, n] = sum_k x[r, k] * code[n, k] * scale[n / 128, k / 128], bf16   */
 /* out. The matrix unit adds 8 neighbouring products as multiples of 2^(e - 13), e   */
 /* the largest exponent among them, everything else in fp32: about 1e-4 by norm.     */
+/* Sums are kept in units of 2^17, so that any finite bf16 input, and rows in 8 bits */
+/* with scales up to 2^120, pass no infinity on the way to a result in range; the    */
+/* least a block's sum can hold is 2^-132 times its weight's scale.                  */
 /* HS_LINEAR_SWIGLU: weight [2 * out_features, in_features] gate | up, out =        */
 /* silu(gate) * up rounded once; HS_LINEAR_SWIGLU_FP8: the same product as rows in  */
 /* 8 bits (out: codes, out_scales: their exponent bytes); out_features a multiple   */
