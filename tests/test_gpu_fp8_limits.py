@@ -90,3 +90,28 @@ def test_inputs_down_to_the_least(hv, cuda, case):
     _near(got, y, tol, epilogue)
     some = xc.float().abs().amax(1) > 0  # (the smallest rows' codes may all be zeros)
     assert bool((got.abs().amax(1) > 0).cpu()[some].all()) and int(some.sum()) > rows // 4
+
+
+@pytest.mark.parametrize("rows,features,quantize", [
+    (3, 256, False), (300, 4096, False), (1100, 4096, False), (2100, 4096, False),
+    (3, 256, True), (300, 1024, True), (300, 4096, True), (1100, 4096, True)])
+def test_silu_of_far_gates(hv, cuda, rows, features, quantize):
+    """Gates from -80 to -88.7, whose exponential is near f32's largest value, times 2^120.
+    The exponent's argument is rounded to 2^-17 there (128 by 2^-24), its quotient to 2^-22."""
+    ops = hv.ops
+    j = torch.arange(features)
+    gate = torch.zeros(features, 128)
+    gate[:, 0], gate[:, 1], gate[:, 2] = -80, -(j % 9), -(j // 9 % 6) / 8
+    gate[:, 2] = torch.where(j % 9 == 8, gate[:, 2], gate[:, 2] * 1.5)
+    up = torch.zeros(features, 128)
+    up[:, 0] = 1
+    scales = torch.ones(features // 64, 1)
+    scales[features // 128:] = 2.0 ** 120
+    w = ops.pack_fp8(_codes(torch.cat([gate, up])).to(cuda), scales.to(cuda))
+    x = torch.zeros(rows, 128, dtype=torch.bfloat16, device=cuda)
+    x[:, :3] = 1
+    got = ops.linear_fp8(x, w, swiglu=True, quantize=quantize)
+    g = gate.double().sum(1)
+    y = (g * torch.sigmoid(g) * 2.0 ** 120)[None].expand(rows, features)
+    assert float(g.min()) < -88.5
+    _near(got if quantize else got.cpu(), y, y.abs() * 2.0 ** -16, "eight" if quantize else "swiglu")
