@@ -1123,6 +1123,15 @@ def _bf16_rows(t: torch.Tensor, most: int = 1 << 40) -> torch.Tensor:
     return t
 
 
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether two elements of t [rows, columns] may share an address: false where one
+    dimension's step passes all of the other."""
+    (m, n), (row, col) = t.shape, t.stride()
+    if m > 1 and n > 1:
+        return not (0 < col and row > (n - 1) * col or 0 < row and col > (m - 1) * row)
+    return m > 1 and row == 0 or n > 1 and col == 0
+
+
 def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
     """bf16 rows x [rows, K], K a multiple of 16, in 8 bits (hs_quantize_rows_fp8): for
     every 128 values of a row the smallest power of two s, at least 2^-126, with |x| <= 448
@@ -1161,8 +1170,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
         if residual.shape != shape or residual.dtype != torch.bfloat16:
             raise ValueError("residual must be bf16 with x's shape")
         row, col = residual.stride()
-        if col < 1 or M > 1 and row < H * col:
-            raise ValueError("residual is updated in place: its rows must not overlap")
+        if (col != 1 or row < H) and _overlaps(residual):
+            raise ValueError("residual is updated in place: its elements must not overlap")
         res = _bf16_rows(residual)
     out = _new_rows_fp8(x, M, H)
     if not M:
