@@ -1211,7 +1211,8 @@ def pack_fp8(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Weight:
 
 def quantize_fp8(weight: torch.Tensor) -> Fp8Weight:
     """A float weight [N, K] to e4m3: the scale of a 128 x 128 block is its largest |w|
-    over 448 (at least 2^-126), the codes are the nearest ones."""
+    over 448 (at least 2^-126), the codes are the nearest ones. NaN and infinities become NaN
+    and take no part in the scale."""
     if weight.dim() != 2 or not weight.is_floating_point() or weight.shape[0] < 1 or \
             weight.shape[1] < 1 or weight.shape[1] % 16:
         raise ValueError("weight must be a floating [N, K] tensor with K a multiple of 16")
@@ -1219,7 +1220,8 @@ def quantize_fp8(weight: torch.Tensor) -> Fp8Weight:
     nb, kb = -(-N // 128), -(-K // 128)
     w = torch.nn.functional.pad(weight.float(), (0, kb * 128 - K, 0, nb * 128 - N))
     w = w.view(nb, 128, kb, 128)
-    scales = (w.abs().amax((1, 3)) / 448).clamp_(min=2.0 ** -126)
+    w = torch.where(torch.isfinite(w), w, float("nan"))
+    scales = (w.abs().nan_to_num(nan=0.0).amax((1, 3)) / 448).clamp_(min=2.0 ** -126)
     codes = (w / scales[:, None, :, None]).clamp_(-448, 448).to(torch.float8_e4m3fn)
     return pack_fp8(codes.view(nb * 128, kb * 128)[:N, :K], scales)
 
