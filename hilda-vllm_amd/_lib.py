@@ -101,6 +101,7 @@ SIGNATURES.update({
     "hs_rmsnorm_fp8": (_i32, [_vp, _i64, _vp, _i64, _vp, _f32, _i32, _i32, _vp, _i64, _vp, _i64,
                               _vp]),
     "hs_linear_fp8_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "hs_linear_fp8_plan": (_i32, [_i32, _i32, _i32, _i32, _i32, _vp]),
     "hs_linear_fp8": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i64,
                              _vp, _i64, _vp, _sz, _vp]),
     "hs_linear": (_i32, [_vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),

@@ -1088,6 +1088,26 @@ size_t hs_linear_fp8_workspace_size(int rows, int in_features, int out_features,
   return plan_of(rows, in_features, out_features, epilogue, bf16_rows != 0).bytes;
 }
 
+int hs_linear_fp8_plan(int rows, int in_features, int out_features, int epilogue, int bf16_rows,
+                       int* plan) {
+  if (!plan || !sizes_ok(rows, in_features, out_features, epilogue)) return HS_ERR_INVALID;
+  if (!sizes_fit(rows, in_features, out_features)) return HS_ERR_UNSUPPORTED;
+  const Fp8Plan p = plan_of(rows, in_features, out_features, epilogue, bf16_rows != 0);
+  if (p.kernel == kRows) {
+    const RowsKernel k = rows_of(rows, (in_features + kStep - 1) / kStep, (out_features + 15) / 16,
+                                 epilogue != HS_LINEAR_PLAIN);
+    plan[0] = 16 * k.tiles;
+    plan[1] = 16 * k.row_tiles;
+    plan[2] = k.waves;
+  } else {
+    plan[0] = kTileTimes[p.kernel].features;
+    plan[1] = kTileTimes[p.kernel].rows;
+    plan[2] = p.kernel == k128x32 ? Tile128x32::kWaves : kBigThreads / 64;
+  }
+  plan[3] = p.split_steps;
+  return HS_OK;
+}
+
 int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t x_scales_stride,
                   const void* packed, const float* scales, int rows, int in_features,
                   int out_features, int epilogue, void* out, int64_t out_stride, void* out_scales,

@@ -592,8 +592,14 @@ int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t resi
 /* x_scales 4-byte aligned; x and packed 16-byte aligned; codes of                   */
 /* HS_LINEAR_SWIGLU_FP8 16-byte aligned with a stride that is a multiple of 16. The  */
 /* workspace needs no preparation and holds nothing between calls.                   */
+/* hs_linear_fp8_plan: what such a call launches, on the host alone: plan[0] and       */
+/* plan[1] the features (gate and up together) and rows of a workgroup, plan[2] its    */
+/* waves, plan[3] the 128-input steps that one of them adds (all, or parts joined by a */
+/* second launch). Calls with the same plan give a row the same bits in any batch.     */
 size_t hs_linear_fp8_workspace_size(int rows, int in_features, int out_features, int epilogue,
                                     int bf16_rows);
+int hs_linear_fp8_plan(int rows, int in_features, int out_features, int epilogue, int bf16_rows,
+                       int* plan);
 int hs_linear_fp8(const void* x, int64_t x_stride, const void* x_scales, int64_t x_scales_stride,
                   const void* packed, const float* scales, int rows, int in_features,
                   int out_features, int epilogue, void* out, int64_t out_stride, void* out_scales,
