@@ -1,0 +1,80 @@
+"""Every kernel for projections of rows in 8 bits, by the sizes of fp8_cases, against the same
+sums in 64 bits."""
+import pytest
+import torch
+
+import fp8_ref as ref
+from fp8_cases import CASES, ids, plan
+from test_gpu_fp8_linear import _reference, _same
+
+pytestmark = pytest.mark.gpu
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _codes(x):
+    return x.clamp(-448, 448).to(E4M3)
+
+
+class Setup:
+    """Weights, row codes and exponents of a case, on the GPU; the codes lie in wider rows and
+    the exponents in words whose other bytes are NaN."""
+
+    def __init__(self, hv, cuda, case, spread=4):
+        self.ops, (self.k, self.n, self.rows, self.epilogue) = hv.ops, case
+        k, rows, steps = self.k, self.rows, -(-self.k // 128)
+        self.gate = self.epilogue != "plain"
+        self.how = dict(swiglu=self.gate, quantize=self.epilogue == "eight")
+        gen = torch.Generator(device=cuda).manual_seed(k + self.n + rows)
+        rand = lambda *size: torch.randn(*size, generator=gen, device=cuda)  # noqa: E731
+        features = self.n * (2 if self.gate else 1)
+        self.wcodes = _codes(rand(features, k) * 100)
+        self.wscales = rand(-(-features // 128), steps).abs() * 2e-3 + 1e-5
+        self.w = hv.ops.pack_fp8(self.wcodes, self.wscales)
+        wide = torch.full((rows, k + 32), 0x7f, dtype=torch.uint8, device=cuda).view(E4M3)
+        wide[:, 16:16 + k] = _codes(rand(rows, k) * 60)
+        self.codes = wide[:, 16:16 + k]
+        self.bytes = torch.full((rows, -(-steps // 4) * 4 + 4), 255, dtype=torch.uint8, device=cuda)
+        e = torch.randint(-spread, 1, (rows, steps), generator=gen, device=cuda)
+        self.bytes[:, :steps] = (e + 120).to(torch.uint8)
+        self.steps = steps
+
+    def exponents(self):
+        return self.bytes[:, :self.steps]
+
+    def x(self):
+        return self.ops.Fp8Rows(self.codes, self.exponents().view(E8M0))
+
+    def run(self, x=None, **more):
+        return self.ops.linear_fp8(self.x() if x is None else x, self.w, **self.how, **more)
+
+    def reference(self):
+        s = torch.exp2(self.exponents().double() - 127)
+        x = ref.values(self.codes, s)
+        return _reference(x, self.wcodes, self.wscales, self.epilogue, self.n)
+
+    def check(self, got, y, tol):
+        if self.epilogue == "eight":
+            ref.check_rows(got.codes, got.scales, y.cpu(), tol.cpu())
+            return
+        err, tol = (got.double() - y).abs(), tol + 2.0 ** -8 * (y.abs() + tol)
+        assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("case", CASES, ids=ids)
+def test_every_kernel(hv, cuda, case):
+    print("fp8 kernel", case, plan(hv, *case), flush=True)
+    s = Setup(hv, cuda, case)
+    got, (y, tol) = s.run(), s.reference()
+    s.check(got, y, tol)
+    assert _same(s.run(), got)
+    if s.epilogue != "eight":  # an output off the 16-byte pieces, between others' values
+        wide = torch.full((s.rows + 1, s.n + 5), 7.0, dtype=torch.bfloat16, device=cuda)
+        out = wide[:s.rows, 3:3 + s.n]
+        assert s.run(out=out) is out and _same(out, got)
+        assert bool((wide[s.rows] == 7).all() and (wide[:, :3] == 7).all())
+        assert bool((wide[:, 3 + s.n:] == 7).all())
+    # bf16 rows: those that the codes of some others stand for
+    x = s.codes.float().mul(torch.exp2(torch.randint(-8, 9, (s.rows, 1), device=cuda).float()))
+    x = x.to(torch.bfloat16)
+    assert _same(s.run(x), s.run(s.ops.quantize_rows_fp8(x)))
