@@ -78,3 +78,28 @@ def test_every_kernel(hv, cuda, case):
     x = s.codes.float().mul(torch.exp2(torch.randint(-8, 9, (s.rows, 1), device=cuda).float()))
     x = x.to(torch.bfloat16)
     assert _same(s.run(x), s.run(s.ops.quantize_rows_fp8(x)))
+
+
+@pytest.mark.parametrize("case", CASES, ids=ids)
+def test_rows_do_not_meet_in_any_kernel(hv, cuda, case):
+    """A NaN code, or a scale that is NaN (byte 255), makes its row NaN; the least scales (bytes 0
+    and 1) make theirs less than 2^-95; the other rows keep their bits. (The bytes behind a row's
+    last scale are 255 all along.)"""
+    print("fp8 rows", case, plan(hv, *case), flush=True)
+    s = Setup(hv, cuda, case)
+    want = s.run()
+    s.codes.view(torch.uint8)[1, s.k - 3] = 0x7f
+    s.exponents()[s.rows - 1, s.steps // 2] = 255
+    s.exponents()[0] = torch.arange(s.steps, device=cuda) % 2
+    got = s.run()
+    if s.epilogue == "eight":
+        values = got.codes.float()
+        least = values[0] * got.scales[0].float().repeat_interleave(128)[:s.n]
+        kept = _same(s.ops.Fp8Rows(got.codes[2:-1], got.scales[2:-1]),
+                     s.ops.Fp8Rows(want.codes[2:-1], want.scales[2:-1]))
+        assert bool((got.scales[[1, s.rows - 1]].float() == 2.0 ** -126).all())
+    else:
+        values, least, kept = got, got[0], _same(got[2:-1], want[2:-1])
+    assert kept
+    assert bool(values[[1, s.rows - 1]].isnan().all())
+    assert bool((least.abs() < 2.0 ** -95).all())
