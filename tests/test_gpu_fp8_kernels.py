@@ -103,3 +103,36 @@ def test_rows_do_not_meet_in_any_kernel(hv, cuda, case):
     assert kept
     assert bool(values[[1, s.rows - 1]].isnan().all())
     assert bool((least.abs() < 2.0 ** -95).all())
+
+
+_BATCHES = (1, 3, 8, 9, 16, 17, 24, 32, 33, 48, 64, 65, 96, 129, 200, 256, 257, 300, 400, 512, 513, 640,
+            777, 1024, 1100, 1500, 2051)
+
+
+@pytest.mark.parametrize("k,n,epilogue", [
+    (1040, 528, "plain"), (1040, 4099, "plain"), (12288, 4096, "plain"), (2064, 8200, "plain"),
+    (1040, 2064, "swiglu"), (4096, 4112, "swiglu"), (1040, 2064, "eight"), (4096, 4112, "eight")])
+def test_a_row_in_many_batches(hv, cuda, k, n, epilogue):
+    """All rows of every batch are within their bounds, and a row has the same bits in every batch
+    of one plan, wherever it lies in it: first and last rows are shared between batches."""
+    print("fp8 batches", k, n, epilogue, flush=True)
+    s = Setup(hv, cuda, (k, n, _BATCHES[-1], epilogue))
+    y, tol = s.reference()
+    plans = {}
+    for m in _BATCHES:
+        last = slice(s.rows - m, s.rows)
+        first = s.run(s.ops.Fp8Rows(s.codes[:m], s.exponents().view(E8M0)[:m]))
+        other = s.run(s.ops.Fp8Rows(s.codes[last], s.exponents().view(E8M0)[last]))
+        s.check(first, y[:m], tol[:m])
+        s.check(other, y[last], tol[last])
+        plans.setdefault(plan(hv, k, n, m, epilogue), []).append((m, first, other))
+    part = (lambda t, at: s.ops.Fp8Rows(t.codes[at], t.scales[at])) if epilogue == "eight" else \
+        (lambda t, at: t[at])
+    for same in plans.values():
+        for (m, first, other), (more, longer, late) in zip(same, same[1:]):
+            assert _same(part(longer, slice(0, m)), first)
+            assert _same(part(late, slice(more - m, more)), other)
+            if more + m > s.rows:  # rows that the first `more` and the last m share
+                both = more + m - s.rows
+                assert _same(part(longer, slice(more - both, more)), part(other, slice(0, both)))
+    assert len(plans) >= 3
