@@ -136,3 +136,52 @@ def test_a_row_in_many_batches(hv, cuda, k, n, epilogue):
                 both = more + m - s.rows
                 assert _same(part(longer, slice(more - both, more)), part(other, slice(0, both)))
     assert len(plans) >= 3
+
+
+# calls that split their steps, and so have a workspace of sums, or one of codes beside it
+_SPLITS = [(12288, 4096, 64, "plain"), (12288, 1030, 300, "plain"), (12288, 1024, 128, "swiglu"),
+           (6160, 2080, 66, "eight"), (12288, 4096, 64, "plain")]
+
+
+def test_captured_splits_share_nothing(hv, cuda):
+    """Graphs of calls that split their steps, of rows in 8 bits and of bf16 rows, replayed at
+    once on two streams over and over with new inputs, with eager calls on both between them."""
+    calls = []
+    for case in _SPLITS:
+        p = plan(hv, *case)
+        assert p[3] < -(-case[0] // 128), (case, p)
+        s = Setup(hv, cuda, case)
+        raw = s.codes.view(torch.uint8)
+        sets = [raw.clone(), raw.flip(0), raw.roll(3, 0)]
+        bf16 = s.codes.to(torch.bfloat16)
+        graphs = []
+        for x in (s.x(), bf16):
+            s.run(x)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                y = s.run(x)
+            graphs.append((g, y))
+        calls.append((s, sets, bf16, graphs))
+    side = torch.cuda.Stream()
+    whole = lambda y: y if isinstance(y, torch.Tensor) else y.codes.view(torch.uint8)  # noqa: E731
+    for turn in range(4):
+        want = []
+        for s, sets, bf16, graphs in calls:
+            s.codes.view(torch.uint8).copy_(sets[turn % 3])
+            bf16.copy_(s.codes)
+            want.append([s.run(), s.run(bf16)])
+            for _, y in graphs:
+                whole(y).zero_()
+        torch.cuda.synchronize()
+        beside, eager = [], []
+        for s, _, bf16, graphs in calls:
+            graphs[0][0].replay()
+            with torch.cuda.stream(side):
+                graphs[1][0].replay()
+                beside.append([s.run(), s.run(bf16)])
+            eager.append([s.run(bf16), s.run()])
+        torch.cuda.synchronize()
+        for (s, _, _, graphs), w, b, e in zip(calls, want, beside, eager):
+            assert _same(graphs[0][1], w[0]) and _same(graphs[1][1], w[1])
+            assert _same(b[0], w[0]) and _same(b[1], w[1])
+            assert _same(e[0], w[1]) and _same(e[1], w[0])
