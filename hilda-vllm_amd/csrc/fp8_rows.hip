@@ -72,6 +72,21 @@ __device__ __forceinline__ float row_sum(float v, float* s_sum) {
   return v;
 }
 
+// A row whose sum of squares passes f32's range (4096 values of 2.9e17) is summed once more in
+// these units: 2^24 values of up to 2^128 stay within it then, and what they lose are values far
+// below the row's root mean square.
+constexpr float kFar = 0x1p-80f;
+
+// 1 / the row's root mean square, given its sum of squares; where that is an infinity, `squares`
+// gives a thread's share in units of kFar. (The least such quotient, 2^-128, has 22 bits.)
+template <int T, class F>
+__device__ __forceinline__ float row_inverse(float sum, const NormArgs& a, float* s_sum,
+                                             F squares) {
+  if (sum != __builtin_inff()) return rsqrtf(sum / (float)a.hidden + a.eps);
+  if constexpr (T > 64) __syncthreads();  // all threads of a row are here; s_sum has been read
+  return rsqrtf(row_sum<T>(squares(), s_sum) / (float)a.hidden) * kFar;
+}
+
 __device__ __forceinline__ uint4 load8(const uint16_t* p, int k, bool live) {
   return live ? *reinterpret_cast<const uint4*>(p + k) : make_uint4(0, 0, 0, 0);
 }
@@ -128,7 +143,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_fp8(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss += h[c][i] * h[c][i];
   }
-  const float inv = rsqrtf(row_sum<T>(ss, s_sum) / (float)a.hidden + a.eps);
+  const float inv = row_inverse<T>(row_sum<T>(ss, s_sum), a, s_sum, [&] {
+    float far = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) far += h[c][i] * kFar * (h[c][i] * kFar);
+    return far;
+  });
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int k = 8 * (c * T + tid);
@@ -153,14 +175,18 @@ __global__ __launch_bounds__(kLongThreads) void k_rmsnorm_fp8_long(NormArgs a) {
       for (int i = 0; i < 8; ++i) h[i] += r[i];
     }
   };
-  float ss = 0.0f;
-  for (int k = 8 * threadIdx.x; k < a.hidden; k += 8 * kLongThreads) {
-    float h[8];
-    load(k, h);
+  auto squares = [&](float unit) {
+    float ss = 0.0f;
+    for (int k = 8 * threadIdx.x; k < a.hidden; k += 8 * kLongThreads) {
+      float h[8];
+      load(k, h);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += h[i] * h[i];
-  }
-  const float inv = rsqrtf(row_sum<kLongThreads>(ss, s_sum) / (float)a.hidden + a.eps);
+      for (int i = 0; i < 8; ++i) ss += h[i] * unit * (h[i] * unit);
+    }
+    return ss;
+  };
+  const float inv = row_inverse<kLongThreads>(row_sum<kLongThreads>(squares(1.0f), s_sum), a,
+                                              s_sum, [&] { return squares(kFar); });
   const int padded = (a.hidden + kFp8Group - 1) / kFp8Group * kFp8Group;
   for (int k = 8 * threadIdx.x; k < padded; k += 8 * kLongThreads) {  // whole groups of lanes
     float h[8];

@@ -560,7 +560,8 @@ int hs_linear_int4(const void* x, int64_t x_stride, const void* packed, const vo
 /* multiple of 8, of codes of 8; x 16-byte, codes 8-byte aligned.                    */
 /* hs_quantize_rows_fp8: of bf16 rows x.                                            */
 /* hs_rmsnorm_fp8: of h * rsqrt(mean(h^2) + eps) * weight in fp32, h = x (+         */
-/* residual); with residual != NULL the residual row is replaced by bf16(h) (its    */
+/* residual), also where its squares' sum passes fp32's range;                       */
+/* with residual != NULL the residual row is replaced by bf16(h) (its               */
 /* stride a multiple of 8, it and weight bf16 and 16-byte aligned; x and residual    */
 /* are the same rows or do not overlap).                                            */
 int hs_quantize_rows_fp8(const void* x, int64_t x_stride, int rows, int width, void* codes,
