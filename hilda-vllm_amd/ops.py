@@ -1298,6 +1298,7 @@ def linear_fp8(x, weight: Fp8Weight, *, swiglu: bool = False, quantize: bool = F
         ws = packed.new_empty(nbytes) if nbytes else None
         _call(dev, "hs_linear_fp8", codes.data_ptr(), codes.stride(0),
               None if exps is None else exps.data_ptr(), 0 if exps is None else exps.stride(0),
-              packed.data_ptr(), scales.data_ptr(), M, K, N, epi, out.data_ptr(), out.stride(0),
+              packed.data_ptr(), scales.data_ptr(), M, K, N, epi, out.data_ptr(),
+              out.stride(0) if M > 1 else N,  # (a single row's may be anything)
               exps_out, exps_row, ws.data_ptr() if nbytes else None, nbytes)
     return rows if quantize else out

@@ -115,3 +115,17 @@ def test_silu_of_far_gates(hv, cuda, rows, features, quantize):
     y = (g * torch.sigmoid(g) * 2.0 ** 120)[None].expand(rows, features)
     assert float(g.min()) < -88.5
     _near(got if quantize else got.cpu(), y, y.abs() * 2.0 ** -16, "eight" if quantize else "swiglu")
+
+
+def test_a_single_row_of_any_stride(hv, cuda):
+    """One row's stride says nothing: an output whose rows would overlap if there were more."""
+    gen = torch.Generator().manual_seed(1)
+    w = hv.ops.quantize_fp8(torch.randn(200, 256, generator=gen).to(cuda))
+    x = torch.randn(1, 256, generator=gen).to(torch.bfloat16).to(cuda)
+    want = hv.ops.linear_fp8(x, w)
+    for out in (torch.empty(200, dtype=torch.bfloat16, device=cuda)[:, None].t(),
+                torch.empty(200, dtype=torch.bfloat16, device=cuda).as_strided((1, 200), (0, 1))):
+        assert hv.ops.linear_fp8(x, w, out=out) is out and torch.equal(out, want)
+    two = torch.empty(400, dtype=torch.bfloat16, device=cuda).as_strided((2, 200), (100, 1))
+    with pytest.raises(RuntimeError):  # rows that do overlap
+        hv.ops.linear_fp8(x.expand(2, 256), w, out=two)
