@@ -1253,11 +1253,11 @@ def linear_fp8(x, weight: Fp8Weight, *, swiglu: bool = False, quantize: bool = F
     """linear with rows and weight in 8 bits (hs_linear_fp8; weight an Fp8Weight or what
     has its fields): x Fp8Rows, or [rows, K] bf16, which goes to 8 bits first as in
     quantize_rows_fp8; up to 2^20 rows -> [rows, N] bf16. Sums are fp32 but for 8 neighbouring
-    products, which keep 13 bits below the largest of them (about 1e-4 by norm); finite
-    inputs may be of any size (rows in 8 bits: with scales up to 2^120). With
-    swiglu=True the weight is [2F, K] (gate | up), F a multiple of 16, and the result
-    silu(gate) * up [rows, F]; with quantize=True beside it that result as Fp8Rows, rounded
-    from fp32 once."""
+    products, which keep 13 bits below the largest of them (up to 1e-4 by norm); finite
+    inputs may be of any size (rows in 8 bits: with scales up to 2^120). out must not overlap
+    the inputs. With swiglu=True the weight is [2F, K] (gate | up), F a multiple of 16, and
+    the result silu(gate) * up [rows, F]; with quantize=True beside it that result as
+    Fp8Rows, rounded from fp32 once."""
     packed, scales, features = weight.packed, weight.scales, weight.out_features
     if isinstance(x, torch.Tensor):
         dev = _need_cuda(x, packed, scales, out)

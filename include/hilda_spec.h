@@ -574,7 +574,8 @@ int hs_rmsnorm_fp8(const void* x, int64_t x_stride, void* residual, int64_t resi
 /* x 128 (no counterpart in the reference), up to 2^20 rows, 2^22 inputs and 2^24    */
 /* outputs: out[r, n] = sum_k x[r, k] * code[n, k] * scale[n / 128, k / 128], bf16   */
 /* out. The matrix unit adds 8 neighbouring products as multiples of 2^(e - 13), e   */
-/* the largest exponent among them, everything else in fp32: about 1e-4 by norm.     */
+/* the largest exponent among them, everything else in fp32: up to 1e-4 by norm. out */
+/* must not overlap the inputs.                                                      */
 /* Sums are kept in units of 2^17, so that any finite bf16 input, and rows in 8 bits */
 /* with scales up to 2^120, pass no infinity on the way to a result in range; the    */
 /* least a block's sum can hold is 2^-132 times its weight's scale.                  */

@@ -105,8 +105,8 @@ def test_rows_do_not_meet_in_any_kernel(hv, cuda, case):
     assert bool((least.abs() < 2.0 ** -95).all())
 
 
-_BATCHES = (1, 3, 8, 9, 16, 17, 24, 32, 33, 48, 64, 65, 96, 129, 200, 256, 257, 300, 400, 512, 513, 640,
-            777, 1024, 1100, 1500, 2051)
+_BATCHES = (1, 3, 8, 9, 16, 17, 24, 32, 33, 48, 64, 65, 96, 129, 200, 256, 257, 300, 400, 512, 513,
+            640, 777, 1024, 1100, 1500, 2051)
 
 
 @pytest.mark.parametrize("k,n,epilogue", [

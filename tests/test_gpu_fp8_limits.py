@@ -81,7 +81,8 @@ def test_inputs_down_to_the_least(hv, cuda, case):
     codes = _codes(torch.randn(n, k, generator=gen) * 100)
     scales = torch.rand(-(-n // 128), -(-k // 128), generator=gen) * 2.0 ** 20
     w = hv.ops.pack_fp8(codes.to(cuda), scales.to(cuda))
-    xc = _codes(torch.randn(rows, k, generator=gen) * torch.exp2(torch.rand(rows, 1, generator=gen) * -12))
+    xc = torch.randn(rows, k, generator=gen)
+    xc = _codes(xc * torch.exp2(torch.rand(rows, 1, generator=gen) * -12))
     xs = torch.randint(1, 12, (rows, -(-k // 128)), generator=gen).to(torch.uint8)
     xs = xs.view(torch.float8_e8m0fnu)
     y, tol = _reference(ref.values(xc, xs).to(cuda), codes.to(cuda), scales.to(cuda), epilogue, n)
@@ -114,7 +115,8 @@ def test_silu_of_far_gates(hv, cuda, rows, features, quantize):
     g = gate.double().sum(1)
     y = (g * torch.sigmoid(g) * 2.0 ** 120)[None].expand(rows, features)
     assert float(g.min()) < -88.5
-    _near(got if quantize else got.cpu(), y, y.abs() * 2.0 ** -16, "eight" if quantize else "swiglu")
+    epilogue = "eight" if quantize else "swiglu"
+    _near(got if quantize else got.cpu(), y, y.abs() * 2.0 ** -16, epilogue)
 
 
 def test_a_single_row_of_any_stride(hv, cuda):
