@@ -151,8 +151,8 @@ __device__ __forceinline__ i32x8_t row_codes(const uint4 (&raw)[4], uint32_t& by
 // RT * 16 rows a workgroup. W: its waves, which share out the steps of its TN weight tiles
 // (with SwiGLU half of them gate and half up tiles) and join their sums in LDS. kBf16: the
 // rows are bf16 and go to 8 bits here, in every workgroup. Bound by the weights' stream: 16
-// rows of 4096 by 151936 features 104 us (6.0 TB/s), by 2 x 12288 features 18.8 us (5.4 TB/s),
-// one row by 4096 features 5.6 us, of which the launch's start and end are 2.
+// rows of 4096 by 151936 features 105 us (5.9 TB/s), by 2 x 12288 features 18.8 us (5.4 TB/s),
+// one row by 4096 features 5.7 us, of which the launch's start and end are 2.
 template <int W, int TN, int RT, bool kGate, bool kBf16>
 __global__ __launch_bounds__(64 * W) void k_fp8_rows(Fp8Args a) {
   constexpr int kOut = kGate ? TN / 2 : TN;
@@ -467,7 +467,7 @@ __device__ __forceinline__ float uniform(float v) {
 // 2048 cycles of the matrix unit, beside 256 KB to and from LDS (half of its 256 bytes a cycle)
 // and 64 KB from L2 (half of a CU's 64 bytes a cycle). Measured are 2300 to 2500. 4096 rows of
 // 4096 by 2 x 12288 features with 8-bit SwiGLU take 342 to 359 us among others (2300 to 2410
-// TFLOP/s; in a trace 384, 349 at least), of which the first loads are 26 and the ends 28 (the
+// TFLOP/s; in two traces 384 and 407), of which the first loads are 26 and the ends 28 (the
 // exponential and the quotient); 325 us if all operands are zeros, for the card's power sets the
 // clock.
 template <int kEpilogue>
@@ -686,7 +686,7 @@ struct Tile {
 // unit and 1000 in all, with some 107 instructions a wave), and by the card's power: with all CUs
 // at work the clock falls from 2.4 to 1.9 GHz, zeros instead of data take a fifth less time, and
 // 89 instructions a step make a lone workgroup 9% faster, all of them 2% at best. 531 rows of
-// 4096 by 6144 features 24.0 us (240 workgroups), 64 rows of 12288 by 4096 features 13.1 us and
+// 4096 by 6144 features 23.9 us (240 workgroups), 64 rows of 12288 by 4096 features 12.9 us and
 // 3.7 for the join.
 template <int kEpilogue, class T>
 __global__ __launch_bounds__(T::kThreads, 2) void k_fp8_tile(Fp8Args a) {
